@@ -15,7 +15,8 @@
  *   - Return 0 on success or a negative VQ_ERR_* code; vq_last_error() gives a
  *     thread-local message.  No C++ exception crosses this boundary.
  *   - Calls only enqueue work on `stream`: they never synchronise (except
- *     vq_device_error) and never allocate; scratch space is caller-provided.
+ *     vq_device_error) and never allocate device memory; scratch space is
+ *     caller-provided.
  *   - Thread-safe for distinct streams.  The one process-wide state is the
  *     pair of SM reserves (vq_set_gategrad_sm_reserve, vq_set_gemm_sm_reserve):
  *     read when a GEMM is launched, they set how many SMs its persistent grid
@@ -50,7 +51,8 @@ int vq_format_info(int ggml_type, int* block_elems /* host */, int* block_bytes 
 
 /* Synchronise `stream`, then return and clear the device error word in *code
  * (host): 0 = none; (1 << 16 | where) = an mbarrier wait gave up after its
- * time limit; (2 << 16) = a kernel met an unknown format. */
+ * time limit; (2 << 16) = a kernel met an unknown format; (4 << 16 | where) =
+ * a lookup met a token id outside its table. */
 int vq_device_error(void* stream, int* code /* host */);
 
 /* K0 -- bit-exact dequantisation of one packed candidate into float32
@@ -321,6 +323,68 @@ int vq_swiglu_fwd(const void* gate, int64_t ldg, const void* up, int64_t ldu, in
 /* dgate = dy * up * silu'(gate), dup = dy * silu(gate); both outputs share ldo. */
 int vq_swiglu_bwd(const void* gate, int64_t ldg, const void* up, int64_t ldu, const void* dy, int64_t lddy, int64_t rows,
                   int64_t F, void* dgate, void* dup, int64_t ldo, void* stream);
+
+/* Norm of every query head of q [B, S, Hq, D] and key head of k [B, S, Hk, D]
+ * with the rotation of its position in the same pass:
+ *   y = x * rsqrt(mean(x^2) + eps) * (weight_offset + weight), per head of D,
+ * then the first R values of a head turned in pairs (j, j + R / 2) by cos / sin
+ * [B, S, R], the rest left as they are.  HOST stride arrays as for vq_rope
+ * ({b, s, h} and {b, s}, elements, multiples of 8); D and R multiples of 16,
+ * R <= D <= 512.  dtype of heads and outputs: 0 = float32, 1 = bfloat16,
+ * 2 = float16; weights and tables are of that type, or float32 when
+ * weight_f32 / cs_f32 is nonzero.  fp32 arithmetic, one rounding; outputs are
+ * contiguous [B, S, H, D].  Replaces q_norm / k_norm followed by
+ * apply_rotary_pos_emb (transformers models/qwen3/modeling_qwen3.py). */
+int vq_qk_norm_rope_fwd(const void* q, const int64_t* q_strides, int64_t Hq, const void* k, const int64_t* k_strides,
+                        int64_t Hk, const void* q_weight, const void* k_weight, int weight_f32, const void* cos,
+                        const void* sin, const int64_t* cs_strides, int cs_f32, int64_t B, int64_t S, int64_t D,
+                        int64_t R, float eps, float weight_offset, int dtype, void* q_out, void* k_out, void* stream);
+
+/* Its backward: dq, dk (contiguous) and, where dq_weight / dk_weight is not
+ * NULL, the weights' gradients (of the weights' type), summed over all heads
+ * and positions in a fixed order; those need `workspace`
+ * (vq_qk_norm_rope_workspace_bytes(D), 16-byte aligned). */
+size_t vq_qk_norm_rope_workspace_bytes(int64_t D);
+int vq_qk_norm_rope_bwd(const void* gq, const int64_t* gq_strides, const void* gk, const int64_t* gk_strides,
+                        const void* q, const int64_t* q_strides, int64_t Hq, const void* k, const int64_t* k_strides,
+                        int64_t Hk, const void* q_weight, const void* k_weight, int weight_f32, const void* cos,
+                        const void* sin, const int64_t* cs_strides, int cs_f32, int64_t B, int64_t S, int64_t D,
+                        int64_t R, float eps, float weight_offset, int dtype, void* dq, void* dk, void* dq_weight,
+                        void* dk_weight, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- gated embedding ----
+ * out[t, :cols] = bf16(scale * sum_k probs[k] * W_k[ids[t] - vocab_start, :cols]) for T token ids (int64, or
+ * int32 when ids_i32), W_k the packed candidates of a table of `rows` rows of padded_cols weights.  An id outside
+ * [vocab_start, vocab_start + rows) gives a row of zeros (a token of another vocabulary shard); with `strict` it
+ * also sets the device error word (4 << 16 | 30).  For scale 1 the rows are vq_mix's bit for bit.  Replaces the
+ * gather, decode and mixture of voodoo_quant/layers.py:669-742 (_MixedEmbeddingRowFunctionLazy) and Q8Embedding's. */
+int vq_embed_mix(int K, const int* types, const void* const* blocks, const float* probs, const void* ids, int ids_i32,
+                 int64_t T, int64_t vocab_start, int64_t rows, int64_t padded_cols, int64_t cols, float scale, int strict,
+                 void* out, int64_t ldo, void* stream);
+
+/* Stable sort of the tokens by their row: keys[i] = row of the i-th token in ascending order (`rows` for ids of
+ * other shards, which come last), order[i] = its position.  keys_tmp / order_tmp: T ints each of scratch. */
+int vq_token_sort(const void* ids, int ids_i32, int64_t T, int64_t vocab_start, int64_t rows, int* keys, int* order,
+                  int* keys_tmp, int* order_tmp, void* stream);
+
+/* grad[k] = scale * sum_t <dy[t], W_k[ids[t] - vocab_start]> over the ids of this table (dy_dtype 0 = float32,
+ * 1 = bfloat16, 2 = float16): the rows of dy of equal tokens are summed first, so every distinct row is decoded
+ * once.  Sums over rows are held in 64 bits and joined in a fixed order.  `workspace`:
+ * vq_embed_gategrad_workspace_bytes(T, K), 16-byte aligned. */
+size_t vq_embed_gategrad_workspace_bytes(int64_t T, int K);
+int vq_embed_gategrad(int K, const int* types, const void* const* blocks, const void* ids, int ids_i32, int64_t T,
+                      int64_t vocab_start, int64_t rows, int64_t padded_cols, int64_t cols, float scale, const void* dy,
+                      int64_t lddy, int dy_dtype, void* workspace, size_t workspace_bytes, float* grad, void* stream);
+
+/* ---- global norm and clipping ----
+ * norm[0] = sqrt(sum of squares) (or, with norm_inf, the largest magnitude) over n contiguous tensors (HOST arrays:
+ * device pointers, element counts, dtypes 0 = float32, 1 = bfloat16, 2 = float16), and every value times
+ * min(1, max_norm / (norm + 1e-6)) in place.  max_norm = infinity only takes the norm.  Tensors of no elements are
+ * skipped; tensors that share memory are refused.  Replaces torch.nn.utils.clip_grad_norm_ in
+ * voodoo_quant/training/trainer.py:2607-2616.  `workspace`: vq_clip_grad_norm_workspace_bytes(n), 8-byte aligned. */
+size_t vq_clip_grad_norm_workspace_bytes(int n);
+int vq_clip_grad_norm(int n, const void* const* ptrs, const int64_t* numel, const int* dtypes, float max_norm,
+                      int norm_inf, void* workspace, size_t workspace_bytes, float* norm, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,293 @@
+// Global norm of many gradients and their clipping in place (HBM-bandwidth
+// bound; for a few hundred tensors of a few values, launch bound).
+//
+//   norm = sqrt(sum over tensors of sum g^2)  or  max |g|
+//   g   *= min(1, max_norm / (norm + 1e-6))
+//
+// Pass 1 leaves one 64-bit partial per block; pass 2 joins the partials in
+// every block in the same order, so the result does not depend on which
+// block ends first, and scales.  The tensors come as kernel parameters: no
+// copy of a descriptor table to the device, and a captured graph holds its
+// own.  A tensor is walked in chunks of 16 KB of the address range, so vector
+// loads are aligned whatever the tensor's first address is.
+#pragma once
+
+#include "common.cuh"
+
+namespace vq {
+namespace clip {
+
+constexpr int kThreads = 256;
+constexpr int kChunkBytes = 16384;  // 4 vectors of 16 bytes per thread
+constexpr int kVecs = kChunkBytes / (16 * kThreads);
+constexpr int kBlocksPerSm = 4;
+constexpr int kSmallThreads = 1024;
+constexpr int kMaxBlocks = 1024;  // of one launch: the partials it leaves
+
+enum DType : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
+
+// The parameter space of a launch is 32764 bytes; the short table serves the
+// usual few hundred tensors without copying all of it on every launch.
+constexpr int kShortTable = 240;
+constexpr int kLongTable = 1536;
+
+template <int N>
+struct Table {
+  uintptr_t ptr[N];    // first byte
+  long long bytes[N];  // of the tensor
+  int first_chunk[N];  // chunks of the tensors before it
+  uint8_t dtype[N / 8 * 8 + 8];
+  int n;
+  int chunks;  // in all
+};
+
+__device__ __forceinline__ int esize(int dtype) { return dtype == kF32 ? 4 : 2; }
+
+// Values of a 16-byte vector (8 of 16 bits; 4 of 32).
+__device__ __forceinline__ void unpack(const uint4& v, int dtype, float (&f)[8], int& n) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  n = dtype == kF32 ? 4 : 8;
+  if (dtype == kF32) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[i] = __uint_as_float(w[i]);
+      f[4 + i] = 0.f;
+    }
+  } else if (dtype == kBF16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[2 * i] = t.x;
+      f[2 * i + 1] = t.y;
+    }
+  }
+}
+
+__device__ __forceinline__ float load_one(uintptr_t p, int dtype) {
+  if (dtype == kF32) return *reinterpret_cast<const float*>(p);
+  if (dtype == kBF16) return __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(p));
+  return __half2float(*reinterpret_cast<const __half*>(p));
+}
+
+__device__ __forceinline__ void store_one(uintptr_t p, int dtype, float v) {
+  if (dtype == kF32)
+    *reinterpret_cast<float*>(p) = v;
+  else if (dtype == kBF16)
+    *reinterpret_cast<__nv_bfloat16*>(p) = __float2bfloat16_rn(v);
+  else
+    *reinterpret_cast<__half*>(p) = __float2half_rn(v);
+}
+
+__device__ __forceinline__ uint4 scale_vec(const uint4& v, int dtype, float s) {
+  float f[8];
+  int n;
+  unpack(v, dtype, f, n);
+  uint4 r;
+  uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+  if (dtype == kF32) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(f[i] * s);
+  } else if (dtype == kBF16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i] * s, f[2 * i + 1] * s);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 h = __floats2half2_rn(f[2 * i] * s, f[2 * i + 1] * s);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  return r;
+}
+
+// Joins one value into a partial: the sum of squares, or the largest
+// magnitude with a NaN kept.
+template <bool kMax>
+__device__ __forceinline__ double join(double acc, double v) {
+  if (!kMax) return acc + v;
+  return (acc > v || acc != acc) ? acc : v;
+}
+
+template <bool kMax>
+__device__ __forceinline__ double one(float f) {
+  return kMax ? static_cast<double>(fabsf(f)) : static_cast<double>(f) * static_cast<double>(f);
+}
+
+// A vector's share.  The squares of a vector are summed in fp32, which holds
+// them to 2^-22, and joined in 64 bits; where that sum leaves the range that
+// fp32 squares keep their precision in, it is taken in 64 bits instead.
+template <bool kMax>
+__device__ __forceinline__ double of_vec(const uint4& v, int dtype) {
+  float f[8];
+  int n;
+  unpack(v, dtype, f, n);
+  if (kMax) {
+    double m = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = join<true>(m, static_cast<double>(fabsf(f[i])));
+    return m;
+  }
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s = fmaf(f[i], f[i], s);
+  if (s > 1e-26f && s < 1e37f) return static_cast<double>(s);
+  double d = 0.0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) d += static_cast<double>(f[i]) * static_cast<double>(f[i]);
+  return d;
+}
+
+// Sum (or maximum) over the block in a fixed order; every thread gets it.
+template <bool kMax>
+__device__ __forceinline__ double block_join(double v, double* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = join<kMax>(v, __shfl_down_sync(0xffffffffu, v, o));
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  double t = red[0];
+  for (int w = 1; w < static_cast<int>(blockDim.x) / 32; ++w) t = join<kMax>(t, red[w]);
+  return t;
+}
+
+template <int N>
+__device__ __forceinline__ int tensor_of(const Table<N>& tab, int chunk) {
+  int lo = 0, hi = tab.n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (tab.first_chunk[mid] <= chunk)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+
+// Address range [b, e) of a chunk, its tensor's type, and the vectors' base.
+struct Chunk {
+  uintptr_t base, b, e;
+  int dtype;
+};
+
+template <int N>
+__device__ __forceinline__ Chunk chunk_at(const Table<N>& tab, int chunk) {
+  const int t = tensor_of(tab, chunk);
+  const uintptr_t p = tab.ptr[t], end = p + static_cast<uintptr_t>(tab.bytes[t]);
+  Chunk c;
+  c.base = (p & ~uintptr_t(15)) + static_cast<uintptr_t>(chunk - tab.first_chunk[t]) * kChunkBytes;
+  c.b = c.base > p ? c.base : p;
+  c.e = c.base + kChunkBytes < end ? c.base + kChunkBytes : end;
+  c.dtype = tab.dtype[t];
+  return c;
+}
+
+__device__ __forceinline__ float clip_scale(double total, bool is_max, float max_norm, float* norm) {
+  const float nf = static_cast<float>(is_max ? total : sqrt(total));
+  *norm = nf;
+  const float s = max_norm / (nf + 1e-6f);
+  return s < 1.f || s != s ? s : 1.f;
+}
+
+template <int N, bool kMax>
+__global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ Table<N> tab,
+                                                        double* __restrict__ partials) {
+  __shared__ double red[kThreads / 32];
+  double acc = 0.0;
+  for (int chunk = blockIdx.x; chunk < tab.chunks; chunk += gridDim.x) {
+    const Chunk c = chunk_at(tab, chunk);
+    uint4 v[kVecs];
+    bool whole[kVecs];
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) {
+      const uintptr_t a = c.base + 16 * (threadIdx.x + j * kThreads);
+      whole[j] = a >= c.b && a + 16 <= c.e;
+      v[j] = whole[j] ? *reinterpret_cast<const uint4*>(a) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) {
+      if (whole[j]) {
+        acc = join<kMax>(acc, of_vec<kMax>(v[j], c.dtype));
+      } else {
+        const uintptr_t a = c.base + 16 * (threadIdx.x + j * kThreads);
+        const int es = esize(c.dtype);
+        for (uintptr_t e = a; e < a + 16; e += es)
+          if (e >= c.b && e + es <= c.e) acc = join<kMax>(acc, one<kMax>(load_one(e, c.dtype)));
+      }
+    }
+  }
+  acc = block_join<kMax>(acc, red);
+  if (threadIdx.x == 0) partials[blockIdx.x] = acc;
+}
+
+// Walks the chunks from the last to the first: what pass 1 read last is
+// still in L2.
+template <int N, bool kMax>
+__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ Table<N> tab,
+                                                         const double* __restrict__ partials, int num_partials,
+                                                         float max_norm, bool scale, float* __restrict__ norm_out) {
+  __shared__ double red[kThreads / 32];
+  double acc = 0.0;
+  for (int i = threadIdx.x; i < num_partials; i += kThreads) acc = join<kMax>(acc, partials[i]);
+  float norm;
+  const float s = clip_scale(block_join<kMax>(acc, red), kMax, max_norm, &norm);
+  if (blockIdx.x == 0 && threadIdx.x == 0 && norm_out != nullptr) *norm_out = norm;
+  if (!scale || s == 1.f) return;  // nothing changes
+  for (int chunk = tab.chunks - 1 - static_cast<int>(blockIdx.x); chunk >= 0; chunk -= gridDim.x) {
+    const Chunk c = chunk_at(tab, chunk);
+    uint4 v[kVecs];
+    bool whole[kVecs];
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) {
+      const uintptr_t a = c.base + 16 * (threadIdx.x + j * kThreads);
+      whole[j] = a >= c.b && a + 16 <= c.e;
+      v[j] = whole[j] ? *reinterpret_cast<const uint4*>(a) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) {
+      const uintptr_t a = c.base + 16 * (threadIdx.x + j * kThreads);
+      if (whole[j]) {
+        *reinterpret_cast<uint4*>(a) = scale_vec(v[j], c.dtype, s);
+      } else {
+        const int es = esize(c.dtype);
+        for (uintptr_t e = a; e < a + 16; e += es)
+          if (e >= c.b && e + es <= c.e) store_one(e, c.dtype, load_one(e, c.dtype) * s);
+      }
+    }
+  }
+}
+
+// Few values in all: one block takes the norm and scales, in one launch.  A
+// warp per tensor, since such tensors (a layer's gates) hold a few values.
+template <int N, bool kMax>
+__global__ void __launch_bounds__(kSmallThreads) small_kernel(const __grid_constant__ Table<N> tab, float max_norm,
+                                                              bool scale, float* __restrict__ norm_out) {
+  __shared__ double red[kSmallThreads / 32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  double acc = 0.0;
+  for (int t = warp; t < tab.n; t += kSmallThreads / 32) {
+    const int dt = tab.dtype[t], es = esize(dt);
+    const uintptr_t e = tab.ptr[t] + static_cast<uintptr_t>(tab.bytes[t]);
+    for (uintptr_t a = tab.ptr[t] + lane * es; a < e; a += 32 * es) acc = join<kMax>(acc, one<kMax>(load_one(a, dt)));
+  }
+  float norm;
+  const float s = clip_scale(block_join<kMax>(acc, red), kMax, max_norm, &norm);
+  if (threadIdx.x == 0 && norm_out != nullptr) *norm_out = norm;
+  if (!scale || s == 1.f) return;
+  for (int t = warp; t < tab.n; t += kSmallThreads / 32) {
+    const int dt = tab.dtype[t], es = esize(dt);
+    const uintptr_t e = tab.ptr[t] + static_cast<uintptr_t>(tab.bytes[t]);
+    for (uintptr_t a = tab.ptr[t] + lane * es; a < e; a += 32 * es) store_one(a, dt, load_one(a, dt) * s);
+  }
+}
+
+}  // namespace clip
+}  // namespace vq

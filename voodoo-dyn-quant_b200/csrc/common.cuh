@@ -20,6 +20,7 @@ enum DeviceError : int {
   kDevWaitTimeout = 1,  // an mbarrier wait exceeded kWaitTimeoutNs
   kDevBadFormat = 2,    // unknown block format reached a kernel
   kDevBadSmemAlign = 3, // dynamic shared memory not 1024-byte aligned
+  kDevBadIndex = 4,     // a token id outside the table of a lookup
 };
 
 // Every spin on an mbarrier gives up after this long, records

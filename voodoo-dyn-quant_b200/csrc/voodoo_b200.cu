@@ -12,7 +12,9 @@
 
 #include <cstdarg>
 #include <cstdint>
+#include <cmath>
 #include <cstdio>
+#include <cstdlib>
 #include <atomic>
 #include <cstring>
 #include <mutex>
@@ -24,6 +26,9 @@
 #include "loss.cuh"
 #include "blocks.cuh"
 #include "quant.cuh"
+#include "qk_norm.cuh"
+#include "embed.cuh"
+#include "clip.cuh"
 #include "../../include/voodoo_b200.h"
 
 namespace {
@@ -1122,3 +1127,498 @@ int vq_quantize(int ggml_type, const void* w, int w_dtype, int64_t rows, int64_t
 
 }  // extern "C"
 
+
+namespace {
+
+// ---- norm of the query and key heads with their rotation ----
+struct QkPlan {
+  int team_log2, q_chunks, q_iters, q_blocks, k_chunks, k_iters, k_blocks;
+};
+
+// How the heads of a position are spread over warps, and the warps over
+// blocks.  A warp walks all heads of its side at a position (their table and
+// weight values then stay in registers) unless that leaves fewer warps than
+// the GPU holds at 32 per SM; then the heads are split as far as that needs.
+int qk_plan(QkPlan* p, int64_t positions, int64_t Hq, int64_t Hk, int64_t D) {
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  p->team_log2 = 0;
+  while ((16LL << p->team_log2) < D) ++p->team_log2;
+  const int per_warp = 32 >> p->team_log2;
+  const long long warps = 32LL * sms;
+  const int64_t H[2] = {Hq, Hk};
+  int* chunks[2] = {&p->q_chunks, &p->k_chunks};
+  int* iters[2] = {&p->q_iters, &p->k_iters};
+  long long items[2];
+  for (int i = 0; i < 2; ++i) {
+    const long long all = (H[i] + per_warp - 1) / per_warp;
+    long long split = positions > 0 ? (warps + positions - 1) / positions : 1;
+    if (split > all) split = all;
+    if (split < 1) split = 1;
+    *iters[i] = static_cast<int>((all + split - 1) / split);
+    *chunks[i] = *iters[i] > 0 ? static_cast<int>((all + *iters[i] - 1) / *iters[i]) : 0;
+    items[i] = positions * *chunks[i];
+  }
+  // blocks of 4 warps, 8 a SM, shared by the sides as their heads are
+  const long long cap = 8LL * sms < vq::qknorm::kMaxBlocks ? 8LL * sms : vq::qknorm::kMaxBlocks;
+  long long qb = (items[0] + vq::qknorm::kWarps - 1) / vq::qknorm::kWarps;
+  long long kb = (items[1] + vq::qknorm::kWarps - 1) / vq::qknorm::kWarps;
+  if (qb + kb > cap) {
+    long long qc = cap * Hq / (Hq + Hk);
+    if (Hq > 0 && qc < 1) qc = 1;
+    if (Hk > 0 && qc > cap - 1) qc = cap - 1;
+    if (qb > qc) qb = qc;
+    if (kb > cap - qc) kb = cap - qc;
+  }
+  p->q_blocks = static_cast<int>(qb);
+  p->k_blocks = static_cast<int>(kb);
+  return 0;
+}
+
+int check_heads(const void* p, const int64_t* st, int64_t H, const char* name) {
+  if (H == 0) return 0;
+  if (p == nullptr || !aligned16(p)) return fail(VQ_ERR_INVALID, "%s: null pointer or not 16-byte aligned", name);
+  if (st == nullptr) return fail(VQ_ERR_INVALID, "%s: null stride array", name);
+  for (int i = 0; i < 3; ++i)
+    if (st[i] < 0 || st[i] % 8 != 0)
+      return fail(VQ_ERR_INVALID, "%s: strides must be non-negative multiples of 8", name);
+  return 0;
+}
+
+int check_qk(int64_t Hq, int64_t Hk, int64_t B, int64_t S, int64_t D, int64_t R, const void* q_weight,
+             const void* k_weight, const void* cos, const void* sin, const int64_t* cs_strides, int dtype) {
+  if (B < 0 || S < 0 || Hq < 0 || Hk < 0) return fail(VQ_ERR_INVALID, "negative shape");
+  if (D <= 0 || D % 16 != 0 || D > vq::qknorm::kMaxDim)
+    return fail(VQ_ERR_INVALID, "head dimension %lld must be a multiple of 16 up to %d", (long long)D, vq::qknorm::kMaxDim);
+  if (R <= 0 || R % 16 != 0 || R > D)
+    return fail(VQ_ERR_INVALID, "rotary dimension %lld must be a multiple of 16 up to the head dimension", (long long)R);
+  if (dtype < 0 || dtype > 2) return fail(VQ_ERR_INVALID, "dtype %d (0 = float32, 1 = bfloat16, 2 = float16)", dtype);
+  if (Hq > 65535 || Hk > 65535 || S > 0x7fffffffLL || (S > 0 && B > 0x7fffffffLL / S))
+    return fail(VQ_ERR_INVALID, "shape too large");
+  if (B == 0 || S == 0 || Hq + Hk == 0) return 0;
+  if ((Hq > 0 && (q_weight == nullptr || !aligned16(q_weight))) || (Hk > 0 && (k_weight == nullptr || !aligned16(k_weight))))
+    return fail(VQ_ERR_INVALID, "weights must be 16-byte aligned pointers");
+  if (cos == nullptr || sin == nullptr || !aligned16(cos) || !aligned16(sin))
+    return fail(VQ_ERR_INVALID, "cos/sin must be 16-byte aligned pointers");
+  if (cs_strides == nullptr) return fail(VQ_ERR_INVALID, "null stride array");
+  if (cs_strides[0] < 0 || cs_strides[1] < 0 || cs_strides[0] % 8 != 0 || cs_strides[1] % 8 != 0)
+    return fail(VQ_ERR_INVALID, "cos/sin strides must be non-negative multiples of 8");
+  return 0;
+}
+
+struct QkArgs {
+  const void *q, *k, *gq, *gk, *q_weight, *k_weight, *cos, *sin;
+  const int64_t *qs, *ks, *gqs, *gks, *cs;
+  int64_t Hq, Hk, B, S, D, R;
+  bool w_f32, cs_f32;
+  float eps, offset;
+  void *q_out, *k_out;
+};
+
+template <typename T, bool kBackward>
+int launch_qk(const QkArgs& a, const QkPlan& p, float* partials, cudaStream_t st) {
+  using namespace vq::qknorm;
+  auto side = [](const void* x, const int64_t* xs, const void* g, const int64_t* gs, void* out, const void* w, int64_t H,
+                 int chunks, int iters, int blocks) {
+    Side<T> s{};
+    if (H == 0) return s;
+    s.x = static_cast<const T*>(x);
+    s.xb = xs[0], s.xs = xs[1], s.xh = xs[2];
+    if (kBackward) {
+      s.g = static_cast<const T*>(g);
+      s.gb = gs[0], s.gs = gs[1], s.gh = gs[2];
+    }
+    s.out = static_cast<T*>(out);
+    s.w = w;
+    s.H = static_cast<int>(H);
+    s.chunks = chunks, s.iters = iters, s.blocks = blocks;
+    return s;
+  };
+  const Side<T> q = side(a.q, a.qs, a.gq, a.gqs, a.q_out, a.q_weight, a.Hq, p.q_chunks, p.q_iters, p.q_blocks);
+  const Side<T> k = side(a.k, a.ks, a.gk, a.gks, a.k_out, a.k_weight, a.Hk, p.k_chunks, p.k_iters, p.k_blocks);
+  Shape sh{};
+  sh.cos = a.cos, sh.sin = a.sin;
+  sh.cb = a.cs[0], sh.cs = a.cs[1];
+  sh.positions = a.B * a.S;
+  sh.S = static_cast<int>(a.S), sh.D = static_cast<int>(a.D), sh.R = static_cast<int>(a.R);
+  sh.team_log2 = p.team_log2;
+  sh.eps = a.eps, sh.offset = a.offset;
+  sh.w_f32 = a.w_f32, sh.cs_f32 = a.cs_f32;
+  qk_norm_rope_kernel<T, kBackward><<<p.q_blocks + p.k_blocks, kThreads, 0, st>>>(q, k, sh, partials);
+  VQ_CUDA(cudaGetLastError());
+  return 0;
+}
+
+template <bool kBackward>
+int launch_qk_dtype(const QkArgs& a, const QkPlan& p, int dtype, float* partials, cudaStream_t st) {
+  if (dtype == 0) return launch_qk<float, kBackward>(a, p, partials, st);
+  if (dtype == 1) return launch_qk<__nv_bfloat16, kBackward>(a, p, partials, st);
+  return launch_qk<__half, kBackward>(a, p, partials, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+int vq_qk_norm_rope_fwd(const void* q, const int64_t* q_strides, int64_t Hq, const void* k, const int64_t* k_strides,
+                        int64_t Hk, const void* q_weight, const void* k_weight, int weight_f32, const void* cos,
+                        const void* sin, const int64_t* cs_strides, int cs_f32, int64_t B, int64_t S, int64_t D,
+                        int64_t R, float eps, float weight_offset, int dtype, void* q_out, void* k_out, void* stream) {
+  DeviceScope scope(q_out != nullptr ? q_out : k_out);
+  if (int rc = check_qk(Hq, Hk, B, S, D, R, q_weight, k_weight, cos, sin, cs_strides, dtype)) return rc;
+  if (B == 0 || S == 0 || Hq + Hk == 0) return 0;
+  if (int rc = check_heads(q, q_strides, Hq, "q")) return rc;
+  if (int rc = check_heads(k, k_strides, Hk, "k")) return rc;
+  if ((Hq > 0 && (q_out == nullptr || !aligned16(q_out))) || (Hk > 0 && (k_out == nullptr || !aligned16(k_out))))
+    return fail(VQ_ERR_INVALID, "outputs must be 16-byte aligned pointers");
+  QkPlan p;
+  if (int rc = qk_plan(&p, B * S, Hq, Hk, D)) return rc;
+  const QkArgs a{q,  k,  nullptr, nullptr, q_weight, k_weight, cos, sin, q_strides, k_strides, nullptr, nullptr, cs_strides,
+                 Hq, Hk, B,       S,       D,        R,        weight_f32 != 0, cs_f32 != 0, eps, weight_offset, q_out, k_out};
+  return launch_qk_dtype<false>(a, p, dtype, nullptr, static_cast<cudaStream_t>(stream));
+}
+
+size_t vq_qk_norm_rope_workspace_bytes(int64_t D) {
+  return D > 0 && D <= vq::qknorm::kMaxDim ? static_cast<size_t>(vq::qknorm::kMaxBlocks) * D * sizeof(float) : 0;
+}
+
+int vq_qk_norm_rope_bwd(const void* gq, const int64_t* gq_strides, const void* gk, const int64_t* gk_strides,
+                        const void* q, const int64_t* q_strides, int64_t Hq, const void* k, const int64_t* k_strides,
+                        int64_t Hk, const void* q_weight, const void* k_weight, int weight_f32, const void* cos,
+                        const void* sin, const int64_t* cs_strides, int cs_f32, int64_t B, int64_t S, int64_t D,
+                        int64_t R, float eps, float weight_offset, int dtype, void* dq, void* dk, void* dq_weight,
+                        void* dk_weight, void* workspace, size_t workspace_bytes, void* stream) {
+  DeviceScope scope(dq != nullptr ? dq : dk);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (int rc = check_qk(Hq, Hk, B, S, D, R, q_weight, k_weight, cos, sin, cs_strides, dtype)) return rc;
+  const bool want_dw = dq_weight != nullptr || dk_weight != nullptr;
+  const size_t wbytes = static_cast<size_t>(D) * (weight_f32 || dtype == 0 ? 4 : 2);
+  if (B == 0 || S == 0 || Hq + Hk == 0) {
+    if (dq_weight != nullptr) VQ_CUDA(cudaMemsetAsync(dq_weight, 0, wbytes, st));
+    if (dk_weight != nullptr) VQ_CUDA(cudaMemsetAsync(dk_weight, 0, wbytes, st));
+    return 0;
+  }
+  if (int rc = check_heads(q, q_strides, Hq, "q")) return rc;
+  if (int rc = check_heads(k, k_strides, Hk, "k")) return rc;
+  if (int rc = check_heads(gq, gq_strides, Hq, "gq")) return rc;
+  if (int rc = check_heads(gk, gk_strides, Hk, "gk")) return rc;
+  if ((Hq > 0 && (dq == nullptr || !aligned16(dq))) || (Hk > 0 && (dk == nullptr || !aligned16(dk))))
+    return fail(VQ_ERR_INVALID, "outputs must be 16-byte aligned pointers");
+  if (want_dw && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < vq_qk_norm_rope_workspace_bytes(D)))
+    return fail(VQ_ERR_INVALID, "workspace of %zu bytes needed for the weight gradients", vq_qk_norm_rope_workspace_bytes(D));
+  QkPlan p;
+  if (int rc = qk_plan(&p, B * S, Hq, Hk, D)) return rc;
+  const QkArgs a{q,  k,  gq, gk, q_weight, k_weight, cos, sin, q_strides, k_strides, gq_strides, gk_strides, cs_strides,
+                 Hq, Hk, B,  S,  D,        R,        weight_f32 != 0, cs_f32 != 0, eps, weight_offset, dq, dk};
+  float* partials = want_dw ? static_cast<float*>(workspace) : nullptr;
+  if (int rc = launch_qk_dtype<true>(a, p, dtype, partials, st)) return rc;
+  if (!want_dw) return 0;
+  const dim3 grid(static_cast<unsigned>((D + 31) / 32), 2);
+  const bool f32 = weight_f32 != 0 || dtype == 0;
+  if (dtype == 2)
+    vq::qknorm::qk_norm_weight_grad_kernel<__half><<<grid, 512, 0, st>>>(partials, p.q_blocks, p.k_blocks, (int)D, f32,
+                                                                         dq_weight, dk_weight);
+  else
+    vq::qknorm::qk_norm_weight_grad_kernel<__nv_bfloat16><<<grid, 512, 0, st>>>(partials, p.q_blocks, p.k_blocks, (int)D,
+                                                                                f32, dq_weight, dk_weight);
+  VQ_CUDA(cudaGetLastError());
+  return 0;
+}
+
+}  // extern "C"
+
+namespace {
+
+// ---- gated embedding ----
+int check_table(const vq::CandSet& cs, int64_t T, int64_t vocab_start, int64_t rows, int64_t padded_cols, int64_t cols) {
+  (void)cs;
+  if (T < 0 || rows < 0 || cols < 0 || vocab_start < 0) return fail(VQ_ERR_INVALID, "negative shape or vocabulary start");
+  if (padded_cols < cols || padded_cols % 256 != 0)
+    return fail(VQ_ERR_INVALID, "padded columns %lld must be a multiple of 256 that holds %lld", (long long)padded_cols,
+                (long long)cols);
+  if (T > (1LL << 30) || rows > (1LL << 30) || padded_cols > (1LL << 30)) return fail(VQ_ERR_INVALID, "shape too large");
+  return 0;
+}
+
+template <typename T>
+int launch_embed_gategrad(const vq::CandSet& cs, const int* keys, const int* order, int T_, int rows, int upr, int cols,
+                          const void* dy, long long lddy, double* partials, int* blocks, int* err, cudaStream_t st) {
+  using namespace vq::embed;
+  auto kern = embed_gategrad_kernel<T>;
+  const int smem = cs.K * kThreads * static_cast<int>(sizeof(double)) + kWarps * warp_bytes(cs);
+  VQ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  int per_sm = 0, sms = 0;
+  VQ_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kThreads, smem));
+  if (per_sm < 1) return fail(VQ_ERR_INVALID, "%d candidates do not fit one SM", cs.K);
+  if (int rc = sm_count(&sms)) return rc;
+  const long long groups = (upr + kUnits - 1) / kUnits;
+  const long long resident = static_cast<long long>(sms) * per_sm * kWarps;
+  // the longest run of sorted tokens that still leaves four items a resident warp
+  int window = 1;
+  while (window < 32 && (T_ + 2 * window - 1) / (2 * window) * groups >= 4 * resident) window *= 2;
+  const long long items = (T_ + window - 1) / window * groups;
+  long long grid = (items + kWarps - 1) / kWarps;
+  if (grid > static_cast<long long>(sms) * per_sm) grid = static_cast<long long>(sms) * per_sm;
+  if (grid > vq::embed::kMaxBlocks) grid = vq::embed::kMaxBlocks;
+  *blocks = static_cast<int>(grid);
+  kern<<<*blocks, kThreads, smem, st>>>(cs, keys, order, T_, rows, upr, cols, window, static_cast<const T*>(dy), lddy,
+                                        partials, err);
+  VQ_CUDA(cudaGetLastError());
+  return 0;
+}
+
+inline size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
+
+}  // namespace
+
+extern "C" {
+
+int vq_embed_mix(int K, const int* types, const void* const* blocks, const float* probs, const void* ids, int ids_i32,
+                 int64_t T, int64_t vocab_start, int64_t rows, int64_t padded_cols, int64_t cols, float scale, int strict,
+                 void* out, int64_t ldo, void* stream) {
+  DeviceScope scope(out);
+  vq::CandSet cs;
+  if (int rc = build_candset(&cs, K, types, blocks)) return rc;
+  if (int rc = check_table(cs, T, vocab_start, rows, padded_cols, cols)) return rc;
+  if (int rc = check_matrix(out, T, cols, ldo, "out")) return rc;
+  if (T == 0 || cols == 0) return 0;
+  if (probs == nullptr || ids == nullptr) return fail(VQ_ERR_INVALID, "null pointer");
+  if (reinterpret_cast<uintptr_t>(ids) % (ids_i32 ? 4 : 8) != 0) return fail(VQ_ERR_INVALID, "misaligned token ids");
+  int* err = nullptr;
+  if (int rc = device_error_ptr(&err)) return rc;
+  using namespace vq::embed;
+  const int smem = kWarps * warp_bytes(cs);
+  VQ_CUDA(cudaFuncSetAttribute(embed_mix_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  int per_sm = 0, sms = 0;
+  VQ_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, embed_mix_kernel, kThreads, smem));
+  if (per_sm < 1) return fail(VQ_ERR_INVALID, "mixture of %d candidates does not fit one SM", K);
+  if (int rc = sm_count(&sms)) return rc;
+  const int upr = static_cast<int>(padded_cols / 256);
+  const long long units = T * upr;
+  long long grid = (units + kWarps * kUnits - 1) / (kWarps * kUnits);
+  if (grid > static_cast<long long>(sms) * per_sm) grid = static_cast<long long>(sms) * per_sm;
+  embed_mix_kernel<<<static_cast<unsigned>(grid), kThreads, smem, static_cast<cudaStream_t>(stream)>>>(
+      cs, probs, Ids{ids, ids_i32 != 0}, T, vocab_start, rows, upr, static_cast<int>(cols), scale, strict != 0,
+      static_cast<__nv_bfloat16*>(out), ldo, err);
+  VQ_CUDA(cudaGetLastError());
+  return 0;
+}
+
+size_t vq_embed_gategrad_workspace_bytes(int64_t T, int K) {
+  if (T < 0 || T > (1LL << 30) || K < 1 || K > vq::kMaxCandidates) return 0;
+  // sorted keys and tokens, twice (a radix pass reads one pair and writes the other); the blocks' partials
+  return 4 * round256(static_cast<size_t>(T) * sizeof(int)) + round256(static_cast<size_t>(vq::embed::kMaxBlocks) * K * sizeof(double));
+}
+
+int vq_token_sort(const void* ids, int ids_i32, int64_t T, int64_t vocab_start, int64_t rows, int* keys, int* order,
+                  int* keys_tmp, int* order_tmp, void* stream) {
+  DeviceScope scope(keys);
+  if (T < 0 || rows < 0 || vocab_start < 0) return fail(VQ_ERR_INVALID, "negative shape or vocabulary start");
+  if (T > (1LL << 30) || rows > (1LL << 30)) return fail(VQ_ERR_INVALID, "shape too large");
+  if (T == 0) return 0;
+  if (ids == nullptr || keys == nullptr || order == nullptr || keys_tmp == nullptr || order_tmp == nullptr)
+    return fail(VQ_ERR_INVALID, "null pointer");
+  if (reinterpret_cast<uintptr_t>(ids) % (ids_i32 ? 4 : 8) != 0) return fail(VQ_ERR_INVALID, "misaligned token ids");
+  using namespace vq::embed;
+  int bits = 1;
+  while ((rows >> bits) != 0) ++bits;
+  const int passes = (bits + kDigitBits - 1) / kDigitBits;
+  const int ctas = static_cast<int>(T >= static_cast<int64_t>(kSortCtas) * kSortThreads ? kSortCtas
+                                                                                        : (T + kSortThreads - 1) / kSortThreads);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(kSortThreads);
+  cfg.dynamicSmemBytes = kSortSmem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(ctas);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  VQ_CUDA(cudaLaunchKernelEx(&cfg, token_sort_kernel, Ids{ids, ids_i32 != 0}, static_cast<int>(T),
+                             static_cast<long long>(vocab_start), static_cast<int>(rows), passes, keys, order, keys_tmp,
+                             order_tmp));
+  VQ_CUDA(cudaGetLastError());
+  return 0;
+}
+
+int vq_embed_gategrad(int K, const int* types, const void* const* blocks, const void* ids, int ids_i32, int64_t T,
+                      int64_t vocab_start, int64_t rows, int64_t padded_cols, int64_t cols, float scale, const void* dy,
+                      int64_t lddy, int dy_dtype, void* workspace, size_t workspace_bytes, float* grad, void* stream) {
+  DeviceScope scope(grad);
+  vq::CandSet cs;
+  if (int rc = build_candset(&cs, K, types, blocks)) return rc;
+  if (int rc = check_table(cs, T, vocab_start, rows, padded_cols, cols)) return rc;
+  if (int rc = check_matrix(dy, T, cols, lddy, "dy")) return rc;
+  if (dy_dtype < 0 || dy_dtype > 2) return fail(VQ_ERR_INVALID, "dtype %d (0 = float32, 1 = bfloat16, 2 = float16)", dy_dtype);
+  if (grad == nullptr) return fail(VQ_ERR_INVALID, "null pointer");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (T == 0 || cols == 0 || rows == 0) {
+    VQ_CUDA(cudaMemsetAsync(grad, 0, K * sizeof(float), st));
+    return 0;
+  }
+  if (ids == nullptr || workspace == nullptr) return fail(VQ_ERR_INVALID, "null pointer");
+  const size_t need = vq_embed_gategrad_workspace_bytes(T, K);
+  if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0 || workspace_bytes < need)
+    return fail(VQ_ERR_INVALID, "workspace of %zu bytes (16-byte aligned) needed, got %zu", need, workspace_bytes);
+  const size_t part = round256(static_cast<size_t>(T) * sizeof(int));
+  char* ws = static_cast<char*>(workspace);
+  int* keys = reinterpret_cast<int*>(ws);
+  int* order = reinterpret_cast<int*>(ws + part);
+  double* partials = reinterpret_cast<double*>(ws + 4 * part);
+  if (int rc = vq_token_sort(ids, ids_i32, T, vocab_start, rows, keys, order, reinterpret_cast<int*>(ws + 2 * part),
+                             reinterpret_cast<int*>(ws + 3 * part), stream))
+    return rc;
+  int* err = nullptr;
+  if (int rc = device_error_ptr(&err)) return rc;
+  const int upr = static_cast<int>(padded_cols / 256);
+  int n = 0, rc = 0;
+  if (dy_dtype == 0)
+    rc = launch_embed_gategrad<float>(cs, keys, order, (int)T, (int)rows, upr, (int)cols, dy, lddy, partials, &n, err, st);
+  else if (dy_dtype == 1)
+    rc = launch_embed_gategrad<__nv_bfloat16>(cs, keys, order, (int)T, (int)rows, upr, (int)cols, dy, lddy, partials, &n, err, st);
+  else
+    rc = launch_embed_gategrad<__half>(cs, keys, order, (int)T, (int)rows, upr, (int)cols, dy, lddy, partials, &n, err, st);
+  if (rc) return rc;
+  vq::embed::embed_gategrad_join_kernel<<<1, 32 * vq::kMaxCandidates, 0, st>>>(partials, n, K, scale, grad);
+  VQ_CUDA(cudaGetLastError());
+  return 0;
+}
+
+}  // extern "C"
+
+namespace {
+
+// ---- global norm and clipping ----
+struct Range {
+  uintptr_t b, e;
+};
+
+int range_less(const void* x, const void* y) {
+  const uintptr_t a = static_cast<const Range*>(x)->b, b = static_cast<const Range*>(y)->b;
+  return a < b ? -1 : a > b;
+}
+
+// Values that one block takes and scales in one launch, at most.
+constexpr long long kClipSmallValues = 16384;
+
+template <int N>
+void fill_table(vq::clip::Table<N>* t, const void* const* ptrs, const int64_t* numel, const int* dtypes, int n) {
+  long long chunks = 0;
+  t->n = n;
+  for (int i = 0; i < n; ++i) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(ptrs[i]);
+    const long long bytes = numel[i] * (dtypes[i] == vq::clip::kF32 ? 4 : 2);
+    t->ptr[i] = p;
+    t->bytes[i] = bytes;
+    t->dtype[i] = static_cast<uint8_t>(dtypes[i]);
+    t->first_chunk[i] = static_cast<int>(chunks);
+    const uintptr_t span = p + bytes - (p & ~uintptr_t(15));
+    chunks += static_cast<long long>((span + vq::clip::kChunkBytes - 1) / vq::clip::kChunkBytes);
+  }
+  t->chunks = static_cast<int>(chunks);
+}
+
+template <int N, bool kMax>
+int launch_clip(const void* const* ptrs, const int64_t* numel, const int* dtypes, int n, long long total,
+                float max_norm, double* partials, int max_partials, float* norm, cudaStream_t st) {
+  using namespace vq::clip;
+  static_assert(sizeof(Table<N>) + 64 <= 32764, "kernel parameters");
+  Table<N> tab;
+  if (n <= N && total <= kClipSmallValues) {
+    fill_table(&tab, ptrs, numel, dtypes, n);
+    small_kernel<N, kMax><<<1, kSmallThreads, 0, st>>>(tab, max_norm, max_norm != INFINITY, norm);
+    VQ_CUDA(cudaGetLastError());
+    return 0;
+  }
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  int cap = kBlocksPerSm * sms < vq::clip::kMaxBlocks ? kBlocksPerSm * sms : vq::clip::kMaxBlocks;
+  int used = 0;
+  for (int i = 0; i < n; i += N) {
+    const int m = n - i < N ? n - i : N;
+    fill_table(&tab, ptrs + i, numel + i, dtypes + i, m);
+    const int grid = tab.chunks < cap ? tab.chunks : cap;
+    if (used + grid > max_partials) return fail(VQ_ERR_INVALID, "workspace too small");
+    norm_kernel<N, kMax><<<grid, kThreads, 0, st>>>(tab, partials + used);
+    VQ_CUDA(cudaGetLastError());
+    used += grid;
+  }
+  // pass 2, the last table first (it is the one at hand); a norm alone needs one block, which joins the partials
+  const bool scale = max_norm != INFINITY;
+  for (int i = scale ? (n - 1) / N * N : 0; i >= 0; i -= N) {
+    const int m = n - i < N ? n - i : N;
+    if (scale && n > N) fill_table(&tab, ptrs + i, numel + i, dtypes + i, m);
+    const int grid = !scale ? 1 : tab.chunks < cap ? tab.chunks : cap;
+    scale_kernel<N, kMax><<<grid, kThreads, 0, st>>>(tab, partials, used, max_norm, scale, i == 0 ? norm : nullptr);
+    VQ_CUDA(cudaGetLastError());
+  }
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t vq_clip_grad_norm_workspace_bytes(int n) {
+  if (n < 0) return 0;
+  const size_t launches = static_cast<size_t>(n) / vq::clip::kShortTable + 1;
+  return launches * vq::clip::kMaxBlocks * sizeof(double);
+}
+
+int vq_clip_grad_norm(int n, const void* const* ptrs, const int64_t* numel, const int* dtypes, float max_norm,
+                      int norm_inf, void* workspace, size_t workspace_bytes, float* norm, void* stream) {
+  DeviceScope scope(norm);
+  if (n < 0) return fail(VQ_ERR_INVALID, "negative count");
+  if (norm == nullptr) return fail(VQ_ERR_INVALID, "null pointer");
+  if (!(max_norm >= 0.f)) return fail(VQ_ERR_INVALID, "max_norm must not be negative or NaN");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (n > 0 && (ptrs == nullptr || numel == nullptr || dtypes == nullptr)) return fail(VQ_ERR_INVALID, "null array");
+  if (n > (1 << 20)) return fail(VQ_ERR_INVALID, "too many tensors");
+  // the tensors that hold something, checked, with their ranges in order
+  Range* r = static_cast<Range*>(std::malloc(static_cast<size_t>(n + 1) * sizeof(Range)));
+  const void** p = static_cast<const void**>(std::malloc(static_cast<size_t>(n + 1) * sizeof(void*)));
+  int64_t* c = static_cast<int64_t*>(std::malloc(static_cast<size_t>(n + 1) * sizeof(int64_t)));
+  int* d = static_cast<int*>(std::malloc(static_cast<size_t>(n + 1) * sizeof(int)));
+  struct Free {
+    void *a, *b, *c, *d;
+    ~Free() { std::free(a), std::free(b), std::free(c), std::free(d); }
+  } guard{r, static_cast<void*>(p), c, d};
+  if (r == nullptr || p == nullptr || c == nullptr || d == nullptr) return fail(VQ_ERR_INVALID, "out of host memory");
+  int m = 0;
+  long long total = 0;
+  for (int i = 0; i < n; ++i) {
+    if (numel[i] < 0 || numel[i] > (1LL << 40)) return fail(VQ_ERR_INVALID, "tensor %d: bad size", i);
+    if (dtypes[i] < 0 || dtypes[i] > 2) return fail(VQ_ERR_INVALID, "tensor %d: dtype %d (0 = float32, 1 = bfloat16, 2 = float16)", i, dtypes[i]);
+    if (numel[i] == 0) continue;
+    const int es = dtypes[i] == 0 ? 4 : 2;
+    const uintptr_t b = reinterpret_cast<uintptr_t>(ptrs[i]);
+    if (b == 0 || b % es != 0) return fail(VQ_ERR_INVALID, "tensor %d: null or misaligned pointer", i);
+    p[m] = ptrs[i], c[m] = numel[i], d[m] = dtypes[i];
+    r[m] = Range{b, b + static_cast<uintptr_t>(numel[i]) * es};
+    total += numel[i];
+    ++m;
+  }
+  if (total > (1LL << 42)) return fail(VQ_ERR_INVALID, "too many values");
+  std::qsort(r, m, sizeof(Range), range_less);
+  for (int i = 1; i < m; ++i)
+    if (r[i].b < r[i - 1].e) return fail(VQ_ERR_INVALID, "two of the tensors share memory: each value is scaled once");
+  if (m == 0) {
+    VQ_CUDA(cudaMemsetAsync(norm, 0, sizeof(float), st));
+    return 0;
+  }
+  const size_t need = vq_clip_grad_norm_workspace_bytes(n);
+  if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 7u) != 0 || workspace_bytes < need)
+    return fail(VQ_ERR_INVALID, "workspace of %zu bytes needed, got %zu", need, workspace_bytes);
+  double* part = static_cast<double*>(workspace);
+  const int cap = static_cast<int>(workspace_bytes / sizeof(double) < 0x7fffffff ? workspace_bytes / sizeof(double) : 0x7fffffff);
+  const bool small = m <= vq::clip::kShortTable;
+  if (norm_inf)
+    return small ? launch_clip<vq::clip::kShortTable, true>(p, c, d, m, total, max_norm, part, cap, norm, st)
+                 : launch_clip<vq::clip::kLongTable, true>(p, c, d, m, total, max_norm, part, cap, norm, st);
+  return small ? launch_clip<vq::clip::kShortTable, false>(p, c, d, m, total, max_norm, part, cap, norm, st)
+               : launch_clip<vq::clip::kLongTable, false>(p, c, d, m, total, max_norm, part, cap, norm, st);
+}
+
+}  // extern "C"

@@ -77,6 +77,20 @@ def _declare(lib):
         "vq_rope": (_int, [_vp, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _int, _vp, _vp, _vp]),
         "vq_swiglu_fwd": (_int, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _vp]),
         "vq_swiglu_bwd": (_int, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp]),
+        "vq_qk_norm_rope_fwd": (_int, [_vp, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _int, _vp, _vp, _vp, _int, _i64, _i64,
+                                       _i64, _i64, _f32, _f32, _int, _vp, _vp, _vp]),
+        "vq_qk_norm_rope_workspace_bytes": (ctypes.c_size_t, [_i64]),
+        "vq_qk_norm_rope_bwd": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _int, _vp, _vp, _vp,
+                                       _int, _i64, _i64, _i64, _i64, _f32, _f32, _int, _vp, _vp, _vp, _vp, _vp,
+                                       ctypes.c_size_t, _vp]),
+        "vq_embed_mix": (_int, [_int, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, _i64, _f32, _int, _vp, _i64,
+                                _vp]),
+        "vq_token_sort": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
+        "vq_embed_gategrad_workspace_bytes": (ctypes.c_size_t, [_i64, _int]),
+        "vq_embed_gategrad": (_int, [_int, _vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, _i64, _f32, _vp, _i64, _int, _vp,
+                                     ctypes.c_size_t, _vp, _vp]),
+        "vq_clip_grad_norm_workspace_bytes": (ctypes.c_size_t, [_int]),
+        "vq_clip_grad_norm": (_int, [_int, _vp, _vp, _vp, _f32, _int, _vp, ctypes.c_size_t, _vp, _vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -92,6 +106,9 @@ EXPORTED = (
     "vq_mixgemm_fwd", "vq_mixgemm_fwd_fused", "vq_mixgemm_dx",
     "vq_loss_fused", "vq_loss_stats", "vq_loss_combine", "vq_loss_grad",
     "vq_rmsnorm_fwd", "vq_rmsnorm_bwd", "vq_add_rmsnorm_fwd", "vq_rmsnorm_bwd_add", "vq_rope", "vq_swiglu_fwd", "vq_swiglu_bwd",
+    "vq_qk_norm_rope_fwd", "vq_qk_norm_rope_workspace_bytes", "vq_qk_norm_rope_bwd",
+    "vq_embed_mix", "vq_token_sort", "vq_embed_gategrad_workspace_bytes", "vq_embed_gategrad",
+    "vq_clip_grad_norm_workspace_bytes", "vq_clip_grad_norm",
 )
 
 
@@ -135,6 +152,23 @@ def _require_cuda(*ts: torch.Tensor) -> None:
 
 def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
+
+
+# dtype codes of the entry points that take more than one floating type
+_FLOAT_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _float_code(t: torch.Tensor, name: str) -> int:
+    code = _FLOAT_CODE.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{name}: float32, bfloat16 or float16 expected, got {t.dtype}")
+    return code
+
+
+def _require_one_device(*ts: torch.Tensor) -> None:
+    for t in ts[1:]:
+        if t.device != ts[0].device:
+            raise ValueError(f"tensors on one device expected, got {ts[0].device} and {t.device}")
 
 
 def format_info(qtype: str) -> tuple[int, int]:
@@ -577,3 +611,202 @@ def swiglu_bwd(gate: torch.Tensor, up: torch.Tensor, dy: torch.Tensor, out: torc
                               rows, F, dg.data_ptr(), du.data_ptr(), dg.stride(0), _stream(gate)))
     return dg, du
 
+
+
+# ---------------------------------------------------------------- head norms with rotation
+def _heads_operand(t: torch.Tensor) -> torch.Tensor:
+    """[B, S, H, D] view with unit stride over D, the others multiples of 8, 16-byte aligned; copied otherwise."""
+    if t.numel() and (t.stride(-1) != 1 or any(st % 8 for st in t.stride()[:3]) or t.data_ptr() % 16 != 0):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+def _qk_operands(q, k, q_weight, k_weight, cos, sin):
+    """Checked and laid out operands, and the scalar arguments that both directions pass on."""
+    _require_cuda(q, k, q_weight, k_weight, cos, sin)
+    _require_one_device(q, k, q_weight, k_weight, cos, sin)
+    if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
+        raise ValueError(f"qk_norm_rope: q [B, S, Hq, D] and k [B, S, Hk, D] expected, got {tuple(q.shape)} and "
+                         f"{tuple(k.shape)}")
+    dtype = _float_code(q, "qk_norm_rope")
+    if k.dtype != q.dtype:
+        raise ValueError(f"qk_norm_rope: q is {q.dtype}, k is {k.dtype}")
+    B, S, _, D = q.shape
+    for w in (q_weight, k_weight):
+        _float_code(w, "qk_norm_rope weight")
+        if tuple(w.shape) != (D,):
+            raise ValueError(f"qk_norm_rope: weights of shape ({D},) expected, got {tuple(w.shape)}")
+    for c in (cos, sin):
+        _float_code(c, "qk_norm_rope table")
+        if c.dim() not in (2, 3) or c.shape != cos.shape or c.shape[-2] != S or (c.dim() == 3 and c.shape[0] not in (1, B)):
+            raise ValueError(f"qk_norm_rope: cos and sin [B or 1, S, R] expected, got {tuple(cos.shape)} and "
+                             f"{tuple(sin.shape)} for q {tuple(q.shape)}")
+    R = cos.shape[-1]
+    if not (q_weight.dtype == k_weight.dtype == q.dtype):
+        q_weight, k_weight = q_weight.float(), k_weight.float()
+    if not (cos.dtype == sin.dtype == q.dtype):
+        cos, sin = cos.float(), sin.float()
+    q_weight, k_weight = _aligned(q_weight), _aligned(k_weight)
+    if cos.stride() != sin.stride() or cos.stride(-1) != 1 or any(st % 8 for st in cos.stride()[:-1]) or \
+            cos.data_ptr() % 16 or sin.data_ptr() % 16:
+        cos = cos.clone(memory_format=torch.contiguous_format)
+        sin = sin.clone(memory_format=torch.contiguous_format)
+    c3, s3 = cos.expand(B, S, R), sin.expand(B, S, R)
+    return _heads_operand(q), _heads_operand(k), q_weight, k_weight, c3, s3, (B, S, D, R), dtype
+
+
+def _strides(t: torch.Tensor, n: int):
+    return (ctypes.c_int64 * n)(*t.stride()[:n])
+
+
+def qk_norm_rope_fwd(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                     cos: torch.Tensor, sin: torch.Tensor, eps: float, weight_offset: float = 0.0):
+    """Norm of each head of q [B, S, Hq, D] and k [B, S, Hk, D] (float32, bfloat16 or float16, any strides) with
+    weights ``weight_offset + weight`` [D], then the rotation of its first R values by cos / sin [B or 1, S, R];
+    contiguous outputs of q's type, rounded once."""
+    q, k, wq, wk, c, s, (B, S, D, R), dtype = _qk_operands(q, k, q_weight, k_weight, cos, sin)
+    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    _check(_lib.vq_qk_norm_rope_fwd(q.data_ptr(), _strides(q, 3), q.shape[2], k.data_ptr(), _strides(k, 3), k.shape[2],
+                                    wq.data_ptr(), wk.data_ptr(), int(wq.dtype == torch.float32), c.data_ptr(),
+                                    s.data_ptr(), _strides(c, 2), int(c.dtype == torch.float32), B, S, D, R, float(eps),
+                                    float(weight_offset), dtype, qo.data_ptr(), ko.data_ptr(), _stream(q)))
+    return qo, ko
+
+
+def qk_norm_rope_bwd(gq: torch.Tensor, gk: torch.Tensor, q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
+                     k_weight: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, eps: float,
+                     weight_offset: float = 0.0, want_weight_grads: bool = True):
+    """(dq, dk, dq_weight, dk_weight) of ``qk_norm_rope_fwd`` for the outputs' gradients gq, gk; the weights' are
+    None unless wanted."""
+    dts = q_weight.dtype, k_weight.dtype
+    q, k, wq, wk, c, s, (B, S, D, R), dtype = _qk_operands(q, k, q_weight, k_weight, cos, sin)
+    if gq.shape != q.shape or gk.shape != k.shape or gq.dtype != q.dtype or gk.dtype != q.dtype:
+        raise ValueError(f"qk_norm_rope: gradients of the outputs' shapes and type expected, got {tuple(gq.shape)} "
+                         f"{gq.dtype} and {tuple(gk.shape)} {gk.dtype}")
+    _require_one_device(q, gq, gk)
+    gq, gk = _heads_operand(gq), _heads_operand(gk)
+    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    dwq = dwk = ws = None
+    need = 0
+    if want_weight_grads:
+        dwq, dwk = torch.empty_like(wq), torch.empty_like(wk)
+        need = int(_lib.vq_qk_norm_rope_workspace_bytes(D))
+        ws = torch.empty(max(need, 4), dtype=torch.uint8, device=q.device)
+    _check(_lib.vq_qk_norm_rope_bwd(gq.data_ptr(), _strides(gq, 3), gk.data_ptr(), _strides(gk, 3), q.data_ptr(),
+                                    _strides(q, 3), q.shape[2], k.data_ptr(), _strides(k, 3), k.shape[2], wq.data_ptr(),
+                                    wk.data_ptr(), int(wq.dtype == torch.float32), c.data_ptr(), s.data_ptr(),
+                                    _strides(c, 2), int(c.dtype == torch.float32), B, S, D, R, float(eps),
+                                    float(weight_offset), dtype, dq.data_ptr(), dk.data_ptr(), _ptr(dwq), _ptr(dwk),
+                                    _ptr(ws), need, _stream(q)))
+    if want_weight_grads:
+        dwq, dwk = dwq.to(dts[0]), dwk.to(dts[1])
+    return dq, dk, dwq, dwk
+
+
+# ---------------------------------------------------------------- gated embedding
+def _table_operands(ids, qtypes, qbytes, rows: int, padded_cols: int, cols: int):
+    _require_cuda(ids, *qbytes)
+    _require_one_device(ids, *qbytes)
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"token ids must be int64 or int32, got {ids.dtype}")
+    if not 1 <= len(qtypes) <= 8 or len(qtypes) != len(qbytes):
+        raise ValueError(f"1..8 candidates with their blocks expected, got {len(qtypes)} types and {len(qbytes)} tensors")
+    if rows < 0 or cols < 0 or cols > padded_cols or padded_cols % 256:
+        raise ValueError(f"table of {rows} rows: {padded_cols} stored columns must be a multiple of 256 that holds {cols}")
+    for qt, qb in zip(qtypes, qbytes):
+        if qt not in GGML_TYPE:
+            raise ValueError(f"Unknown quant type: {qt}. Supported: {list(GGML_TYPE)}")
+        be, bb = format_info(qt)
+        if qb.dtype != torch.uint8 or not qb.is_contiguous() or qb.numel() != rows * (padded_cols // be) * bb:
+            raise ValueError(f"{qt}: contiguous uint8 blocks of {rows * (padded_cols // be) * bb} bytes expected, got "
+                             f"{qb.dtype} {tuple(qb.shape)}")
+    return ids.contiguous()
+
+
+def embed_mix(ids: torch.Tensor, qtypes, qbytes, probs: torch.Tensor, rows: int, padded_cols: int, cols: int,
+              scale: float = 1.0, vocab_start: int | None = None) -> torch.Tensor:
+    """Rows scale * sum_k probs[k] W_k[ids] of a table of packed candidates -> bf16 [*ids.shape, cols].  With
+    ``vocab_start`` the table holds the vocabulary from there on and tokens of other shards get rows of zeros;
+    without it such ids are reported by ``device_error`` as well."""
+    ids = _table_operands(ids, qtypes, qbytes, rows, padded_cols, cols)
+    if probs.numel() != len(qtypes):
+        raise ValueError(f"{len(qtypes)} probabilities expected, got {tuple(probs.shape)}")
+    _require_cuda(probs)
+    _require_one_device(ids, probs)
+    K, types, ptrs = _cand_arrays(qtypes, qbytes)
+    p = probs.detach().to(torch.float32).contiguous()
+    out = torch.empty(*ids.shape, cols, dtype=torch.bfloat16, device=ids.device)
+    _check(_lib.vq_embed_mix(K, types, ptrs, p.data_ptr(), ids.data_ptr(), int(ids.dtype == torch.int32), ids.numel(),
+                             vocab_start or 0, rows, padded_cols, cols, float(scale), int(vocab_start is None),
+                             out.data_ptr(), cols, _stream(ids)))
+    return out
+
+
+def token_sort(ids: torch.Tensor, rows: int, vocab_start: int = 0):
+    """(keys, order), int32 [T]: the tokens' rows in ascending order (``rows`` for ids outside the table, last) and
+    the position that each came from; equal tokens keep their order."""
+    _require_cuda(ids)
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"token ids must be int64 or int32, got {ids.dtype}")
+    ids = ids.contiguous().reshape(-1)
+    T = ids.numel()
+    buf = torch.empty(4, T, dtype=torch.int32, device=ids.device)
+    _check(_lib.vq_token_sort(ids.data_ptr(), int(ids.dtype == torch.int32), T, vocab_start, rows, buf[0].data_ptr(),
+                              buf[1].data_ptr(), buf[2].data_ptr(), buf[3].data_ptr(), _stream(ids)))
+    return buf[0], buf[1]
+
+
+def embed_gategrad(dy: torch.Tensor, ids: torch.Tensor, qtypes, qbytes, rows: int, padded_cols: int, cols: int,
+                   scale: float = 1.0, vocab_start: int | None = None) -> torch.Tensor:
+    """grad[k] = scale * sum_t <dy[t], W_k[ids[t]]> (float32 [K]) for dy [*ids.shape, cols] in float32, bfloat16 or
+    float16; ids outside the table add nothing."""
+    ids = _table_operands(ids, qtypes, qbytes, rows, padded_cols, cols)
+    _require_cuda(dy)
+    _require_one_device(ids, dy)
+    code = _float_code(dy, "embed_gategrad")
+    if tuple(dy.shape) != (*ids.shape, cols):
+        raise ValueError(f"gradient of shape {(*ids.shape, cols)} expected, got {tuple(dy.shape)}")
+    T = ids.numel()
+    dy = dy.reshape(T, cols)
+    if dy.stride(-1) != 1 or dy.stride(0) < cols:
+        dy = dy.contiguous()
+    K, types, ptrs = _cand_arrays(qtypes, qbytes)
+    need = int(_lib.vq_embed_gategrad_workspace_bytes(T, K))
+    ws = torch.empty(max(need, 4), dtype=torch.uint8, device=ids.device)
+    g = torch.empty(K, dtype=torch.float32, device=ids.device)
+    _check(_lib.vq_embed_gategrad(K, types, ptrs, ids.data_ptr(), int(ids.dtype == torch.int32), T, vocab_start or 0,
+                                  rows, padded_cols, cols, float(scale), dy.data_ptr(), max(dy.stride(0), cols), code,
+                                  ws.data_ptr(), need, g.data_ptr(), _stream(ids)))
+    return g
+
+
+# ---------------------------------------------------------------- global norm and clipping
+def clip_grad_norm(tensors, max_norm: float = float("inf"), norm_inf: bool = False) -> torch.Tensor:
+    """Global 2-norm (or largest magnitude) of dense, non-overlapping CUDA tensors as a float32 scalar on their device,
+    and every value times min(1, max_norm / (norm + 1e-6)) in place; an infinite ``max_norm`` leaves them as they are."""
+    n = len(tensors)
+    if n == 0:
+        raise ValueError("clip_grad_norm: no tensors")
+    _require_cuda(*tensors)
+    dev = tensors[0].device
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    try:
+        codes = [_FLOAT_CODE[t.dtype] for t in tensors]
+    except KeyError as e:
+        raise ValueError(f"clip_grad_norm: float32, bfloat16 or float16 expected, got {e.args[0]}") from None
+    for t in tensors:
+        if t.device != dev or not t.is_contiguous():
+            raise ValueError("clip_grad_norm: contiguous tensors on one device expected")
+    need = int(_lib.vq_clip_grad_norm_workspace_bytes(n))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    _check(_lib.vq_clip_grad_norm(n, (_vp * n)(*[t.data_ptr() for t in tensors]),
+                                  (ctypes.c_int64 * n)(*[t.numel() for t in tensors]), (_int * n)(*codes),
+                                  float(max_norm), int(norm_inf), ws.data_ptr(), need, norm.data_ptr(), _stream(norm)))
+    return norm

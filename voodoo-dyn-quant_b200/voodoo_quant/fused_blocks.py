@@ -8,7 +8,10 @@ views) and the SwiGLU product run as separate torch kernels, forward and
 backward: a third of an 8B step's device time and over half of a 0.6B step's.
 ``fuse_llama_blocks`` routes those three through one-pass CUDA kernels of
 ``libvoodoo_b200`` (``vq_rmsnorm_fwd/bwd``, ``vq_rope``,
-``vq_swiglu_fwd/bwd``).  The attention itself stays torch's
+``vq_swiglu_fwd/bwd``).  ``fuse_qwen3_blocks`` does the same for the Qwen3
+block, whose attention also normalises every query and key head before the
+rotation: norm and rotation are one kernel there (``vq_qk_norm_rope_fwd/bwd``).
+The attention itself stays torch's
 ``scaled_dot_product_attention`` (cuDNN on B200), called as the Hugging Face
 ``sdpa`` path calls it for a causal, unpadded, cache-free training batch.
 
@@ -24,6 +27,7 @@ import types
 import torch
 import torch.nn.functional as F
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from voodoo_quant import _C
 
@@ -93,6 +97,29 @@ class _RopeFn(Function):
         return dq, dk, None, None
 
 
+class _QKNormRopeFn(Function):
+    """Norm of each query and key head and its rotation; the backward reads
+    the heads before the norm again instead of keeping the normed ones."""
+
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, cos, sin, eps: float, weight_offset: float):
+        qo, ko = _C.qk_norm_rope_fwd(q, k, q_weight, k_weight, cos, sin, eps, weight_offset)
+        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin)
+        ctx.args = (eps, weight_offset)
+        return qo, ko
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gq: torch.Tensor, gk: torch.Tensor):
+        q, k, q_weight, k_weight, cos, sin = ctx.saved_tensors
+        eps, offset = ctx.args
+        need = ctx.needs_input_grad
+        dq, dk, dwq, dwk = _C.qk_norm_rope_bwd(gq, gk, q, k, q_weight, k_weight, cos, sin, eps, offset,
+                                               want_weight_grads=need[2] or need[3])
+        return (dq if need[0] else None, dk if need[1] else None, dwq if need[2] else None, dwk if need[3] else None,
+                None, None, None, None)
+
+
 class _SwiGLUFn(Function):
     @staticmethod
     def forward(ctx, gate: torch.Tensor, up: torch.Tensor):
@@ -159,6 +186,18 @@ def rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor)
     return _RopeFn.apply(q, k, cos, sin)
 
 
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, cos: torch.Tensor,
+                 sin: torch.Tensor, eps: float = 1e-6, weight_offset: float = 0.0):
+    """RMSNorm of every head of q [B, S, Hq, D] and k [B, S, Hk, D] with weights ``weight_offset + weight`` [D], then
+    the rotary embedding of its first R values with cos / sin [B or 1, S, R] (R < D leaves the rest of a head
+    unturned), in one pass; contiguous [B, S, H, D] outputs of q's type, rounded once.  q and k in float32, bfloat16
+    or float16 with any strides; weights and tables of any of the three.  Differentiable in q, k and the weights; cos
+    and sin are constants.  D and R are multiples of 16, D up to 512."""
+    if cos.requires_grad or sin.requires_grad:
+        raise ValueError("qk_norm_rope: cos and sin are constants; they cannot require a gradient")
+    return _QKNormRopeFn.apply(q, k, q_weight, k_weight, cos, sin, float(eps), float(weight_offset))
+
+
 def swiglu(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     return _SwiGLUFn.apply(gate, up)
 
@@ -192,8 +231,21 @@ def _mlp_forward(self, x: torch.Tensor) -> torch.Tensor:
     return self.down_proj(swiglu(g, u))
 
 
+def _head_norms_fusable(attn, hidden_states: torch.Tensor) -> bool:
+    """Whether an attention with head norms can run them fused with the
+    rotation: both norms with one eps, no attention window shorter than the
+    batch and no dropout."""
+    window = getattr(attn, "sliding_window", None)
+    return (attn.head_dim <= 512 and attn.q_norm.variance_epsilon == attn.k_norm.variance_epsilon
+            and (window is None or hidden_states.shape[1] <= window)
+            and not (attn.training and getattr(attn, "attention_dropout", 0.0)))
+
+
 def _attention_forward(self, hidden_states: torch.Tensor, position_embeddings=None, attention_mask=None,
                        past_key_values=None, **kwargs):
+    if getattr(self, "q_norm", None) is not None and not _head_norms_fusable(self, hidden_states):
+        return self._vq_orig_forward(hidden_states, position_embeddings=position_embeddings,
+                                     attention_mask=attention_mask, past_key_values=past_key_values, **kwargs)
     if getattr(self, "_vq_causal_batches", False) and past_key_values is None:
         # batches of the distillation step are causal and unpadded: the only
         # mask Hugging Face builds for them is the causal one, which it
@@ -220,7 +272,10 @@ def _attention_forward(self, hidden_states: torch.Tensor, position_embeddings=No
         k = self.k_proj(hidden_states).view(B, S, -1, self.head_dim)
         v = self.v_proj(hidden_states).view(B, S, -1, self.head_dim)
     cos, sin = position_embeddings
-    q, k = rope(q, k, cos, sin)
+    if getattr(self, "q_norm", None) is not None:
+        q, k = qk_norm_rope(q, k, self.q_norm.weight, self.k_norm.weight, cos, sin, self.q_norm.variance_epsilon)
+    else:
+        q, k = rope(q, k, cos, sin)
     o = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), is_causal=S > 1,
                                        scale=self.scaling, enable_gqa=q.shape[2] != k.shape[2])
     o = o.transpose(1, 2).reshape(B, S, -1)
@@ -307,7 +362,8 @@ def _chained_model_forward(self, input_ids=None, attention_mask=None, position_i
     if not plain:
         plain = not (_norm_weights_fusable(self.norm) and all(
             hasattr(l, "_vq_orig_forward") and hasattr(l.self_attn, "_vq_orig_forward")
-            and hasattr(l.mlp, "_vq_orig_forward") and _norm_weights_fusable(l.input_layernorm)
+            and hasattr(l.mlp, "_vq_orig_forward") and getattr(l.self_attn, "sliding_window", None) is None
+            and _norm_weights_fusable(l.input_layernorm)
             and _norm_weights_fusable(l.post_attention_layernorm) for l in layers))
     if plain:
         return self._vq_chain_orig_forward(input_ids=input_ids, attention_mask=attention_mask,
@@ -349,20 +405,36 @@ def fuse_llama_blocks(model: torch.nn.Module, causal_batches: bool = False) -> i
     (``_chained_model_forward``)."""
     from transformers.models.llama import modeling_llama as L
 
-    table = ((L.LlamaRMSNorm, _rmsnorm_forward), (L.LlamaAttention, _attention_forward),
-             (L.LlamaMLP, _mlp_forward), (L.LlamaDecoderLayer, _decoder_forward))
+    return _fuse_blocks(model, causal_batches, L.LlamaRMSNorm, L.LlamaAttention, L.LlamaMLP, L.LlamaDecoderLayer,
+                        L.LlamaModel)
+
+
+def fuse_qwen3_blocks(model: torch.nn.Module, causal_batches: bool = False) -> int:
+    """``fuse_llama_blocks`` for a Hugging Face Qwen3 model, whose attention
+    normalises every query and key head: norm and rotation run as one kernel
+    (``qk_norm_rope``).  Layers with an attention window shorter than the
+    batch keep their own attention."""
+    from transformers.models.qwen3 import modeling_qwen3 as Q
+
+    return _fuse_blocks(model, causal_batches, Q.Qwen3RMSNorm, Q.Qwen3Attention, Q.Qwen3MLP, Q.Qwen3DecoderLayer,
+                        Q.Qwen3Model)
+
+
+def _fuse_blocks(model, causal_batches: bool, norm_cls, attention_cls, mlp_cls, layer_cls, model_cls) -> int:
+    table = ((norm_cls, _rmsnorm_forward), (attention_cls, _attention_forward), (mlp_cls, _mlp_forward),
+             (layer_cls, _decoder_forward))
     n = 0
     for m in model.modules():
         for cls, fwd in table:
             if type(m) is cls and not hasattr(m, "_vq_orig_forward"):
-                if cls is L.LlamaMLP and getattr(m.config, "hidden_act", "silu") not in ("silu", "swish"):
+                if cls is mlp_cls and getattr(m.config, "hidden_act", "silu") not in ("silu", "swish"):
                     continue
                 m._vq_orig_forward = m.forward
                 m.forward = types.MethodType(fwd, m)
                 n += 1
-        if type(m) is L.LlamaAttention and causal_batches:
+        if type(m) is attention_cls and causal_batches:
             m._vq_causal_batches = True
-        if type(m) is L.LlamaModel and causal_batches and not hasattr(m, "_vq_chain_orig_forward"):
+        if type(m) is model_cls and causal_batches and not hasattr(m, "_vq_chain_orig_forward"):
             m._vq_chain_orig_forward = m.forward
             m.forward = types.MethodType(_chained_model_forward, m)
             n += 1
@@ -401,21 +473,22 @@ def _sp_model_forward(self, input_ids=None, attention_mask=None, position_ids=No
 
 
 def use_sequence_parallel(model: torch.nn.Module) -> int:
-    """Let a tensor-parallel Hugging Face Llama model run sequence parallel
+    """Let a tensor-parallel Hugging Face Llama or Qwen3 model run sequence parallel
     while ``parallel.enable_sequence_parallel`` is on: its LlamaModel forward
     becomes ``_sp_model_forward`` and every decoder layer's forward
     ``_decoder_forward`` (the layers of ``fuse_llama_blocks``, also where the
     fused kernels do not apply).  Idempotent; returns the number of modules
     patched."""
     from transformers.models.llama import modeling_llama as L
+    from transformers.models.qwen3 import modeling_qwen3 as Q
 
     n = 0
     for m in model.modules():
-        if type(m) is L.LlamaModel and not hasattr(m, "_vq_sp_orig_forward"):
+        if type(m) in (L.LlamaModel, Q.Qwen3Model) and not hasattr(m, "_vq_sp_orig_forward"):
             m._vq_sp_orig_forward = m.forward
             m.forward = types.MethodType(_sp_model_forward, m)
             n += 1
-        elif type(m) is L.LlamaDecoderLayer and not hasattr(m, "_vq_orig_forward"):
+        elif type(m) in (L.LlamaDecoderLayer, Q.Qwen3DecoderLayer) and not hasattr(m, "_vq_orig_forward"):
             m._vq_orig_forward = m.forward
             m.forward = types.MethodType(_decoder_forward, m)
             n += 1

@@ -32,6 +32,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 import voodoo_quant
 from voodoo_quant import _C
@@ -707,6 +708,46 @@ class _GatedEmbeddingRowsFunction(Function):
         return out, None, None, None
 
 
+class _GatedEmbeddingFunction(Function):
+    """Token rows of a gated table in one kernel, its gate gradient over the
+    sorted tokens in another (``vq_embed_mix``, ``vq_embed_gategrad``): no
+    gathered blocks, no decoded rows, no host round trip."""
+
+    @staticmethod
+    def forward(ctx, probs: torch.Tensor, ids: torch.Tensor, qtypes: tuple, rows: int, padded_cols: int, cols: int,
+                scale: float, vocab_start: int | None, dtype: torch.dtype, *qbytes: torch.Tensor):
+        ctx.save_for_backward(ids, *qbytes)
+        ctx.args = (qtypes, rows, padded_cols, cols, scale, vocab_start, probs.dtype, probs.shape)
+        # the mixture is bf16 everywhere on this path (W_mix); other types hold its bf16 values
+        return _C.embed_mix(ids, qtypes, qbytes, probs, rows, padded_cols, cols, scale, vocab_start).to(dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g: torch.Tensor):
+        ids, *qbytes = ctx.saved_tensors
+        qtypes, rows, padded_cols, cols, scale, vocab_start, pdtype, pshape = ctx.args
+        gp = _C.embed_gategrad(g, ids, qtypes, qbytes, rows, padded_cols, cols, scale, vocab_start)
+        return (gp.to(pdtype).view(pshape), *[None] * (8 + len(qbytes)))
+
+
+def gated_embedding(ids: torch.Tensor, probs: torch.Tensor, candidate_types, candidate_blocks, num_embeddings: int,
+                    embedding_dim: int, scale: float = 1.0, vocab_start: int | None = None,
+                    dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``scale`` times the rows of sum_k probs[k] W_k that the token ``ids`` (int64 or int32, any shape) name, for a
+    table whose K candidates are packed GGUF blocks (uint8, rows padded to a multiple of 256 weights):
+    [*ids.shape, embedding_dim] in ``dtype``.  Differentiable in ``probs``.
+
+    ``vocab_start``: the table is the vocabulary shard of ``num_embeddings`` rows from there on; tokens of other shards
+    get zeros and add nothing to the gradient.  Without it every id must be a row of the table: another one gets zeros
+    and sets the device error word (``_C.device_error``)."""
+    if dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise ValueError(f"gated_embedding: float32, bfloat16 or float16 rows, got {dtype}")
+    if vocab_start is not None and vocab_start < 0:
+        raise ValueError(f"gated_embedding: vocab_start {vocab_start} is negative")
+    return _GatedEmbeddingFunction.apply(probs, ids, tuple(candidate_types), num_embeddings, _padded(embedding_dim),
+                                         embedding_dim, float(scale), vocab_start, dtype, *candidate_blocks)
+
+
 # --------------------------------------------------------------------------- modules
 class _MixedQuantBase(nn.Module):
     """Candidate loading, gates and bookkeeping shared by Linear and Embedding."""
@@ -991,13 +1032,15 @@ class MixedQuantLinear(_MixedQuantBase):
 
 
 class MixedQuantEmbedding(_MixedQuantBase):
-    """Embedding whose table is the softmax mixture of K packed candidates."""
+    """Embedding whose table is the softmax mixture of K packed candidates;
+    ``scale`` multiplies the rows it returns (models that scale their
+    embeddings)."""
 
     def __init__(self, num_embeddings: int, embedding_dim: int, candidate_types: list[str],
                  source_weight: torch.Tensor, imatrix: torch.Tensor | None = None, device=None,
                  lazy: bool = False, tensor_name: str = "unknown", qbytes_device=None, shard_spec=None,
                  full_source_weight: torch.Tensor | None = None, candidate_bytes: dict | None = None,
-                 candidate_bytes_local: bool = False):
+                 candidate_bytes_local: bool = False, scale: float = 1.0):
         super().__init__(candidate_types=candidate_types, source_weight=source_weight,
                          out_features=num_embeddings, in_features=embedding_dim, imatrix=imatrix,
                          device=device, lazy=lazy, tensor_name=tensor_name, qbytes_device=qbytes_device,
@@ -1005,6 +1048,7 @@ class MixedQuantEmbedding(_MixedQuantBase):
                          candidate_bytes=candidate_bytes, candidate_bytes_local=candidate_bytes_local)
         self.num_embeddings = num_embeddings
         self.embedding_dim = embedding_dim
+        self.scale = float(scale)
         if shard_spec is not None and shard_spec.vocab_start is not None:
             self.tp_vocab_start = shard_spec.vocab_start
             self.tp_vocab_end = shard_spec.vocab_start + num_embeddings
@@ -1019,7 +1063,16 @@ class MixedQuantEmbedding(_MixedQuantBase):
             out.append(qb.view(self.num_embeddings, nbpr * info.block_bytes).index_select(0, rows).reshape(-1))
         return out
 
+    def _fused_lookup(self, ids: torch.Tensor, vocab_start: int | None = None) -> torch.Tensor:
+        dev = self._cand_arena.device
+        return gated_embedding(ids.to(dev), self.get_probs().to(dev), self.candidate_types, self._candidate_blocks(),
+                               self.num_embeddings, self.embedding_dim, self.scale, vocab_start, self.source_dtype)
+
     def _embedding_lookup(self, ids: torch.Tensor) -> torch.Tensor:
+        e = self._rows_lookup(ids)
+        return e if self.scale == 1.0 else (e.float() * self.scale).to(e.dtype)
+
+    def _rows_lookup(self, ids: torch.Tensor) -> torch.Tensor:
         dev = self._cand_arena.device
         probs = self.get_probs().to(dev)
         if _STATIC_STATE.enabled:  # one row per token: no host round trip
@@ -1040,9 +1093,14 @@ class MixedQuantEmbedding(_MixedQuantBase):
 
     def forward(self, input: torch.Tensor) -> torch.Tensor:
         spec = self.shard_spec
+        # one kernel for the mixture's rows; PTQR keeps one candidate per row
+        fused = self._cand_arena.is_cuda and not _PTQR_STATE.enabled
         if spec is not None and spec.vocab_start is not None:
             from voodoo_quant.parallel import sp_enabled, tp_all_reduce_sum_
             v0, v1 = self.tp_vocab_start, self.tp_vocab_end
+            if fused:  # zeros for other shards' tokens
+                emb = self._fused_lookup(input, v0)
+                return emb if sp_enabled() else tp_all_reduce_sum_(emb)
             ids = input.to(self._cand_arena.device)
             in_shard = (ids >= v0) & (ids < v1)
             if _STATIC_STATE.enabled:
@@ -1058,7 +1116,7 @@ class MixedQuantEmbedding(_MixedQuantBase):
             emb = emb_in.new_zeros(*ids.shape, self.embedding_dim)
             emb[in_shard] = emb_in
             return emb if sp_enabled() else tp_all_reduce_sum_(emb)
-        return self._embedding_lookup(input)
+        return self._fused_lookup(input) if fused else self._embedding_lookup(input)
 
 
 # --------------------------------------------------------------------------- walkers
@@ -1149,6 +1207,14 @@ def replace_linear_with_mixed_quant(module: nn.Module, candidate_types: list[str
     return replaced
 
 
+def embed_scale(emb: nn.Embedding) -> float:
+    """Factor that an nn.Embedding subclass multiplies its rows by (its
+    ``embed_scale``, in the weight's type, as such a module applies it); 1
+    for a plain embedding."""
+    s = getattr(emb, "embed_scale", None)
+    return 1.0 if s is None else float(torch.as_tensor(s).to(emb.weight.dtype))
+
+
 def replace_embedding_with_mixed_quant(module: nn.Module, candidate_types: list[str] | None, prefix: str = "",
                                        skip_names: Optional[set[str]] = None,
                                        imatrix_dict: Optional[dict[str, torch.Tensor]] = None, device=None,
@@ -1179,7 +1245,7 @@ def replace_embedding_with_mixed_quant(module: nn.Module, candidate_types: list[
                 candidate_bytes=_provided(candidate_provider, full_name,
                                           full_w if full_w is not None else child.weight.data, types,
                                           spec if local else None),
-                candidate_bytes_local=local)
+                candidate_bytes_local=local, scale=embed_scale(child))
             setattr(module, name, new)
             replaced[full_name] = new
         else:

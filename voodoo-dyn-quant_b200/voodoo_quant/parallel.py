@@ -729,7 +729,10 @@ class RowParallelLinear(nn.Linear):
 
 
 class VocabParallelEmbedding(nn.Embedding):
-    """Vocabulary rows sharded; masked lookup + all-reduce."""
+    """Vocabulary rows sharded; masked lookup + all-reduce.  ``embed_scale``
+    (of a module that scales its rows) is kept and applied."""
+
+    embed_scale = None
 
     def __init__(self, weight_slice: torch.Tensor, spec: ShardSpec, full_weight: torch.Tensor):
         super().__init__(spec.local_out, spec.full_in, device="meta", dtype=weight_slice.dtype)
@@ -745,6 +748,8 @@ class VocabParallelEmbedding(nn.Embedding):
         mask = (input < v0) | (input >= v1)
         out = F.embedding((input - v0).clamp(0, self.num_embeddings - 1), self.weight)
         out = out * (~mask).unsqueeze(-1).to(out.dtype)
+        if self.embed_scale is not None:
+            out = out * torch.as_tensor(self.embed_scale).to(out)
         return out if sp_enabled() else tp_all_reduce_sum(out)
 
 
@@ -773,6 +778,7 @@ def _shard_child(parent: nn.Module, name: str, *, row_offset=None, row_len=None,
         spec = ShardSpec(full_out=w.shape[0], full_in=w.shape[1], row_offset=row_offset, row_len=row_len,
                          vocab_start=vocab_start)
         new = VocabParallelEmbedding(spec.slice_weight(w), spec, w)
+        new.embed_scale = getattr(child, "embed_scale", None)
         setattr(parent, name, new)
         return new
     raise TypeError(f"parallel: cannot shard {type(child).__name__} at '{name}'")

@@ -1,0 +1,86 @@
+"""Global gradient norm over many tensors, and clipping, on the B200 kernels.
+
+The reference's step clips its gates' gradients with
+``torch.nn.utils.clip_grad_norm_`` (voodoo_quant/training/trainer.py:2607-2616):
+a norm per tensor, a norm of the norms and a product per tensor.  Here two
+launches (one for a few thousand values) take the norm of all tensors and
+scale them in place (``vq_clip_grad_norm``); nothing is read on the host.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from voodoo_quant import _C
+
+
+def _norm_is_inf(norm_type: float) -> bool:
+    if float(norm_type) not in (2.0, math.inf):
+        raise ValueError(f"norm_type must be 2 or inf, got {norm_type}")
+    return math.isinf(norm_type)
+
+
+def _dense(g: torch.Tensor) -> torch.Tensor | None:
+    """A contiguous view of all of g's memory, or None where g has gaps or overlaps."""
+    if g.is_contiguous():
+        return g
+    order = sorted(range(g.dim()), key=lambda d: (g.stride(d), g.shape[d]), reverse=True)
+    v = g.permute(order)
+    return v if v.is_contiguous() else None
+
+
+def _run(grads, max_norm: float, norm_type: float) -> torch.Tensor:
+    norm_inf = _norm_is_inf(norm_type)
+    flat, copies = [], []
+    for g in grads:
+        if g.layout != torch.strided:
+            raise ValueError("clip_grad_norm_: dense gradients expected")
+        v = _dense(g)
+        if v is None:  # scaled as a copy
+            if any(st == 0 and n > 1 for st, n in zip(g.stride(), g.shape)):
+                raise ValueError("clip_grad_norm_: an expanded gradient shares memory with itself")
+            v = g.contiguous()
+            copies.append((g, v))
+        flat.append(v)
+    norm = _C.clip_grad_norm(flat, max_norm, norm_inf)
+    if not math.isinf(max_norm):
+        for g, v in copies:
+            g.copy_(v)
+    return norm
+
+
+def grad_norm(grads, norm_type: float = 2.0) -> torch.Tensor:
+    """Global norm of ``grads`` (CUDA tensors in float32, bfloat16 or float16, mixed freely, on one device) as a
+    float32 scalar on that device; ``norm_type`` 2 or inf."""
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    if not grads:
+        return torch.tensor(0.0)
+    with torch.no_grad():
+        return _run(grads, math.inf, norm_type)
+
+
+def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0,
+                    error_if_nonfinite: bool = False) -> torch.Tensor:
+    """Scale the gradients of ``parameters`` in place so that their global norm is at most ``max_norm`` and return the
+    norm they had (a float32 scalar on their device), as ``torch.nn.utils.clip_grad_norm_`` does: every value times
+    min(1, max_norm / (norm + 1e-6)), a norm that is not finite included (NaN gives NaN, inf gives zeros and NaN).
+    An infinite ``max_norm`` leaves the gradients as they are.  ``error_if_nonfinite`` reads the norm on the host and
+    raises RuntimeError before anything is scaled.  Parameters without a gradient are skipped; ``norm_type`` 2 or inf;
+    gradients that share memory are refused."""
+    params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    grads = [p.grad for p in params if p.grad is not None]
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must not be negative or NaN, got {max_norm}")
+    if not grads:
+        _norm_is_inf(norm_type)
+        return torch.tensor(0.0)
+    with torch.no_grad():
+        if error_if_nonfinite:
+            norm = _run(grads, math.inf, norm_type)
+            if not bool(torch.isfinite(norm)):
+                raise RuntimeError(f"The total norm of order {float(norm_type)} for gradients from `parameters` is "
+                                   "non-finite, so it cannot be clipped")
+        return _run(grads, max_norm, norm_type)

@@ -117,9 +117,10 @@ def q8_swiglu_group(gate, up, x: torch.Tensor) -> torch.Tensor:
 class Q8Embedding(nn.Module):
     """nn.Embedding stand-in holding Q8_0 bytes; decodes the touched rows."""
 
-    def __init__(self, qbytes: torch.Tensor, num_embeddings: int, embedding_dim: int, device=None):
+    def __init__(self, qbytes: torch.Tensor, num_embeddings: int, embedding_dim: int, device=None, scale: float = 1.0):
         super().__init__()
         self.num_embeddings = num_embeddings
+        self.scale = float(scale)
         self.embedding_dim = embedding_dim
         dev = torch.device(device) if device is not None else qbytes.device
         self.register_buffer("qweight", qbytes.reshape(-1, 34).to(dev).contiguous())
@@ -129,7 +130,14 @@ class Q8Embedding(nn.Module):
     def forward(self, ids: torch.Tensor) -> torch.Tensor:
         from voodoo_quant.layers import _STATIC_STATE
 
-        if _STATIC_STATE.enabled:  # one row per token, repeats included: no host round trip
+        if self.qweight.is_cuda:  # decode, scale and place the tokens' rows in one kernel
+            return _C.embed_mix(ids, ["Q8_0"], [self.qweight], self._one, self.num_embeddings, self.embedding_dim,
+                                self.embedding_dim, self.scale)
+        e = self._rows(ids, _STATIC_STATE.enabled)
+        return e if self.scale == 1.0 else (e.float() * self.scale).to(e.dtype)
+
+    def _rows(self, ids: torch.Tensor, static: bool) -> torch.Tensor:
+        if static:  # one row per token, repeats included: no host round trip
             flat = ids.reshape(-1)
             sub = _q8_rows(self.qweight, self.num_embeddings, self.embedding_dim).index_select(0, flat)
             w = _C.mix(["Q8_0"], [sub.reshape(-1)], self._one, flat.numel(), self.embedding_dim,
@@ -174,7 +182,10 @@ def wrap_q8_teacher(model: nn.Module, quantizer: Callable[[torch.Tensor], torch.
             del child
         elif isinstance(child, nn.Embedding):
             w = child.weight.data
-            new = Q8Embedding(quantizer(w), child.num_embeddings, child.embedding_dim, device=w.device)
+            from voodoo_quant.layers import embed_scale
+
+            new = Q8Embedding(quantizer(w), child.num_embeddings, child.embedding_dim, device=w.device,
+                              scale=embed_scale(child))
             if hasattr(child, "tp_vocab_start"):
                 new = _VocabParallelQ8(new, child.tp_vocab_start, child.num_embeddings)
             setattr(model, name, new)

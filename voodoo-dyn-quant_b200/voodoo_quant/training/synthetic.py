@@ -37,6 +37,8 @@ class ModelShape:
     non_attention_candidates: list[str] | None = None
     # sigma of per-row log-normal(0, sigma) scales on every weight matrix (0 = none)
     row_scale_sigma: float = 0.0
+    # norms of the query and key heads (a Qwen3 decoder instead of a Llama one)
+    qk_norm: bool = False
 
 
 # Config 5's seven candidates in the order the configuration lists them.  Its
@@ -52,6 +54,9 @@ SHAPES = {
     # CPU-runnable tiny step
     "tiny": ModelShape(2, 256, 4, 4, 768, 4096, False, candidates=["Q4_K", "Q5_K", "Q6_K", "Q8_0"], batch=2,
                        seq=128, budget=0.45),
+    # the tiny step with head norms and grouped queries
+    "tiny-qk": ModelShape(2, 256, 4, 2, 768, 4096, False, head_dim=64, candidates=["Q4_K", "Q5_K", "Q6_K", "Q8_0"],
+                          batch=2, seq=128, budget=0.45, qk_norm=True),
     # config 3: ~0.6B dense decoder, tied embeddings
     "0.6b": ModelShape(28, 1024, 16, 8, 3072, 151936, True, head_dim=128, batch=8, seq=2048, budget=0.45),
     # config 4: 8B Llama-3 shape
@@ -65,31 +70,35 @@ SHAPES = {
 
 
 def llama_config(shape: ModelShape):
-    from transformers import LlamaConfig
+    from transformers import LlamaConfig, Qwen3Config
 
     kw = dict(vocab_size=shape.vocab, hidden_size=shape.hidden, intermediate_size=shape.ffn,
               num_hidden_layers=shape.layers, num_attention_heads=shape.heads,
               num_key_value_heads=shape.kv_heads, rms_norm_eps=1e-6, rope_theta=1e4,
               tie_word_embeddings=shape.tied, max_position_embeddings=max(shape.seq, 256),
-              attention_bias=False, mlp_bias=False)
+              attention_bias=False)
     if shape.head_dim is not None:
         kw["head_dim"] = shape.head_dim
-    cfg = LlamaConfig(**kw)
+    cfg = Qwen3Config(**kw) if shape.qk_norm else LlamaConfig(**kw, mlp_bias=False)
     cfg._attn_implementation = "sdpa"
     return cfg
 
 
 def build_llama(shape: ModelShape, device, dtype=torch.bfloat16, seed: int = 0):
-    """Random-init LlamaForCausalLM on `device`: every weight N(0, 0.02), norms 1.
+    """Random-init LlamaForCausalLM (``shape.qk_norm``: Qwen3ForCausalLM) on `device`: every weight N(0, 0.02), norms 1.
     With ``shape.row_scale_sigma`` > 0, each row of every weight matrix is then
     scaled by its own log-normal(0, sigma) factor (drawn right after the
     matrix, from the same generator)."""
-    from transformers import LlamaForCausalLM
-    from transformers.models.llama.modeling_llama import LlamaRotaryEmbedding
+    if shape.qk_norm:
+        from transformers import Qwen3ForCausalLM as CausalLM
+        from transformers.models.qwen3.modeling_qwen3 import Qwen3RotaryEmbedding as RotaryEmbedding
+    else:
+        from transformers import LlamaForCausalLM as CausalLM
+        from transformers.models.llama.modeling_llama import LlamaRotaryEmbedding as RotaryEmbedding
 
     cfg = llama_config(shape)
     with torch.device("meta"):
-        model = LlamaForCausalLM(cfg)
+        model = CausalLM(cfg)
     model = model.to_empty(device=device).to(dtype)
     g = torch.Generator(device=device).manual_seed(seed)
     with torch.no_grad():
@@ -101,7 +110,7 @@ def build_llama(shape: ModelShape, device, dtype=torch.bfloat16, seed: int = 0):
                 if shape.row_scale_sigma > 0 and p.dim() == 2:
                     z = torch.randn(p.shape[0], 1, generator=g, device=device, dtype=torch.float32)
                     p.copy_((p.float() * torch.exp(z * shape.row_scale_sigma)).to(dtype))
-    model.model.rotary_emb = LlamaRotaryEmbedding(cfg, device=device)
+    model.model.rotary_emb = RotaryEmbedding(cfg, device=device)
     if shape.tied:
         model.tie_weights()
     return model

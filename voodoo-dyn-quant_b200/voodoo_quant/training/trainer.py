@@ -25,6 +25,7 @@ import torch
 import torch.nn as nn
 
 from voodoo_quant.layers import GateBank, set_ptqr, set_static_shapes
+from voodoo_quant.training.grad_clip import clip_grad_norm_
 from voodoo_quant.training.loss import chunked_head_loss, distillation_loss, tp_distillation_loss
 
 
@@ -333,8 +334,16 @@ class GatedDistillTrainer:
             local = self.teacher(input_ids=x[g * b:(g + 1) * b], use_cache=False).logits
         return redistribute_vocab_shards(local, t, group=_fwd_group())
 
+    def _clip_fused(self) -> bool:
+        """Gates on one CUDA device (the usual case): one launch takes the norm and clips."""
+        dev = self.trainable[0].device
+        return dev.type == "cuda" and all(g.device == dev for g in self.trainable)
+
     def apply_update(self) -> None:
-        torch.nn.utils.clip_grad_norm_(self.trainable, max_norm=1.0)
+        if self._clip_fused():
+            clip_grad_norm_(self.trainable, max_norm=1.0)
+        else:
+            torch.nn.utils.clip_grad_norm_(self.trainable, max_norm=1.0)
         self.optimizer.step()
         self.scheduler.step()
         self.step_idx += 1
@@ -427,7 +436,8 @@ def build_distill(shape_name: str, device, seed: int = 0, args: StepArgs | None 
     both models are sharded by the Llama adapter before replacement, so the
     candidates are packed from the FULL tensors and sliced per rank.  On a
     CUDA device ``fused_blocks`` routes the Llama blocks' RMSNorm, rotary
-    embedding and SwiGLU through the fused kernels (``voodoo_quant.fused_blocks``).
+    embedding and SwiGLU (and, for shapes with ``qk_norm``, the norms of the query
+    and key heads) through the fused kernels (``voodoo_quant.fused_blocks``).
     Under TP with
     ``overlap_sms`` > 0, each attention / MLP block's gate-gradient GEMMs
     run beside the all-reduce of the block's input gradient on a second
@@ -485,10 +495,11 @@ def build_distill(shape_name: str, device, seed: int = 0, args: StepArgs | None 
             tp_patch_model(teacher, verbose=False)
     wrap_q8_teacher(teacher, S.q8_quantizer)
     if fused_blocks and torch.device(device).type == "cuda":
-        from voodoo_quant.fused_blocks import fuse_llama_blocks
+        from voodoo_quant.fused_blocks import fuse_llama_blocks, fuse_qwen3_blocks
 
-        fuse_llama_blocks(base, causal_batches=True)
-        fuse_llama_blocks(teacher, causal_batches=True)
+        fuse = fuse_qwen3_blocks if shape.qk_norm else fuse_llama_blocks
+        fuse(base, causal_batches=True)
+        fuse(teacher, causal_batches=True)
     if tp and TP.enabled:
         from voodoo_quant.parallel import enable_sequence_parallel
 
