@@ -353,28 +353,33 @@ int vq_qk_norm_rope_bwd(const void* gq, const int64_t* gq_strides, const void* g
                         void* dk_weight, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- gated embedding ----
- * out[t, :cols] = bf16(scale * sum_k probs[k] * W_k[ids[t] - vocab_start, :cols]) for T token ids (int64, or
- * int32 when ids_i32), W_k the packed candidates of a table of `rows` rows of padded_cols weights.  An id outside
- * [vocab_start, vocab_start + rows) gives a row of zeros (a token of another vocabulary shard); with `strict` it
- * also sets the device error word (4 << 16 | 30).  For scale 1 the rows are vq_mix's bit for bit.  Replaces the
- * gather, decode and mixture of voodoo_quant/layers.py:669-742 (_MixedEmbeddingRowFunctionLazy) and Q8Embedding's. */
+ * Plan of T token ids (int64, or int32 when ids_i32) over a table of `rows` rows that holds the vocabulary from
+ * vocab_start on: the tokens in the order of their rows (stable; ids outside the table last), cut into pieces of equal
+ * rows and at most 16 tokens.  `plan` (vq_embed_plan_bytes(T), 16-byte aligned) holds int32: the number of pieces P
+ * at byte 0; order[T] from byte 256; then, each from a multiple of 256 bytes, start[P] with T behind the last, and
+ * the pieces' rows key[P] (`rows` for ids outside the table). */
+size_t vq_embed_plan_bytes(int64_t T);
+int vq_embed_plan(const void* ids, int ids_i32, int64_t T, int64_t vocab_start, int64_t rows, void* plan,
+                  size_t plan_bytes, void* stream);
+
+/* out[t, :cols] = bf16(scale * sum_k probs[k] * W_k[ids[t] - vocab_start, :cols]) for T token ids, W_k the packed
+ * candidates of a table of `rows` rows of padded_cols weights.  With a plan of the ids each row is decoded once per
+ * piece (ids itself is not read); without (plan NULL) once per token.  An id outside [vocab_start, vocab_start + rows)
+ * gives a row of zeros (a token of another vocabulary shard); with `strict` it also sets the device error word
+ * (4 << 16 | 30).  For scale 1 the rows are vq_mix's bit for bit.  Replaces the gather, decode and mixture of
+ * _MixedEmbeddingRowFunctionLazy, voodoo_quant/layers.py:670-750, and Q8Embedding's, training/q8_teacher.py:156-173. */
 int vq_embed_mix(int K, const int* types, const void* const* blocks, const float* probs, const void* ids, int ids_i32,
-                 int64_t T, int64_t vocab_start, int64_t rows, int64_t padded_cols, int64_t cols, float scale, int strict,
-                 void* out, int64_t ldo, void* stream);
+                 int64_t T, const void* plan, size_t plan_bytes, int64_t vocab_start, int64_t rows, int64_t padded_cols,
+                 int64_t cols, float scale, int strict, void* out, int64_t ldo, void* stream);
 
-/* Stable sort of the tokens by their row: keys[i] = row of the i-th token in ascending order (`rows` for ids of
- * other shards, which come last), order[i] = its position.  keys_tmp / order_tmp: T ints each of scratch. */
-int vq_token_sort(const void* ids, int ids_i32, int64_t T, int64_t vocab_start, int64_t rows, int* keys, int* order,
-                  int* keys_tmp, int* order_tmp, void* stream);
-
-/* grad[k] = scale * sum_t <dy[t], W_k[ids[t] - vocab_start]> over the ids of this table (dy_dtype 0 = float32,
- * 1 = bfloat16, 2 = float16): the rows of dy of equal tokens are summed first, so every distinct row is decoded
- * once.  Sums over rows are held in 64 bits and joined in a fixed order.  `workspace`:
- * vq_embed_gategrad_workspace_bytes(T, K), 16-byte aligned. */
-size_t vq_embed_gategrad_workspace_bytes(int64_t T, int K);
-int vq_embed_gategrad(int K, const int* types, const void* const* blocks, const void* ids, int ids_i32, int64_t T,
-                      int64_t vocab_start, int64_t rows, int64_t padded_cols, int64_t cols, float scale, const void* dy,
-                      int64_t lddy, int dy_dtype, void* workspace, size_t workspace_bytes, float* grad, void* stream);
+/* grad[k] = scale * sum_t <dy[t], W_k[ids[t] - vocab_start]> over the planned ids of this table (dy_dtype 0 = float32,
+ * 1 = bfloat16, 2 = float16): the rows of dy of a piece are summed first, so a row is decoded once per piece.  Sums
+ * over pieces are held in 64 bits and joined in a fixed order.  `workspace`: vq_embed_gategrad_workspace_bytes(K),
+ * 16-byte aligned. */
+size_t vq_embed_gategrad_workspace_bytes(int K);
+int vq_embed_gategrad(int K, const int* types, const void* const* blocks, const void* plan, size_t plan_bytes, int64_t T,
+                      int64_t rows, int64_t padded_cols, int64_t cols, float scale, const void* dy, int64_t lddy,
+                      int dy_dtype, void* workspace, size_t workspace_bytes, float* grad, void* stream);
 
 /* ---- global norm and clipping ----
  * norm[0] = sqrt(sum of squares) (or, with norm_inf, the largest magnitude) over n contiguous tensors (HOST arrays:

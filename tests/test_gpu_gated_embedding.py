@@ -97,6 +97,9 @@ def test_lookup_and_gradient_against_64_bits(cuda, T, V, D, types, scale, start,
     out = gated_embedding(ids_d, probs, types, shard, rows, D, scale=scale, vocab_start=start, dtype=dtype)
     assert out.shape == (T, D) and out.dtype == dtype
     _check_lookup(out.detach(), ids, dec, p, scale, start, rows)
+    with torch.no_grad():  # without a plan of the tokens
+        assert torch.equal(out, gated_embedding(ids_d, probs, types, shard, rows, D, scale=scale, vocab_start=start,
+                                                dtype=dtype))
     if scale == 1.0:
         here = (ids >= start) & (ids < start + rows)
         sub = [b.view(rows, -1)[(ids[here] - start).to(cuda)].reshape(-1).contiguous() for b in shard]
@@ -110,7 +113,7 @@ def test_lookup_and_gradient_against_64_bits(cuda, T, V, D, types, scale, start,
 
 
 @pytest.mark.parametrize("T,rows", [(1, 1), (5, 3), (1024, 511), (1025, 512), (4097, 70000), (20000, 200), (70001, 151936)])
-def test_token_sort_is_stable(cuda, T, rows):
+def test_plan_is_a_stable_sort_in_pieces(cuda, T, rows):
     from voodoo_quant import _C
 
     g = torch.Generator(device="cpu").manual_seed(T)
@@ -119,9 +122,20 @@ def test_token_sort_is_stable(cuda, T, rows):
     local = ids - start
     keys = torch.where((local >= 0) & (local < rows), local, torch.full_like(local, rows))
     want, order = torch.sort(keys, stable=True)
+    head = torch.ones(T, dtype=torch.bool)
+    head[1:] = want[1:] != want[:-1]
+    head |= torch.arange(T) % 16 == 0
+    at = head.nonzero()[:, 0]
+    step = (4 * T + 255) // 256 * 64
     for dt in (torch.int64, torch.int32):
-        k, o = _C.token_sort(ids.to(dt).to(cuda), rows, start)
-        assert torch.equal(k.cpu().long(), want) and torch.equal(o.cpu().long(), order)
+        plan = _C.embed_plan(ids.to(dt).to(cuda), rows, start).view(torch.int32).cpu().long()
+        P = int(plan[0])
+        second = 64 + step
+        third = second + (4 * (T + 1) + 255) // 256 * 64
+        assert P == at.numel()
+        assert torch.equal(plan[64:64 + T], order)
+        assert torch.equal(plan[second:second + P], at) and plan[second + P] == T
+        assert torch.equal(plan[third:third + P], want[at])
 
 
 def test_one_token_for_all_and_one_shard_without_any(cuda):
@@ -135,12 +149,14 @@ def test_one_token_for_all_and_one_shard_without_any(cuda):
     ids = torch.full((T,), 7)
     g = torch.Generator(device="cpu").manual_seed(1)
     dy = torch.randn(T, D, generator=g).to(torch.bfloat16)
-    grad = _C.embed_gategrad(dy.to(cuda), ids.to(cuda), types, blocks, V, D, D)
+    grad = _C.embed_gategrad(dy.to(cuda), _C.embed_plan(ids.to(cuda), V), types, blocks, V, D, D)
     _check_grad(grad, dy, ids, dec, 1.0, 0, V)
-    none = _C.embed_gategrad(dy.to(cuda), ids.to(cuda), types, blocks, V, D, D, vocab_start=100)
+    plan = _C.embed_plan(ids.to(cuda), V, 100)
+    none = _C.embed_gategrad(dy.to(cuda), plan, types, blocks, V, D, D)
     assert torch.equal(none, torch.zeros_like(none))
-    out = _C.embed_mix(ids.to(cuda), types, blocks, p.to(cuda), V, D, D, vocab_start=100)
-    assert not out.any() and _C.device_error() == 0
+    for q in (plan, None):
+        assert not _C.embed_mix(ids.to(cuda), types, blocks, p.to(cuda), V, D, D, vocab_start=100, plan=q).any()
+    assert _C.device_error() == 0
 
 
 def test_ids_outside_the_table(cuda):
@@ -153,13 +169,15 @@ def test_ids_outside_the_table(cuda):
     ids = torch.tensor([3, -1, 19, 20, 2 ** 40, -2 ** 62, 0])
     good = (ids >= 0) & (ids < V)
     assert _C.device_error() == 0
-    out = _C.embed_mix(ids.to(cuda), types, blocks, p.to(cuda), V, D, D)
-    assert _C.device_error() == (4 << 16 | 30) and _C.device_error() == 0
-    _check_lookup(out[good.to(cuda)], ids[good], dec, p, 1.0, 0, V)
-    assert not out[~good.to(cuda)].any()
+    plan = _C.embed_plan(ids.to(cuda), V)
+    for q in (plan, None):
+        out = _C.embed_mix(ids.to(cuda), types, blocks, p.to(cuda), V, D, D, plan=q)
+        assert _C.device_error() == (4 << 16 | 30) and _C.device_error() == 0
+        _check_lookup(out[good.to(cuda)], ids[good], dec, p, 1.0, 0, V)
+        assert not out[~good.to(cuda)].any()
     dy = torch.ones(7, D, dtype=torch.bfloat16)
     dy[1] = float("nan")  # of an id that is not in the table
-    grad = _C.embed_gategrad(dy.to(cuda), ids.to(cuda), types, blocks, V, D, D)
+    grad = _C.embed_gategrad(dy.to(cuda), plan, types, blocks, V, D, D)
     _check_grad(grad, dy, ids, dec, 1.0, 0, V)
 
 
@@ -216,11 +234,14 @@ def test_streams_graphs_and_repeats(cuda):
     pd = p.to(cuda)
 
     def call(ids, dy):
-        return (_C.embed_mix(ids, types, blocks, pd, V, D, D), _C.embed_gategrad(dy, ids, types, blocks, V, D, D))
+        plan = _C.embed_plan(ids, V)
+        return (_C.embed_mix(ids, types, blocks, pd, V, D, D), _C.embed_mix(ids, types, blocks, pd, V, D, D, plan=plan),
+                _C.embed_gategrad(dy, plan, types, blocks, V, D, D))
 
     want = [call(*s) for s in sets]
     again = [call(*s) for s in sets]
     assert all(torch.equal(a, b) for x, y in zip(want, again) for a, b in zip(x, y))
+    assert all(torch.equal(x[0], x[1]) for x in want)  # the same rows with a plan and without
     graphs, outs = [], []
     for s in sets:
         g = torch.cuda.CUDAGraph()

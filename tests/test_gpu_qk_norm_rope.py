@@ -204,7 +204,8 @@ def test_another_stream_a_captured_graph_and_repeats(cuda):
     cos, sin = _tables(S, D, torch.bfloat16, cuda)
 
     def call(q, k, gq, gk):
-        return (*_C.qk_norm_rope_fwd(q, k, w, w, cos, sin, 1e-6), *_C.qk_norm_rope_bwd(gq, gk, q, k, w, w, cos, sin, 1e-6))
+        qo, ko, operands, layout = _C.qk_norm_rope_fwd(q, k, w, w, cos, sin, 1e-6, saved=True)
+        return (qo, ko, *_C.qk_norm_rope_bwd(gq, gk, operands, layout))
 
     want = [call(*s) for s in sets]
     side = torch.cuda.Stream()

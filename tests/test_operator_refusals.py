@@ -78,33 +78,40 @@ def test_gated_embedding_refuses():
     lib = _lib()
 
     def mix(types=(8,), ptrs=(ONE,), probs=ONE, ids=ONE, i32=0, T=4, start=0, rows=10, padded=256, cols=256, out=ONE,
-            ldo=256):
+            ldo=256, plan=None, nplan=0):
         K, t, p = _table(types, ptrs)
-        return lib.vq_embed_mix(K, t, p, probs, ids, i32, T, start, rows, padded, cols, 1.0, 1, out, ldo, None)
+        return lib.vq_embed_mix(K, t, p, probs, ids, i32, T, plan, nplan, start, rows, padded, cols, 1.0, 1, out, ldo, None)
 
     for kw, text in ((dict(padded=250), "multiple of 256"), (dict(cols=300, ldo=300), "multiple of 256"),
                      (dict(T=-1), "negative"), (dict(rows=-1), "negative"), (dict(start=-1), "negative"),
                      (dict(ldo=255), "leading dimension"), (dict(ptrs=(None,)), "null block pointer"),
                      (dict(ptrs=(ONE + 1,)), "2-byte aligned"), (dict(types=(8,) * 9, ptrs=(ONE,) * 9), "number of candidates"),
-                     (dict(probs=None), "null pointer"), (dict(ids=ONE + 4), "misaligned"), (dict(T=1 << 31), "too large")):
+                     (dict(probs=None), "null pointer"), (dict(ids=ONE + 4), "misaligned"), (dict(T=1 << 31), "too large"),
+                     (dict(ids=None), "null token ids"), (dict(plan=ONE, nplan=100), "plan of"),
+                     (dict(plan=ONE + 8, nplan=1 << 20), "plan of")):
         _refused(mix(**kw), text)
     K, t, p = _table((99,), (ONE,))
-    assert lib.vq_embed_mix(K, t, p, ONE, ONE, 0, 4, 0, 10, 256, 256, 1.0, 1, ONE, 256, None) == -3
+    assert lib.vq_embed_mix(K, t, p, ONE, ONE, 0, 4, None, 0, 0, 10, 256, 256, 1.0, 1, ONE, 256, None) == -3
     assert mix(T=0) == 0 and mix(cols=0, ldo=0) == 0
 
-    def grad(T=4, cols=256, lddy=256, code=1, dy=ONE, ws=ONE, nbytes=None, out=ONE):
+    def grad(T=4, cols=256, lddy=256, code=1, dy=ONE, ws=ONE, nbytes=None, out=ONE, plan=ONE, nplan=None):
         K, t, p = _table((8,), (ONE,))
-        need = lib.vq_embed_gategrad_workspace_bytes(T, 1) if nbytes is None else nbytes
-        return lib.vq_embed_gategrad(K, t, p, ONE, 0, T, 0, 10, 256, cols, 1.0, dy, lddy, code, ws, need, out, None)
+        need = lib.vq_embed_gategrad_workspace_bytes(1) if nbytes is None else nbytes
+        pb = lib.vq_embed_plan_bytes(T) if nplan is None else nplan
+        return lib.vq_embed_gategrad(K, t, p, plan, pb, T, 10, 256, cols, 1.0, dy, lddy, code, ws, need, out, None)
 
     for kw, text in ((dict(code=5), "dtype"), (dict(lddy=100), "leading dimension"), (dict(dy=None), "null pointer"),
-                     (dict(ws=None), "null pointer"), (dict(nbytes=16), "workspace"), (dict(ws=ONE + 8), "workspace"),
-                     (dict(out=None), "null pointer")):
+                     (dict(ws=None), "workspace"), (dict(nbytes=16), "workspace"), (dict(ws=ONE + 8), "workspace"),
+                     (dict(out=None), "null pointer"), (dict(plan=None), "plan of"), (dict(nplan=256), "plan of")):
         _refused(grad(**kw), text)
-    assert lib.vq_embed_gategrad_workspace_bytes(4, 9) == 0 and lib.vq_embed_gategrad_workspace_bytes(-1, 1) == 0
-    _refused(lib.vq_token_sort(None, 0, 4, 0, 10, ONE, ONE, ONE, ONE, None), "null pointer")
-    _refused(lib.vq_token_sort(ONE, 0, -4, 0, 10, ONE, ONE, ONE, ONE, None), "negative")
-    assert lib.vq_token_sort(None, 0, 0, 0, 10, None, None, None, None, None) == 0
+    assert lib.vq_embed_gategrad_workspace_bytes(9) == 0 and lib.vq_embed_gategrad_workspace_bytes(0) == 0
+    assert lib.vq_embed_plan_bytes(-1) == 0 and lib.vq_embed_plan_bytes(1 << 31) == 0
+    big = 1 << 20
+    _refused(lib.vq_embed_plan(None, 0, 4, 0, 10, ONE, big, None), "null token ids")
+    _refused(lib.vq_embed_plan(ONE, 0, -4, 0, 10, ONE, big, None), "negative")
+    _refused(lib.vq_embed_plan(ONE, 0, 4, 0, 1 << 31, ONE, big, None), "too large")
+    _refused(lib.vq_embed_plan(ONE, 0, 4, 0, 10, ONE, 100, None), "plan of")
+    assert lib.vq_embed_plan(None, 0, 0, 0, 10, None, 0, None) == 0
 
 
 def test_clip_refuses():

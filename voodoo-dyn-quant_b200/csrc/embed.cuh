@@ -7,14 +7,14 @@
 //
 // Neither writes a decoded row of a candidate: the lookup decodes and mixes a
 // token's packed rows in registers, the gradient sums the rows of dy of equal
-// tokens first (token_sort_kernel brings them together) and multiplies the
+// tokens first (token_plan_kernel brings them together) and multiplies the
 // decoded weights into that sum as it decodes them.  Both are bound by HBM
 // (packed rows, and T x D of out or dy), closely followed by the decoding.
 //
-// A warp holds four units (256 weights) of a row, eight lanes a unit, a lane
-// 32 consecutive weights.  The lanes of a unit copy its packed bytes of every
-// candidate into their own slots of shared memory (16-byte asynchronous
-// copies), so that no block-wide barrier is needed.
+// Eight lanes hold a unit (256 weights) of a row, a lane 32 consecutive
+// weights.  The lanes of a unit copy its packed bytes of every candidate into
+// their own slots of shared memory (16-byte asynchronous copies), the next
+// unit's while this one's are decoded, so that no block-wide barrier is needed.
 #pragma once
 
 #include <type_traits>
@@ -26,7 +26,8 @@ namespace embed {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kUnits = 4;  // units of a warp
+constexpr int kUnits = 4;   // units of a warp
+constexpr int kStages = 2;  // of a warp's slots: the next units' bytes arrive while these are decoded
 constexpr int kMaxBlocks = 1184;  // of a gradient launch: the partials it leaves
 
 // A unit's slot: the 16-byte aligned span of a 2-byte aligned unit, and a
@@ -83,43 +84,118 @@ __device__ __forceinline__ long long local_row(long long id, long long vocab_sta
   return r >= 0 && r < rows ? r : -1;
 }
 
+// The tokens of a call in the order of their rows, cut into pieces of equal
+// rows (token_plan_kernel): piece i holds the tokens order[start[i]] to
+// order[start[i + 1] - 1], all naming row key[i].
+struct Plan {
+  int *order, *start, *key, *count;
+};
+
+// Most tokens of a piece: a token that fills much of a batch is then worked
+// on by many warps, each decoding its row again.
+constexpr int kPieceTokens = 16;
+
+// A team's unit: which of a row, and the tokens that want it.
+struct Unit {
+  long long row;     // of the table, -1: of another one
+  long long begin;   // tokens: places in the order, or (kRuns false) the token itself
+  long long end;
+  int u;             // unit of the row
+};
+
+// The units that eight lanes work on one after the other: unit u of piece
+// (or token) i, i * units_per_row + u ascending by a fixed stride.
+template <bool kRuns>
+struct UnitWalk {
+  Plan plan;
+  Ids ids;
+  long long count;  // pieces, or tokens
+  long long vocab_start, rows;
+  int units_per_row;
+  long long i, di;
+  int u, du;
+
+  __device__ __forceinline__ void start_at(long long first, long long stride) {
+    i = first / units_per_row;
+    u = static_cast<int>(first - i * units_per_row);
+    di = stride / units_per_row;
+    du = static_cast<int>(stride - di * units_per_row);
+  }
+  __device__ __forceinline__ bool done() const { return i >= count; }
+  __device__ __forceinline__ void step() {
+    i += di;
+    u += du;
+    if (u >= units_per_row) {
+      u -= units_per_row;
+      ++i;
+    }
+  }
+  __device__ __forceinline__ Unit get() const {
+    Unit n;
+    n.u = u;
+    if (i >= count) {
+      n.row = -1;
+      n.begin = n.end = 0;
+    } else if (kRuns) {
+      const int key = plan.key[i];
+      n.row = key < rows ? key : -1;
+      n.begin = plan.start[i];
+      n.end = plan.start[i + 1];
+    } else {
+      n.row = local_row(ids.at(i), vocab_start, rows);
+      n.begin = i;
+      n.end = i + 1;
+    }
+    return n;
+  }
+};
+
 // ---------------------------------------------------------------- lookup
 // Rows of ids outside [vocab_start, vocab_start + rows) are written as zeros
 // (another shard's tokens); `strict` also reports them.  The mixture is
 // mix_units_kernel's, in the same order, so for scale 1 the rows are those of
-// W_mix bit for bit; the scaled row is rounded to bf16 once.
-__global__ void __launch_bounds__(kThreads) embed_mix_kernel(CandSet cs, const float* __restrict__ probs, Ids ids,
-                                                             long long T, long long vocab_start, long long rows,
-                                                             int units_per_row, int cols, float scale, bool strict,
-                                                             __nv_bfloat16* __restrict__ out, long long ldo, int* err) {
+// W_mix bit for bit; the scaled row is rounded to bf16 once.  kRuns: each row
+// is decoded once per piece of the plan and written to all its tokens;
+// otherwise once per token, with no plan to wait for.
+template <bool kRuns>
+__global__ void __launch_bounds__(kThreads, 2) embed_mix_kernel(CandSet cs, const float* __restrict__ probs, Ids ids,
+                                                                long long T, Plan plan, long long vocab_start,
+                                                                long long rows, int units_per_row, int cols, float scale,
+                                                                bool strict, __nv_bfloat16* __restrict__ out,
+                                                                long long ldo, int* err) {
   extern __shared__ __align__(16) uint8_t esmem[];
   __shared__ float pk_s[kMaxCandidates];
   if (threadIdx.x < cs.K) pk_s[threadIdx.x] = probs[threadIdx.x];
   __syncthreads();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int lu = lane >> 3, c = lane & 7;
-  uint8_t* buf = esmem + warp * warp_bytes(cs);
-  const long long total = T * units_per_row;
+  const int wbytes = warp_bytes(cs);
+  uint8_t* buf = esmem + warp * kStages * wbytes;
+  UnitWalk<kRuns> w{plan, ids, kRuns ? *plan.count : T, vocab_start, rows, units_per_row};
   const long long stride = static_cast<long long>(gridDim.x) * kWarps * kUnits;
+  w.start_at((static_cast<long long>(blockIdx.x) * kWarps + warp) * kUnits + lu, stride);
   bool bad = false, fmt_ok = true;
-  for (long long f0 = (static_cast<long long>(blockIdx.x) * kWarps + warp) * kUnits; f0 < total; f0 += stride) {
-    const long long f = f0 + lu;
-    const bool in = f < total;
-    const long long t = in ? f / units_per_row : 0;
-    const int u = in ? static_cast<int>(f - t * units_per_row) : 0;
-    const long long row = in ? local_row(ids.at(t), vocab_start, rows) : -1;
-    const long long unit = row * units_per_row + u;
-    if (row >= 0) stage_unit(cs, smem_u32(buf), lu, c, unit);
-    bad |= in && row < 0;
+  Unit now = w.get();
+  if (now.row >= 0) stage_unit(cs, smem_u32(buf), lu, c, now.row * units_per_row + now.u);
+  async_commit();
+  w.step();
+  Unit next = w.get();
+  int st = 0;
+  while (__any_sync(0xffffffffu, now.begin < now.end)) {
+    if (next.row >= 0) stage_unit(cs, smem_u32(buf + (st ^ 1) * wbytes), lu, c, next.row * units_per_row + next.u);
     async_commit();
-    async_wait<0>();
+    w.step();
+    const Unit after = w.get();
+    async_wait<1>();
     __syncwarp();
     float2 acc[16];
 #pragma unroll
     for (int j = 0; j < 16; ++j) acc[j] = make_float2(0.f, 0.f);
     float cst[2] = {0.f, 0.f};
-    if (row >= 0) {
-      const uint8_t* region = buf;
+    const int col = 256 * now.u + 32 * c;
+    if (now.row >= 0 && col < cols) {
+      const uint8_t* region = buf + st * wbytes;
+      const long long unit = now.row * units_per_row + now.u;
       for (int k = 0; k < cs.K; ++k) {
         const URef ur = staged(cs, region, k, lu, unit);
         const float pk = pk_s[k];
@@ -136,48 +212,51 @@ __global__ void __launch_bounds__(kThreads) embed_mix_kernel(CandSet cs, const f
         region += kUnits * slot_bytes(cs.ubytes[k]);
       }
     }
-    const int col = 256 * u + 32 * c;
-    if (in && col < cols) {
-      __nv_bfloat16* dst = out + t * ldo + col;
-      if (col + 32 <= cols && (reinterpret_cast<uintptr_t>(dst) & 15u) == 0) {
+    bad |= now.row < 0 && now.begin < now.end;
+    if (col < cols) {
+      __align__(16) __nv_bfloat162 hv[16];
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          __align__(16) __nv_bfloat162 hv[4];
-          const float cs0 = cst[v >> 1];
+      for (int j = 0; j < 16; ++j) {
+        const float cs0 = cst[j >> 3];
+        hv[j] = __floats2bfloat162_rn((acc[j].x + cs0) * scale, (acc[j].y + cs0) * scale);
+      }
+      for (long long i = now.begin; i < now.end; ++i) {
+        __nv_bfloat16* dst = out + (kRuns ? static_cast<long long>(plan.order[i]) : i) * ldo + col;
+        if (col + 32 <= cols && (reinterpret_cast<uintptr_t>(dst) & 15u) == 0) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 e = acc[4 * v + j];
-            hv[j] = __floats2bfloat162_rn((e.x + cs0) * scale, (e.y + cs0) * scale);
+          for (int v = 0; v < 4; ++v) reinterpret_cast<uint4*>(dst)[v] = reinterpret_cast<const uint4*>(hv)[v];
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            if (col + 2 * j < cols) dst[2 * j] = hv[j].x;
+            if (col + 2 * j + 1 < cols) dst[2 * j + 1] = hv[j].y;
           }
-          reinterpret_cast<uint4*>(dst)[v] = *reinterpret_cast<const uint4*>(hv);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float cs0 = cst[j >> 3];
-          if (col + 2 * j < cols) dst[2 * j] = __float2bfloat16_rn((acc[j].x + cs0) * scale);
-          if (col + 2 * j + 1 < cols) dst[2 * j + 1] = __float2bfloat16_rn((acc[j].y + cs0) * scale);
         }
       }
     }
     __syncwarp();  // the slots are filled again
+    now = next;
+    next = after;
+    st ^= 1;
   }
   if (bad && strict) report_error(err, kDevBadIndex, 30);
   if (!fmt_ok) report_error(err, kDevBadFormat, 3);
 }
 
-// ---------------------------------------------------------------- sort
+// ---------------------------------------------------------------- plan
 // Stable radix sort of the tokens' local rows by one cluster, nine bits a
-// pass: keys[i] in ascending order, order[i] the token it came from; tokens of
-// other shards get the key `rows` and so end up last.  Each CTA owns a
-// contiguous slice of the pass's input: its digit counts are read by the
-// others through distributed shared memory, and its tokens are placed a tile
-// of 1024 at a time, ranked within a warp by matching digits.
+// pass, and the pieces of equal rows.  Tokens of other shards get the key
+// `rows` and so end up last.  Each CTA owns a contiguous slice of a pass's
+// input and ranks it a tile of 1024 tokens at a time: within a warp by
+// matching digits, over the warps and tiles by counts; the slices' counts
+// meet through distributed shared memory.  Latency bound: a dozen barriers
+// and the round trips between them.
 constexpr int kSortThreads = 1024;
 constexpr int kSortCtas = 8;  // largest portable cluster
 constexpr int kDigitBits = 9;
 constexpr int kBins = 1 << kDigitBits;
 constexpr int kSortSmem = 32 * kBins * 2;
+constexpr int kKeepTiles = 2;  // tiles whose keys and ranks stay in registers between the two halves of a pass
 
 __device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
   int v;
@@ -185,14 +264,17 @@ __device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
   return v;
 }
 
-__global__ void __launch_bounds__(kSortThreads) token_sort_kernel(Ids ids, int T, long long vocab_start, int rows,
-                                                                  int passes, int* keys, int* order, int* keys_tmp,
+__global__ void __launch_bounds__(kSortThreads) token_plan_kernel(Ids ids, int T, long long vocab_start, int rows,
+                                                                  int passes, Plan plan, int* keys, int* keys_tmp,
                                                                   int* order_tmp) {
   extern __shared__ __align__(16) uint8_t ssmem[];
   uint16_t* wcount = reinterpret_cast<uint16_t*>(ssmem);  // [32 warps][kBins]
-  __shared__ int hist[kBins];
+  __shared__ int count[kBins];                            // this slice's tokens of each digit, so far
   __shared__ int base[kBins];
   __shared__ int wsum[32];
+  __shared__ int pieces;
+  int* order = plan.order;
+  int* ranks = plan.start;  // free until the pieces are written
   uint32_t nctas;
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(nctas));
   const int rank = static_cast<int>(cluster_ctarank());
@@ -211,38 +293,10 @@ __global__ void __launch_bounds__(kSortThreads) token_sort_kernel(Ids ids, int T
       const long long r = local_row(ids.at(i), vocab_start, rows);
       return r < 0 ? rows : static_cast<int>(r);
     };
-    for (int d = tid; d < kBins; d += kSortThreads) hist[d] = 0;
-    __syncthreads();
-    for (int i = b + tid; i < e; i += kSortThreads) atomicAdd(&hist[(key_at(i) >> shift) & (kBins - 1)], 1);
-    cluster_sync();
-    // first place of each digit of this slice: smaller digits, then the same digit in earlier slices
-    int total = 0, before = 0;
-    if (tid < kBins) {
-      for (int r = 0; r < static_cast<int>(nctas); ++r) {
-        const int h = ld_cluster_s32(map_to_rank(smem_u32(&hist[tid]), r));
-        before += r < rank ? h : 0;
-        total += h;
-      }
-    }
-    int x = total;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    if (lane == 31) wsum[warp] = x;
-    __syncthreads();
-    if (tid < kBins) {
-      int ahead = 0;
-      for (int w = 0; w < warp; ++w) ahead += wsum[w];
-      base[tid] = ahead + x - total + before;
-    }
-    for (int i0 = b; i0 < e; i0 += kSortThreads) {
-      const int i = i0 + tid;
-      const bool in = i < e;
-      const int key = in ? key_at(i) : 0;
-      const int tok = in ? (p > 0 ? __ldcg(osrc + i) : i) : 0;
-      const int d = in ? (key >> shift) & (kBins - 1) : kBins;  // no digit
+    auto digit = [&](int key) { return (key >> shift) & (kBins - 1); };
+    // place of token i among this slice's tokens of the same digit
+    auto rank_of = [&](bool in, int key) -> int {
+      const int d = in ? digit(key) : kBins;  // no digit
       uint4* mine = reinterpret_cast<uint4*>(wcount + warp * kBins);
       for (int v = lane; v < kBins / 8; v += 32) mine[v] = make_uint4(0, 0, 0, 0);
       __syncwarp();
@@ -260,16 +314,104 @@ __global__ void __launch_bounds__(kSortThreads) token_sort_kernel(Ids ids, int T
         }
       }
       __syncthreads();
-      if (in) {
-        const int at = base[d] + wcount[warp * kBins + d] + ahead;
-        kdst[at] = key;
-        odst[at] = tok;
-      }
+      const int r = in ? count[d] + wcount[warp * kBins + d] + ahead : 0;
       __syncthreads();
-      if (tid < kBins) base[tid] += run;
+      if (tid < kBins) count[tid] += run;
+      return r;
+    };
+    for (int d = tid; d < kBins; d += kSortThreads) count[d] = 0;
+    int kept_key[kKeepTiles], kept_rank[kKeepTiles];
+#pragma unroll
+    for (int t = 0; t < kKeepTiles; ++t) {
+      const int i0 = b + t * kSortThreads;
+      if (i0 >= e) break;
+      const bool in = i0 + tid < e;
+      kept_key[t] = in ? key_at(i0 + tid) : 0;
+      kept_rank[t] = rank_of(in, kept_key[t]);
+    }
+    for (int i0 = b + kKeepTiles * kSortThreads; i0 < e; i0 += kSortThreads) {
+      const bool in = i0 + tid < e;
+      const int r = rank_of(in, in ? key_at(i0 + tid) : 0);
+      if (in) ranks[i0 + tid] = r;
+    }
+    cluster_sync();
+    // first place of each digit of this slice: smaller digits, then the same digit in earlier slices
+    int total = 0, before = 0;
+    if (tid < kBins) {
+      for (int r = 0; r < static_cast<int>(nctas); ++r) {
+        const int h = ld_cluster_s32(map_to_rank(smem_u32(&count[tid]), r));
+        before += r < rank ? h : 0;
+        total += h;
+      }
+    }
+    int x = total;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) wsum[warp] = x;
+    __syncthreads();
+    if (tid < kBins) {
+      int ahead = 0;
+      for (int w = 0; w < warp; ++w) ahead += wsum[w];
+      base[tid] = ahead + x - total + before;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < kKeepTiles; ++t) {
+      const int i = b + t * kSortThreads + tid;
+      if (i < e) {
+        const int at = base[digit(kept_key[t])] + kept_rank[t];
+        kdst[at] = kept_key[t];
+        odst[at] = p > 0 ? __ldcg(osrc + i) : i;
+      }
+    }
+    for (int i = b + kKeepTiles * kSortThreads + tid; i < e; i += kSortThreads) {
+      const int key = key_at(i);
+      const int at = base[digit(key)] + ranks[i];
+      kdst[at] = key;
+      odst[at] = p > 0 ? __ldcg(osrc + i) : i;
     }
     cluster_sync();  // this pass's keys are written, and nobody reads the counts any more
   }
+  // pieces: where a row begins, and every kPieceTokens-th place of the order
+  auto begins = [&](int i) -> bool {
+    return i < e && (i % kPieceTokens == 0 || __ldcg(keys + i) != __ldcg(keys + i - 1));
+  };
+  int mine = 0;
+  for (int i0 = b; i0 < e; i0 += kSortThreads) mine += __syncthreads_count(begins(i0 + tid));
+  if (tid == 0) pieces = mine;
+  cluster_sync();
+  int at = 0, all = 0;
+  for (int r = 0; r < static_cast<int>(nctas); ++r) {
+    const int n = ld_cluster_s32(map_to_rank(smem_u32(&pieces), r));
+    at += r < rank ? n : 0;
+    all += n;
+  }
+  for (int i0 = b; i0 < e; i0 += kSortThreads) {
+    const int i = i0 + tid;
+    const bool f = begins(i);
+    const uint32_t m = __ballot_sync(0xffffffffu, f);
+    if (lane == 0) wsum[warp] = __popc(m);
+    __syncthreads();
+    int ahead = __popc(m & ((1u << lane) - 1u)), sum = 0;
+    for (int w = 0; w < 32; ++w) {
+      ahead += w < warp ? wsum[w] : 0;
+      sum += wsum[w];
+    }
+    if (f) {
+      plan.start[at + ahead] = i;
+      plan.key[at + ahead] = __ldcg(keys + i);
+    }
+    at += sum;
+    __syncthreads();
+  }
+  if (rank == 0 && tid == 0) {
+    plan.start[all] = T;
+    *plan.count = all;
+  }
+  cluster_sync();  // nobody reads this CTA's shared memory any more
 }
 
 // ---------------------------------------------------------------- gradient
@@ -329,76 +471,79 @@ __device__ __forceinline__ void add_row(const T* row, int col, int cols, float2 
   }
 }
 
-// A warp's work item: `window` sorted tokens and four units of their rows.
-// It sums the rows of dy of each run of equal tokens in registers, then takes
-// the products with every candidate's decoded weights; a run that goes on in
-// the next window is finished there, the products being linear.  Sums over
-// runs are held in 64 bits, in the thread's own place of shared memory (an
-// index that varies would put a register array into local memory), and the
-// block's are left in partials[blockIdx.x][K].
+// Eight lanes take a unit of a piece of the plan: they sum the unit's columns
+// of the rows of dy of the piece's tokens in registers, then multiply every
+// candidate's decoded weights into the sum; a run of equal tokens that is cut
+// into several pieces is finished in each, the products being linear.  Sums
+// over pieces are held in 64 bits, in the thread's own place of shared memory
+// (an index that varies would put a register array into local memory), and
+// the block's are left in partials[blockIdx.x][K].
 template <typename T>
-__global__ void __launch_bounds__(kThreads) embed_gategrad_kernel(CandSet cs, const int* __restrict__ keys,
-                                                                  const int* __restrict__ order, int ntok, int rows,
-                                                                  int units_per_row, int cols, int window,
-                                                                  const T* __restrict__ dy, long long lddy,
-                                                                  double* __restrict__ partials, int* err) {
+__global__ void __launch_bounds__(kThreads, 2) embed_gategrad_kernel(CandSet cs, Plan plan, long long rows,
+                                                                     int units_per_row, int cols,
+                                                                     const T* __restrict__ dy, long long lddy,
+                                                                     double* __restrict__ partials, int* err) {
   extern __shared__ __align__(16) uint8_t esmem[];
   double* acc = reinterpret_cast<double*>(esmem);  // [K][kThreads]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int lu = lane >> 3, c = lane & 7;
-  uint8_t* buf = esmem + cs.K * kThreads * sizeof(double) + warp * warp_bytes(cs);
+  const int wbytes = warp_bytes(cs);
+  uint8_t* buf = esmem + cs.K * kThreads * sizeof(double) + warp * kStages * wbytes;
   for (int k = 0; k < cs.K; ++k) acc[k * kThreads + threadIdx.x] = 0.0;
-  const int groups = (units_per_row + kUnits - 1) / kUnits;
-  const long long items = static_cast<long long>((ntok + window - 1) / window) * groups;
+  UnitWalk<true> w{plan, Ids{nullptr, false}, *plan.count, 0, rows, units_per_row};
+  const long long stride = static_cast<long long>(gridDim.x) * kWarps * kUnits;
+  w.start_at((static_cast<long long>(blockIdx.x) * kWarps + warp) * kUnits + lu, stride);
   bool fmt_ok = true;
-  for (long long item = static_cast<long long>(blockIdx.x) * kWarps + warp; item < items;
-       item += static_cast<long long>(gridDim.x) * kWarps) {
-    const int w = static_cast<int>(item / groups);
-    const int u = static_cast<int>(item - static_cast<long long>(w) * groups) * kUnits + lu;
-    const bool on = u < units_per_row;
-    const int col = 256 * u + 32 * c;
-    int i = w * window;
-    const int end = min(ntok, i + window);
-    while (i < end) {
-      const int key = keys[i];
-      if (key >= rows) break;  // only other shards' tokens follow
-      const long long unit = static_cast<long long>(key) * units_per_row + u;
-      if (on) stage_unit(cs, smem_u32(buf), lu, c, unit);
-      async_commit();
-      float2 g[16];
+  Unit now = w.get();
+  if (now.row >= 0) stage_unit(cs, smem_u32(buf), lu, c, now.row * units_per_row + now.u);
+  async_commit();
+  w.step();
+  Unit next = w.get();
+  int st = 0;
+  while (__any_sync(0xffffffffu, now.row >= 0)) {  // other shards' pieces come last
+    if (next.row >= 0) stage_unit(cs, smem_u32(buf + (st ^ 1) * wbytes), lu, c, next.row * units_per_row + next.u);
+    async_commit();
+    w.step();
+    const Unit after = w.get();
+    const int col = 256 * now.u + 32 * c;
+    const bool on = now.row >= 0 && col < cols;
+    float2 g[16];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) g[j] = make_float2(0.f, 0.f);
-      do {
-        if (on) add_row<T>(dy + static_cast<long long>(order[i]) * lddy, col, cols, g);
-        ++i;
-      } while (i < end && keys[i] == key);
-      float gs[2] = {0.f, 0.f};
+    for (int j = 0; j < 16; ++j) g[j] = make_float2(0.f, 0.f);
+    if (on)
+      for (long long i = now.begin; i < now.end; ++i)
+        add_row<T>(dy + static_cast<long long>(plan.order[i]) * lddy, col, cols, g);
+    float gs[2] = {0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < 16; ++j) gs[j >> 3] += g[j].x + g[j].y;
-      async_wait<0>();
-      __syncwarp();
-      if (on && col < cols) {
-        const uint8_t* region = buf;
-        for (int k = 0; k < cs.K; ++k) {
-          const URef ur = staged(cs, region, k, lu, unit);
-          float d = 0.f;
-          switch (cs.fmt[k]) {
-            case kQ8_0: d = dot_chunk<kQ8_0>(ur, c, g, gs); break;
-            case kQ2_K: d = dot_chunk<kQ2_K>(ur, c, g, gs); break;
-            case kQ3_K: d = dot_chunk<kQ3_K>(ur, c, g, gs); break;
-            case kQ4_K: d = dot_chunk<kQ4_K>(ur, c, g, gs); break;
-            case kQ5_K: d = dot_chunk<kQ5_K>(ur, c, g, gs); break;
-            case kQ6_K: d = dot_chunk<kQ6_K>(ur, c, g, gs); break;
-            case kIQ4_XS: d = dot_chunk<kIQ4_XS>(ur, c, g, gs); break;
-            default: fmt_ok = false;
-          }
-          acc[k * kThreads + threadIdx.x] += static_cast<double>(d);
-          region += kUnits * slot_bytes(cs.ubytes[k]);
+    for (int j = 0; j < 16; ++j) gs[j >> 3] += g[j].x + g[j].y;
+    async_wait<1>();
+    __syncwarp();
+    if (on) {
+      const uint8_t* region = buf + st * wbytes;
+      const long long unit = now.row * units_per_row + now.u;
+      for (int k = 0; k < cs.K; ++k) {
+        const URef ur = staged(cs, region, k, lu, unit);
+        float d = 0.f;
+        switch (cs.fmt[k]) {
+          case kQ8_0: d = dot_chunk<kQ8_0>(ur, c, g, gs); break;
+          case kQ2_K: d = dot_chunk<kQ2_K>(ur, c, g, gs); break;
+          case kQ3_K: d = dot_chunk<kQ3_K>(ur, c, g, gs); break;
+          case kQ4_K: d = dot_chunk<kQ4_K>(ur, c, g, gs); break;
+          case kQ5_K: d = dot_chunk<kQ5_K>(ur, c, g, gs); break;
+          case kQ6_K: d = dot_chunk<kQ6_K>(ur, c, g, gs); break;
+          case kIQ4_XS: d = dot_chunk<kIQ4_XS>(ur, c, g, gs); break;
+          default: fmt_ok = false;
         }
+        acc[k * kThreads + threadIdx.x] += static_cast<double>(d);
+        region += kUnits * slot_bytes(cs.ubytes[k]);
       }
-      __syncwarp();  // the slots are filled again
     }
+    __syncwarp();  // the slots are filled again
+    now = next;
+    next = after;
+    st ^= 1;
   }
+  async_wait<0>();
   if (!fmt_ok) report_error(err, kDevBadFormat, 4);
   __syncthreads();
   for (int k = warp; k < cs.K; k += kWarps) {

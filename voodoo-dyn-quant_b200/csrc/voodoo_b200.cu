@@ -10,6 +10,7 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstdint>
 #include <cmath>
@@ -1139,7 +1140,7 @@ struct QkPlan {
 // blocks.  A warp walks all heads of its side at a position (their table and
 // weight values then stay in registers) unless that leaves fewer warps than
 // the GPU holds at 32 per SM; then the heads are split as far as that needs.
-int qk_plan(QkPlan* p, int64_t positions, int64_t Hq, int64_t Hk, int64_t D) {
+int qk_plan(QkPlan* p, int64_t positions, int64_t Hq, int64_t Hk, int64_t D, int blocks_per_sm) {
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
   p->team_log2 = 0;
@@ -1159,8 +1160,9 @@ int qk_plan(QkPlan* p, int64_t positions, int64_t Hq, int64_t Hk, int64_t D) {
     *chunks[i] = *iters[i] > 0 ? static_cast<int>((all + *iters[i] - 1) / *iters[i]) : 0;
     items[i] = positions * *chunks[i];
   }
-  // blocks of 4 warps, 8 a SM, shared by the sides as their heads are
-  const long long cap = 8LL * sms < vq::qknorm::kMaxBlocks ? 8LL * sms : vq::qknorm::kMaxBlocks;
+  // one wave of blocks, shared by the sides as their heads are
+  const long long wave = static_cast<long long>(blocks_per_sm) * sms;
+  const long long cap = wave < vq::qknorm::kMaxBlocks ? wave : vq::qknorm::kMaxBlocks;
   long long qb = (items[0] + vq::qknorm::kWarps - 1) / vq::qknorm::kWarps;
   long long kb = (items[1] + vq::qknorm::kWarps - 1) / vq::qknorm::kWarps;
   if (qb + kb > cap) {
@@ -1239,12 +1241,28 @@ int launch_qk(const QkArgs& a, const QkPlan& p, float* partials, cudaStream_t st
   Shape sh{};
   sh.cos = a.cos, sh.sin = a.sin;
   sh.cb = a.cs[0], sh.cs = a.cs[1];
-  sh.positions = a.B * a.S;
-  sh.S = static_cast<int>(a.S), sh.D = static_cast<int>(a.D), sh.R = static_cast<int>(a.R);
+  sh.positions = static_cast<unsigned>(a.B * a.S);
+  sh.S = static_cast<unsigned>(a.S), sh.D = static_cast<int>(a.D), sh.R = static_cast<int>(a.R);
   sh.team_log2 = p.team_log2;
   sh.eps = a.eps, sh.offset = a.offset;
-  sh.w_f32 = a.w_f32, sh.cs_f32 = a.cs_f32;
-  qk_norm_rope_kernel<T, kBackward><<<p.q_blocks + p.k_blocks, kThreads, 0, st>>>(q, k, sh, partials);
+  sh.w_f32 = a.w_f32;
+  const int grid = p.q_blocks + p.k_blocks;
+  if constexpr (!kBackward) {
+    if (a.cs_f32)
+      qk_norm_rope_fwd_kernel<T, float><<<grid, kThreads, 0, st>>>(q, k, sh);
+    else
+      qk_norm_rope_fwd_kernel<T, T><<<grid, kThreads, 0, st>>>(q, k, sh);
+  } else if (a.cs_f32) {
+    if (partials != nullptr)
+      qk_norm_rope_bwd_kernel<T, float, true><<<grid, kThreads, 0, st>>>(q, k, sh, partials);
+    else
+      qk_norm_rope_bwd_kernel<T, float, false><<<grid, kThreads, 0, st>>>(q, k, sh, partials);
+  } else {
+    if (partials != nullptr)
+      qk_norm_rope_bwd_kernel<T, T, true><<<grid, kThreads, 0, st>>>(q, k, sh, partials);
+    else
+      qk_norm_rope_bwd_kernel<T, T, false><<<grid, kThreads, 0, st>>>(q, k, sh, partials);
+  }
   VQ_CUDA(cudaGetLastError());
   return 0;
 }
@@ -1272,7 +1290,7 @@ int vq_qk_norm_rope_fwd(const void* q, const int64_t* q_strides, int64_t Hq, con
   if ((Hq > 0 && (q_out == nullptr || !aligned16(q_out))) || (Hk > 0 && (k_out == nullptr || !aligned16(k_out))))
     return fail(VQ_ERR_INVALID, "outputs must be 16-byte aligned pointers");
   QkPlan p;
-  if (int rc = qk_plan(&p, B * S, Hq, Hk, D)) return rc;
+  if (int rc = qk_plan(&p, B * S, Hq, Hk, D, vq::qknorm::kFwdBlocks)) return rc;
   const QkArgs a{q,  k,  nullptr, nullptr, q_weight, k_weight, cos, sin, q_strides, k_strides, nullptr, nullptr, cs_strides,
                  Hq, Hk, B,       S,       D,        R,        weight_f32 != 0, cs_f32 != 0, eps, weight_offset, q_out, k_out};
   return launch_qk_dtype<false>(a, p, dtype, nullptr, static_cast<cudaStream_t>(stream));
@@ -1307,7 +1325,9 @@ int vq_qk_norm_rope_bwd(const void* gq, const int64_t* gq_strides, const void* g
   if (want_dw && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < vq_qk_norm_rope_workspace_bytes(D)))
     return fail(VQ_ERR_INVALID, "workspace of %zu bytes needed for the weight gradients", vq_qk_norm_rope_workspace_bytes(D));
   QkPlan p;
-  if (int rc = qk_plan(&p, B * S, Hq, Hk, D)) return rc;
+  if (int rc = qk_plan(&p, B * S, Hq, Hk, D,
+                       cs_f32 || dtype == 0 ? vq::qknorm::kBwdBlocksWide : vq::qknorm::kBwdBlocks))
+    return rc;
   const QkArgs a{q,  k,  gq, gk, q_weight, k_weight, cos, sin, q_strides, k_strides, gq_strides, gk_strides, cs_strides,
                  Hq, Hk, B,  S,  D,        R,        weight_f32 != 0, cs_f32 != 0, eps, weight_offset, dq, dk};
   float* partials = want_dw ? static_cast<float*>(workspace) : nullptr;
@@ -1330,8 +1350,7 @@ int vq_qk_norm_rope_bwd(const void* gq, const int64_t* gq_strides, const void* g
 namespace {
 
 // ---- gated embedding ----
-int check_table(const vq::CandSet& cs, int64_t T, int64_t vocab_start, int64_t rows, int64_t padded_cols, int64_t cols) {
-  (void)cs;
+int check_table(int64_t T, int64_t vocab_start, int64_t rows, int64_t padded_cols, int64_t cols) {
   if (T < 0 || rows < 0 || cols < 0 || vocab_start < 0) return fail(VQ_ERR_INVALID, "negative shape or vocabulary start");
   if (padded_cols < cols || padded_cols % 256 != 0)
     return fail(VQ_ERR_INVALID, "padded columns %lld must be a multiple of 256 that holds %lld", (long long)padded_cols,
@@ -1340,91 +1359,93 @@ int check_table(const vq::CandSet& cs, int64_t T, int64_t vocab_start, int64_t r
   return 0;
 }
 
-template <typename T>
-int launch_embed_gategrad(const vq::CandSet& cs, const int* keys, const int* order, int T_, int rows, int upr, int cols,
-                          const void* dy, long long lddy, double* partials, int* blocks, int* err, cudaStream_t st) {
-  using namespace vq::embed;
-  auto kern = embed_gategrad_kernel<T>;
-  const int smem = cs.K * kThreads * static_cast<int>(sizeof(double)) + kWarps * warp_bytes(cs);
-  VQ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  int per_sm = 0, sms = 0;
-  VQ_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kThreads, smem));
-  if (per_sm < 1) return fail(VQ_ERR_INVALID, "%d candidates do not fit one SM", cs.K);
-  if (int rc = sm_count(&sms)) return rc;
-  const long long groups = (upr + kUnits - 1) / kUnits;
-  const long long resident = static_cast<long long>(sms) * per_sm * kWarps;
-  // the longest run of sorted tokens that still leaves four items a resident warp
-  int window = 1;
-  while (window < 32 && (T_ + 2 * window - 1) / (2 * window) * groups >= 4 * resident) window *= 2;
-  const long long items = (T_ + window - 1) / window * groups;
-  long long grid = (items + kWarps - 1) / kWarps;
-  if (grid > static_cast<long long>(sms) * per_sm) grid = static_cast<long long>(sms) * per_sm;
-  if (grid > vq::embed::kMaxBlocks) grid = vq::embed::kMaxBlocks;
-  *blocks = static_cast<int>(grid);
-  kern<<<*blocks, kThreads, smem, st>>>(cs, keys, order, T_, rows, upr, cols, window, static_cast<const T*>(dy), lddy,
-                                        partials, err);
-  VQ_CUDA(cudaGetLastError());
+inline size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
+
+// A plan in memory: the number of pieces; then, T ints each (256-byte steps),
+// order, start (one more), key; then the scratch of the sort.
+struct PlanLayout {
+  size_t order, start, key, keys, keys_tmp, order_tmp, bytes;
+  explicit PlanLayout(int64_t T) {
+    const size_t n = round256(static_cast<size_t>(T) * sizeof(int));
+    order = 256;
+    start = order + n;
+    key = start + round256((static_cast<size_t>(T) + 1) * sizeof(int));
+    keys = key + n;
+    keys_tmp = keys + n;
+    order_tmp = keys_tmp + n;
+    bytes = order_tmp + n;
+  }
+};
+
+vq::embed::Plan plan_at(void* p, const PlanLayout& l) {
+  char* c = static_cast<char*>(p);
+  return vq::embed::Plan{reinterpret_cast<int*>(c + l.order), reinterpret_cast<int*>(c + l.start),
+                         reinterpret_cast<int*>(c + l.key), reinterpret_cast<int*>(c)};
+}
+
+int check_ids(const void* ids, int ids_i32) {
+  if (ids == nullptr) return fail(VQ_ERR_INVALID, "null token ids");
+  if (reinterpret_cast<uintptr_t>(ids) % (ids_i32 ? 4 : 8) != 0) return fail(VQ_ERR_INVALID, "misaligned token ids");
   return 0;
 }
 
-inline size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
+int check_plan(const void* plan, size_t plan_bytes, int64_t T) {
+  const size_t need = PlanLayout(T).bytes;
+  if (plan == nullptr || (reinterpret_cast<uintptr_t>(plan) & 15u) != 0 || plan_bytes < need)
+    return fail(VQ_ERR_INVALID, "plan of %zu bytes (16-byte aligned) needed, got %zu", need, plan_bytes);
+  return 0;
+}
+
+// One wave of blocks of a kernel, or fewer for little work.
+template <typename Kernel>
+int one_wave(Kernel kern, int smem, long long units, int* grid) {
+  using namespace vq::embed;
+  VQ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  int per_sm = 0, sms = 0;
+  VQ_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kThreads, smem));
+  if (per_sm < 1) return fail(VQ_ERR_INVALID, "the candidates do not fit one SM");
+  if (int rc = sm_count(&sms)) return rc;
+  long long n = (units + kWarps * kUnits - 1) / (kWarps * kUnits);
+  if (n > static_cast<long long>(sms) * per_sm) n = static_cast<long long>(sms) * per_sm;
+  *grid = static_cast<int>(n < kMaxBlocks ? n : kMaxBlocks);
+  return 0;
+}
+
+template <typename T>
+int launch_embed_gategrad(const vq::CandSet& cs, const vq::embed::Plan& plan, long long tokens, long long rows, int upr,
+                          int cols, const void* dy, long long lddy, double* partials, int* blocks, int* err,
+                          cudaStream_t st) {
+  using namespace vq::embed;
+  const int smem = cs.K * kThreads * static_cast<int>(sizeof(double)) + kWarps * kStages * warp_bytes(cs);
+  if (int rc = one_wave(embed_gategrad_kernel<T>, smem, tokens * upr, blocks)) return rc;
+  embed_gategrad_kernel<T><<<*blocks, kThreads, smem, st>>>(cs, plan, rows, upr, cols, static_cast<const T*>(dy), lddy,
+                                                            partials, err);
+  VQ_CUDA(cudaGetLastError());
+  return 0;
+}
 
 }  // namespace
 
 extern "C" {
 
-int vq_embed_mix(int K, const int* types, const void* const* blocks, const float* probs, const void* ids, int ids_i32,
-                 int64_t T, int64_t vocab_start, int64_t rows, int64_t padded_cols, int64_t cols, float scale, int strict,
-                 void* out, int64_t ldo, void* stream) {
-  DeviceScope scope(out);
-  vq::CandSet cs;
-  if (int rc = build_candset(&cs, K, types, blocks)) return rc;
-  if (int rc = check_table(cs, T, vocab_start, rows, padded_cols, cols)) return rc;
-  if (int rc = check_matrix(out, T, cols, ldo, "out")) return rc;
-  if (T == 0 || cols == 0) return 0;
-  if (probs == nullptr || ids == nullptr) return fail(VQ_ERR_INVALID, "null pointer");
-  if (reinterpret_cast<uintptr_t>(ids) % (ids_i32 ? 4 : 8) != 0) return fail(VQ_ERR_INVALID, "misaligned token ids");
-  int* err = nullptr;
-  if (int rc = device_error_ptr(&err)) return rc;
-  using namespace vq::embed;
-  const int smem = kWarps * warp_bytes(cs);
-  VQ_CUDA(cudaFuncSetAttribute(embed_mix_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  int per_sm = 0, sms = 0;
-  VQ_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, embed_mix_kernel, kThreads, smem));
-  if (per_sm < 1) return fail(VQ_ERR_INVALID, "mixture of %d candidates does not fit one SM", K);
-  if (int rc = sm_count(&sms)) return rc;
-  const int upr = static_cast<int>(padded_cols / 256);
-  const long long units = T * upr;
-  long long grid = (units + kWarps * kUnits - 1) / (kWarps * kUnits);
-  if (grid > static_cast<long long>(sms) * per_sm) grid = static_cast<long long>(sms) * per_sm;
-  embed_mix_kernel<<<static_cast<unsigned>(grid), kThreads, smem, static_cast<cudaStream_t>(stream)>>>(
-      cs, probs, Ids{ids, ids_i32 != 0}, T, vocab_start, rows, upr, static_cast<int>(cols), scale, strict != 0,
-      static_cast<__nv_bfloat16*>(out), ldo, err);
-  VQ_CUDA(cudaGetLastError());
-  return 0;
-}
+size_t vq_embed_plan_bytes(int64_t T) { return T < 0 || T > (1LL << 30) ? 0 : PlanLayout(T).bytes; }
 
-size_t vq_embed_gategrad_workspace_bytes(int64_t T, int K) {
-  if (T < 0 || T > (1LL << 30) || K < 1 || K > vq::kMaxCandidates) return 0;
-  // sorted keys and tokens, twice (a radix pass reads one pair and writes the other); the blocks' partials
-  return 4 * round256(static_cast<size_t>(T) * sizeof(int)) + round256(static_cast<size_t>(vq::embed::kMaxBlocks) * K * sizeof(double));
-}
-
-int vq_token_sort(const void* ids, int ids_i32, int64_t T, int64_t vocab_start, int64_t rows, int* keys, int* order,
-                  int* keys_tmp, int* order_tmp, void* stream) {
-  DeviceScope scope(keys);
+int vq_embed_plan(const void* ids, int ids_i32, int64_t T, int64_t vocab_start, int64_t rows, void* plan,
+                  size_t plan_bytes, void* stream) {
+  DeviceScope scope(plan);
   if (T < 0 || rows < 0 || vocab_start < 0) return fail(VQ_ERR_INVALID, "negative shape or vocabulary start");
   if (T > (1LL << 30) || rows > (1LL << 30)) return fail(VQ_ERR_INVALID, "shape too large");
   if (T == 0) return 0;
-  if (ids == nullptr || keys == nullptr || order == nullptr || keys_tmp == nullptr || order_tmp == nullptr)
-    return fail(VQ_ERR_INVALID, "null pointer");
-  if (reinterpret_cast<uintptr_t>(ids) % (ids_i32 ? 4 : 8) != 0) return fail(VQ_ERR_INVALID, "misaligned token ids");
+  if (int rc = check_ids(ids, ids_i32)) return rc;
+  if (int rc = check_plan(plan, plan_bytes, T)) return rc;
   using namespace vq::embed;
   int bits = 1;
   while ((rows >> bits) != 0) ++bits;
   const int passes = (bits + kDigitBits - 1) / kDigitBits;
   const int ctas = static_cast<int>(T >= static_cast<int64_t>(kSortCtas) * kSortThreads ? kSortCtas
                                                                                         : (T + kSortThreads - 1) / kSortThreads);
+  const PlanLayout l(T);
+  char* c = static_cast<char*>(plan);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas));
   cfg.blockDim = dim3(kSortThreads);
@@ -1436,20 +1457,56 @@ int vq_token_sort(const void* ids, int ids_i32, int64_t T, int64_t vocab_start, 
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  VQ_CUDA(cudaLaunchKernelEx(&cfg, token_sort_kernel, Ids{ids, ids_i32 != 0}, static_cast<int>(T),
-                             static_cast<long long>(vocab_start), static_cast<int>(rows), passes, keys, order, keys_tmp,
-                             order_tmp));
+  VQ_CUDA(cudaLaunchKernelEx(&cfg, token_plan_kernel, Ids{ids, ids_i32 != 0}, static_cast<int>(T),
+                             static_cast<long long>(vocab_start), static_cast<int>(rows), passes, plan_at(plan, l),
+                             reinterpret_cast<int*>(c + l.keys), reinterpret_cast<int*>(c + l.keys_tmp),
+                             reinterpret_cast<int*>(c + l.order_tmp)));
   VQ_CUDA(cudaGetLastError());
   return 0;
 }
 
-int vq_embed_gategrad(int K, const int* types, const void* const* blocks, const void* ids, int ids_i32, int64_t T,
-                      int64_t vocab_start, int64_t rows, int64_t padded_cols, int64_t cols, float scale, const void* dy,
-                      int64_t lddy, int dy_dtype, void* workspace, size_t workspace_bytes, float* grad, void* stream) {
+int vq_embed_mix(int K, const int* types, const void* const* blocks, const float* probs, const void* ids, int ids_i32,
+                 int64_t T, const void* plan, size_t plan_bytes, int64_t vocab_start, int64_t rows, int64_t padded_cols,
+                 int64_t cols, float scale, int strict, void* out, int64_t ldo, void* stream) {
+  DeviceScope scope(out);
+  vq::CandSet cs;
+  if (int rc = build_candset(&cs, K, types, blocks)) return rc;
+  if (int rc = check_table(T, vocab_start, rows, padded_cols, cols)) return rc;
+  if (int rc = check_matrix(out, T, cols, ldo, "out")) return rc;
+  if (T == 0 || cols == 0) return 0;
+  if (probs == nullptr) return fail(VQ_ERR_INVALID, "null pointer");
+  if (plan == nullptr) {
+    if (int rc = check_ids(ids, ids_i32)) return rc;
+  } else if (int rc = check_plan(plan, plan_bytes, T)) {
+    return rc;
+  }
+  int* err = nullptr;
+  if (int rc = device_error_ptr(&err)) return rc;
+  using namespace vq::embed;
+  const int smem = kWarps * kStages * warp_bytes(cs);
+  const int upr = static_cast<int>(padded_cols / 256);
+  auto kern = plan != nullptr ? embed_mix_kernel<true> : embed_mix_kernel<false>;
+  int grid = 0;
+  if (int rc = one_wave(kern, smem, T * upr, &grid)) return rc;
+  const Plan pl = plan != nullptr ? plan_at(const_cast<void*>(plan), PlanLayout(T)) : Plan{};
+  kern<<<grid, kThreads, smem, static_cast<cudaStream_t>(stream)>>>(
+      cs, probs, Ids{ids, ids_i32 != 0}, T, pl, vocab_start, rows, upr, static_cast<int>(cols), scale, strict != 0,
+      static_cast<__nv_bfloat16*>(out), ldo, err);
+  VQ_CUDA(cudaGetLastError());
+  return 0;
+}
+
+size_t vq_embed_gategrad_workspace_bytes(int K) {
+  return K < 1 || K > vq::kMaxCandidates ? 0 : static_cast<size_t>(vq::embed::kMaxBlocks) * K * sizeof(double);
+}
+
+int vq_embed_gategrad(int K, const int* types, const void* const* blocks, const void* plan, size_t plan_bytes, int64_t T,
+                      int64_t rows, int64_t padded_cols, int64_t cols, float scale, const void* dy, int64_t lddy,
+                      int dy_dtype, void* workspace, size_t workspace_bytes, float* grad, void* stream) {
   DeviceScope scope(grad);
   vq::CandSet cs;
   if (int rc = build_candset(&cs, K, types, blocks)) return rc;
-  if (int rc = check_table(cs, T, vocab_start, rows, padded_cols, cols)) return rc;
+  if (int rc = check_table(T, 0, rows, padded_cols, cols)) return rc;
   if (int rc = check_matrix(dy, T, cols, lddy, "dy")) return rc;
   if (dy_dtype < 0 || dy_dtype > 2) return fail(VQ_ERR_INVALID, "dtype %d (0 = float32, 1 = bfloat16, 2 = float16)", dy_dtype);
   if (grad == nullptr) return fail(VQ_ERR_INVALID, "null pointer");
@@ -1458,28 +1515,22 @@ int vq_embed_gategrad(int K, const int* types, const void* const* blocks, const 
     VQ_CUDA(cudaMemsetAsync(grad, 0, K * sizeof(float), st));
     return 0;
   }
-  if (ids == nullptr || workspace == nullptr) return fail(VQ_ERR_INVALID, "null pointer");
-  const size_t need = vq_embed_gategrad_workspace_bytes(T, K);
-  if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0 || workspace_bytes < need)
+  if (int rc = check_plan(plan, plan_bytes, T)) return rc;
+  const size_t need = vq_embed_gategrad_workspace_bytes(K);
+  if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0 || workspace_bytes < need)
     return fail(VQ_ERR_INVALID, "workspace of %zu bytes (16-byte aligned) needed, got %zu", need, workspace_bytes);
-  const size_t part = round256(static_cast<size_t>(T) * sizeof(int));
-  char* ws = static_cast<char*>(workspace);
-  int* keys = reinterpret_cast<int*>(ws);
-  int* order = reinterpret_cast<int*>(ws + part);
-  double* partials = reinterpret_cast<double*>(ws + 4 * part);
-  if (int rc = vq_token_sort(ids, ids_i32, T, vocab_start, rows, keys, order, reinterpret_cast<int*>(ws + 2 * part),
-                             reinterpret_cast<int*>(ws + 3 * part), stream))
-    return rc;
+  double* partials = static_cast<double*>(workspace);
+  const vq::embed::Plan pl = plan_at(const_cast<void*>(plan), PlanLayout(T));
   int* err = nullptr;
   if (int rc = device_error_ptr(&err)) return rc;
   const int upr = static_cast<int>(padded_cols / 256);
   int n = 0, rc = 0;
   if (dy_dtype == 0)
-    rc = launch_embed_gategrad<float>(cs, keys, order, (int)T, (int)rows, upr, (int)cols, dy, lddy, partials, &n, err, st);
+    rc = launch_embed_gategrad<float>(cs, pl, T, rows, upr, (int)cols, dy, lddy, partials, &n, err, st);
   else if (dy_dtype == 1)
-    rc = launch_embed_gategrad<__nv_bfloat16>(cs, keys, order, (int)T, (int)rows, upr, (int)cols, dy, lddy, partials, &n, err, st);
+    rc = launch_embed_gategrad<__nv_bfloat16>(cs, pl, T, rows, upr, (int)cols, dy, lddy, partials, &n, err, st);
   else
-    rc = launch_embed_gategrad<__half>(cs, keys, order, (int)T, (int)rows, upr, (int)cols, dy, lddy, partials, &n, err, st);
+    rc = launch_embed_gategrad<__half>(cs, pl, T, rows, upr, (int)cols, dy, lddy, partials, &n, err, st);
   if (rc) return rc;
   vq::embed::embed_gategrad_join_kernel<<<1, 32 * vq::kMaxCandidates, 0, st>>>(partials, n, K, scale, grad);
   VQ_CUDA(cudaGetLastError());
@@ -1494,11 +1545,6 @@ namespace {
 struct Range {
   uintptr_t b, e;
 };
-
-int range_less(const void* x, const void* y) {
-  const uintptr_t a = static_cast<const Range*>(x)->b, b = static_cast<const Range*>(y)->b;
-  return a < b ? -1 : a > b;
-}
 
 // Values that one block takes and scales in one launch, at most.
 constexpr long long kClipSmallValues = 16384;
@@ -1601,7 +1647,7 @@ int vq_clip_grad_norm(int n, const void* const* ptrs, const int64_t* numel, cons
     ++m;
   }
   if (total > (1LL << 42)) return fail(VQ_ERR_INVALID, "too many values");
-  std::qsort(r, m, sizeof(Range), range_less);
+  std::sort(r, r + m, [](const Range& x, const Range& y) { return x.b < y.b; });
   for (int i = 1; i < m; ++i)
     if (r[i].b < r[i - 1].e) return fail(VQ_ERR_INVALID, "two of the tensors share memory: each value is scaled once");
   if (m == 0) {

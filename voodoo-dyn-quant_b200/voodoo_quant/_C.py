@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+from array import array
 from pathlib import Path
 
 import torch
@@ -83,12 +84,13 @@ def _declare(lib):
         "vq_qk_norm_rope_bwd": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _int, _vp, _vp, _vp,
                                        _int, _i64, _i64, _i64, _i64, _f32, _f32, _int, _vp, _vp, _vp, _vp, _vp,
                                        ctypes.c_size_t, _vp]),
-        "vq_embed_mix": (_int, [_int, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, _i64, _f32, _int, _vp, _i64,
-                                _vp]),
-        "vq_token_sort": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
-        "vq_embed_gategrad_workspace_bytes": (ctypes.c_size_t, [_i64, _int]),
-        "vq_embed_gategrad": (_int, [_int, _vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, _i64, _f32, _vp, _i64, _int, _vp,
-                                     ctypes.c_size_t, _vp, _vp]),
+        "vq_embed_plan_bytes": (ctypes.c_size_t, [_i64]),
+        "vq_embed_plan": (_int, [_vp, _int, _i64, _i64, _i64, _vp, ctypes.c_size_t, _vp]),
+        "vq_embed_mix": (_int, [_int, _vp, _vp, _vp, _vp, _int, _i64, _vp, ctypes.c_size_t, _i64, _i64, _i64, _i64, _f32,
+                                _int, _vp, _i64, _vp]),
+        "vq_embed_gategrad_workspace_bytes": (ctypes.c_size_t, [_int]),
+        "vq_embed_gategrad": (_int, [_int, _vp, _vp, _vp, ctypes.c_size_t, _i64, _i64, _i64, _i64, _f32, _vp, _i64, _int,
+                                     _vp, ctypes.c_size_t, _vp, _vp]),
         "vq_clip_grad_norm_workspace_bytes": (ctypes.c_size_t, [_int]),
         "vq_clip_grad_norm": (_int, [_int, _vp, _vp, _vp, _f32, _int, _vp, ctypes.c_size_t, _vp, _vp]),
     }
@@ -107,7 +109,7 @@ EXPORTED = (
     "vq_loss_fused", "vq_loss_stats", "vq_loss_combine", "vq_loss_grad",
     "vq_rmsnorm_fwd", "vq_rmsnorm_bwd", "vq_add_rmsnorm_fwd", "vq_rmsnorm_bwd_add", "vq_rope", "vq_swiglu_fwd", "vq_swiglu_bwd",
     "vq_qk_norm_rope_fwd", "vq_qk_norm_rope_workspace_bytes", "vq_qk_norm_rope_bwd",
-    "vq_embed_mix", "vq_token_sort", "vq_embed_gategrad_workspace_bytes", "vq_embed_gategrad",
+    "vq_embed_plan_bytes", "vq_embed_plan", "vq_embed_mix", "vq_embed_gategrad_workspace_bytes", "vq_embed_gategrad",
     "vq_clip_grad_norm_workspace_bytes", "vq_clip_grad_norm",
 )
 
@@ -143,6 +145,11 @@ def _stream(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
+def _raw_stream(device_index: int) -> int:
+    """Current stream's handle on a device, without the Python stream object (a few microseconds of a short call)."""
+    return torch._C._cuda_getCurrentRawStream(device_index)
+
+
 def _require_cuda(*ts: torch.Tensor) -> None:
     load_library()
     for t in ts:
@@ -165,10 +172,16 @@ def _float_code(t: torch.Tensor, name: str) -> int:
     return code
 
 
-def _require_one_device(*ts: torch.Tensor) -> None:
-    for t in ts[1:]:
-        if t.device != ts[0].device:
-            raise ValueError(f"tensors on one device expected, got {ts[0].device} and {t.device}")
+def _device_of(*ts: torch.Tensor) -> int:
+    """Index of the CUDA device that all of the tensors are on."""
+    d = ts[0].get_device()
+    for t in ts:
+        if t.get_device() != d or d < 0:
+            _require_cuda(*ts)
+            raise ValueError(f"tensors on one device expected, got {[str(u.device) for u in ts]}")
+    if _lib is None:
+        load_library()
+    return d
 
 
 def format_info(qtype: str) -> tuple[int, int]:
@@ -177,6 +190,19 @@ def format_info(qtype: str) -> tuple[int, int]:
     rc = lib.vq_format_info(GGML_TYPE.get(qtype, -1), ctypes.byref(be), ctypes.byref(bb))
     _check(rc)
     return be.value, bb.value
+
+
+_GEOMETRY: dict[str, tuple[int, int]] = {}
+
+
+def _geometry(qtype: str) -> tuple[int, int]:
+    """``format_info`` of a supported type, looked up once."""
+    g = _GEOMETRY.get(qtype)
+    if g is None:
+        if qtype not in GGML_TYPE:
+            raise ValueError(f"Unknown quant type: {qtype}. Supported: {list(GGML_TYPE)}")
+        g = _GEOMETRY[qtype] = format_info(qtype)
+    return g
 
 
 def device_error(device: torch.device | None = None) -> int:
@@ -614,176 +640,191 @@ def swiglu_bwd(gate: torch.Tensor, up: torch.Tensor, dy: torch.Tensor, out: torc
 
 
 # ---------------------------------------------------------------- head norms with rotation
-def _heads_operand(t: torch.Tensor) -> torch.Tensor:
-    """[B, S, H, D] view with unit stride over D, the others multiples of 8, 16-byte aligned; copied otherwise."""
-    if t.numel() and (t.stride(-1) != 1 or any(st % 8 for st in t.stride()[:3]) or t.data_ptr() % 16 != 0):
+def _heads_operand(t: torch.Tensor):
+    """(t, its strides over B, S, H): t copied where its strides over the others are no multiples of 8, that over D is
+    not 1 or its first value is not 16-byte aligned."""
+    b, s, h, d = t.stride()
+    if d != 1 or (b | s | h) & 7 or t.data_ptr() & 15:
+        t = t.clone(memory_format=torch.contiguous_format)
+        b, s, h, d = t.stride()
+    return t, b, s, h
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    if not t.is_contiguous() or t.data_ptr() & 15:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    t = t.contiguous()
-    return t.clone() if t.data_ptr() % 16 else t
+def _table_operand(t: torch.Tensor):
+    """A rotary table with unit stride over R, the others multiples of 8, 16-byte aligned; copied otherwise."""
+    st = t.stride()
+    if st[-1] != 1 or st[-2] & 7 or (len(st) == 3 and st[0] & 7) or t.data_ptr() & 15:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
 
 
 def _qk_operands(q, k, q_weight, k_weight, cos, sin):
-    """Checked and laid out operands, and the scalar arguments that both directions pass on."""
-    _require_cuda(q, k, q_weight, k_weight, cos, sin)
-    _require_one_device(q, k, q_weight, k_weight, cos, sin)
-    if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
-        raise ValueError(f"qk_norm_rope: q [B, S, Hq, D] and k [B, S, Hk, D] expected, got {tuple(q.shape)} and "
-                         f"{tuple(k.shape)}")
+    """Checked and laid out operands: device, q, k with their strides, weights, tables, (B, S, D, R), dtype code."""
+    dev = _device_of(q, k, q_weight, k_weight, cos, sin)
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4 or qs[:2] != ks[:2] or qs[3] != ks[3]:
+        raise ValueError(f"qk_norm_rope: q [B, S, Hq, D] and k [B, S, Hk, D] expected, got {tuple(qs)} and {tuple(ks)}")
+    dt = q.dtype
     dtype = _float_code(q, "qk_norm_rope")
-    if k.dtype != q.dtype:
-        raise ValueError(f"qk_norm_rope: q is {q.dtype}, k is {k.dtype}")
-    B, S, _, D = q.shape
-    for w in (q_weight, k_weight):
-        _float_code(w, "qk_norm_rope weight")
-        if tuple(w.shape) != (D,):
-            raise ValueError(f"qk_norm_rope: weights of shape ({D},) expected, got {tuple(w.shape)}")
-    for c in (cos, sin):
-        _float_code(c, "qk_norm_rope table")
-        if c.dim() not in (2, 3) or c.shape != cos.shape or c.shape[-2] != S or (c.dim() == 3 and c.shape[0] not in (1, B)):
-            raise ValueError(f"qk_norm_rope: cos and sin [B or 1, S, R] expected, got {tuple(cos.shape)} and "
-                             f"{tuple(sin.shape)} for q {tuple(q.shape)}")
-    R = cos.shape[-1]
-    if not (q_weight.dtype == k_weight.dtype == q.dtype):
+    if k.dtype != dt:
+        raise ValueError(f"qk_norm_rope: q is {dt}, k is {k.dtype}")
+    B, S, _, D = qs
+    if q_weight.shape != (D,) or k_weight.shape != (D,):
+        raise ValueError(f"qk_norm_rope: weights of shape ({D},) expected, got {tuple(q_weight.shape)} and "
+                         f"{tuple(k_weight.shape)}")
+    cshape = cos.shape
+    if (len(cshape) not in (2, 3) or sin.shape != cshape or cshape[-2] != S
+            or (len(cshape) == 3 and cshape[0] not in (1, B))):
+        raise ValueError(f"qk_norm_rope: cos and sin [B or 1, S, R] expected, got {tuple(cshape)} and "
+                         f"{tuple(sin.shape)} for q {tuple(qs)}")
+    if q_weight.dtype != dt or k_weight.dtype != dt:
+        _float_code(q_weight, "qk_norm_rope weight"), _float_code(k_weight, "qk_norm_rope weight")
         q_weight, k_weight = q_weight.float(), k_weight.float()
-    if not (cos.dtype == sin.dtype == q.dtype):
+    if cos.dtype != dt or sin.dtype != dt:
+        _float_code(cos, "qk_norm_rope table"), _float_code(sin, "qk_norm_rope table")
         cos, sin = cos.float(), sin.float()
-    q_weight, k_weight = _aligned(q_weight), _aligned(k_weight)
-    if cos.stride() != sin.stride() or cos.stride(-1) != 1 or any(st % 8 for st in cos.stride()[:-1]) or \
-            cos.data_ptr() % 16 or sin.data_ptr() % 16:
-        cos = cos.clone(memory_format=torch.contiguous_format)
-        sin = sin.clone(memory_format=torch.contiguous_format)
-    c3, s3 = cos.expand(B, S, R), sin.expand(B, S, R)
-    return _heads_operand(q), _heads_operand(k), q_weight, k_weight, c3, s3, (B, S, D, R), dtype
+    cos, sin = _table_operand(cos), _table_operand(sin)
+    if cos.stride() != sin.stride():
+        cos, sin = cos.contiguous(), sin.contiguous()
+    cst = cos.stride()
+    cb = cst[0] if len(cshape) == 3 and cshape[0] > 1 else 0  # one table for every batch entry
+    return (dev, _heads_operand(q), _heads_operand(k), _aligned(q_weight), _aligned(k_weight), cos, sin, cb, cst[-2],
+            (B, S, D, cshape[-1]), dtype)
 
 
-def _strides(t: torch.Tensor, n: int):
-    return (ctypes.c_int64 * n)(*t.stride()[:n])
+_strides3 = ctypes.c_int64 * 3
+_strides2 = ctypes.c_int64 * 2
 
 
 def qk_norm_rope_fwd(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
-                     cos: torch.Tensor, sin: torch.Tensor, eps: float, weight_offset: float = 0.0):
+                     cos: torch.Tensor, sin: torch.Tensor, eps: float, weight_offset: float = 0.0, saved: bool = False):
     """Norm of each head of q [B, S, Hq, D] and k [B, S, Hk, D] (float32, bfloat16 or float16, any strides) with
     weights ``weight_offset + weight`` [D], then the rotation of its first R values by cos / sin [B or 1, S, R];
-    contiguous outputs of q's type, rounded once."""
-    q, k, wq, wk, c, s, (B, S, D, R), dtype = _qk_operands(q, k, q_weight, k_weight, cos, sin)
-    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    _check(_lib.vq_qk_norm_rope_fwd(q.data_ptr(), _strides(q, 3), q.shape[2], k.data_ptr(), _strides(k, 3), k.shape[2],
-                                    wq.data_ptr(), wk.data_ptr(), int(wq.dtype == torch.float32), c.data_ptr(),
-                                    s.data_ptr(), _strides(c, 2), int(c.dtype == torch.float32), B, S, D, R, float(eps),
-                                    float(weight_offset), dtype, qo.data_ptr(), ko.data_ptr(), _stream(q)))
+    contiguous outputs of q's type, rounded once.  ``saved``: also the operands as they were laid out, for
+    ``qk_norm_rope_bwd``."""
+    dev, (q, qb, qs, qh), (k, kb, ks, kh), wq, wk, c, s, cb, cs, (B, S, D, R), dtype = \
+        _qk_operands(q, k, q_weight, k_weight, cos, sin)
+    qo, ko = q.new_empty(q.shape), k.new_empty(k.shape)
+    qst, kst, cst = _strides3(qb, qs, qh), _strides3(kb, ks, kh), _strides2(cb, cs)
+    wf, cf = wq.dtype == torch.float32, c.dtype == torch.float32
+    _check(_lib.vq_qk_norm_rope_fwd(q.data_ptr(), qst, q.shape[2], k.data_ptr(), kst, k.shape[2], wq.data_ptr(),
+                                    wk.data_ptr(), wf, c.data_ptr(), s.data_ptr(), cst, cf, B, S, D, R, eps,
+                                    weight_offset, dtype, qo.data_ptr(), ko.data_ptr(), _raw_stream(dev)))
+    if saved:
+        return qo, ko, (q, k, wq, wk, c, s), (dev, qst, kst, wf, cst, cf, B, S, D, R, eps, weight_offset, dtype)
     return qo, ko
 
 
-def qk_norm_rope_bwd(gq: torch.Tensor, gk: torch.Tensor, q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
-                     k_weight: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, eps: float,
-                     weight_offset: float = 0.0, want_weight_grads: bool = True):
-    """(dq, dk, dq_weight, dk_weight) of ``qk_norm_rope_fwd`` for the outputs' gradients gq, gk; the weights' are
-    None unless wanted."""
-    dts = q_weight.dtype, k_weight.dtype
-    q, k, wq, wk, c, s, (B, S, D, R), dtype = _qk_operands(q, k, q_weight, k_weight, cos, sin)
+def qk_norm_rope_bwd(gq: torch.Tensor, gk: torch.Tensor, operands, layout, want_weight_grads: bool = True):
+    """(dq, dk, dq_weight, dk_weight) of ``qk_norm_rope_fwd`` for the outputs' gradients gq, gk, from what it saved; the
+    weights' gradients (in the type the weights were laid out in) are None unless wanted."""
+    q, k, wq, wk, c, s = operands
+    dev, qst, kst, wf, cst, cf, B, S, D, R, eps, weight_offset, dtype = layout
     if gq.shape != q.shape or gk.shape != k.shape or gq.dtype != q.dtype or gk.dtype != q.dtype:
         raise ValueError(f"qk_norm_rope: gradients of the outputs' shapes and type expected, got {tuple(gq.shape)} "
                          f"{gq.dtype} and {tuple(gk.shape)} {gk.dtype}")
-    _require_one_device(q, gq, gk)
-    gq, gk = _heads_operand(gq), _heads_operand(gk)
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    if gq.get_device() != dev or gk.get_device() != dev:
+        raise ValueError("qk_norm_rope: gradients on the outputs' device expected")
+    (gq, gqb, gqs, gqh), (gk, gkb, gks, gkh) = _heads_operand(gq), _heads_operand(gk)
+    dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
     dwq = dwk = ws = None
     need = 0
     if want_weight_grads:
         dwq, dwk = torch.empty_like(wq), torch.empty_like(wk)
-        need = int(_lib.vq_qk_norm_rope_workspace_bytes(D))
-        ws = torch.empty(max(need, 4), dtype=torch.uint8, device=q.device)
-    _check(_lib.vq_qk_norm_rope_bwd(gq.data_ptr(), _strides(gq, 3), gk.data_ptr(), _strides(gk, 3), q.data_ptr(),
-                                    _strides(q, 3), q.shape[2], k.data_ptr(), _strides(k, 3), k.shape[2], wq.data_ptr(),
-                                    wk.data_ptr(), int(wq.dtype == torch.float32), c.data_ptr(), s.data_ptr(),
-                                    _strides(c, 2), int(c.dtype == torch.float32), B, S, D, R, float(eps),
-                                    float(weight_offset), dtype, dq.data_ptr(), dk.data_ptr(), _ptr(dwq), _ptr(dwk),
-                                    _ptr(ws), need, _stream(q)))
-    if want_weight_grads:
-        dwq, dwk = dwq.to(dts[0]), dwk.to(dts[1])
+        need = _lib.vq_qk_norm_rope_workspace_bytes(D)
+        ws = q.new_empty(need, dtype=torch.uint8)
+    _check(_lib.vq_qk_norm_rope_bwd(gq.data_ptr(), _strides3(gqb, gqs, gqh), gk.data_ptr(), _strides3(gkb, gks, gkh),
+                                    q.data_ptr(), qst, q.shape[2], k.data_ptr(), kst, k.shape[2], wq.data_ptr(),
+                                    wk.data_ptr(), wf, c.data_ptr(), s.data_ptr(), cst, cf, B, S, D, R, eps,
+                                    weight_offset, dtype, dq.data_ptr(), dk.data_ptr(), _ptr(dwq), _ptr(dwk), _ptr(ws),
+                                    need, _raw_stream(dev)))
     return dq, dk, dwq, dwk
 
 
 # ---------------------------------------------------------------- gated embedding
-def _table_operands(ids, qtypes, qbytes, rows: int, padded_cols: int, cols: int):
-    _require_cuda(ids, *qbytes)
-    _require_one_device(ids, *qbytes)
+def _ids_operand(ids: torch.Tensor) -> torch.Tensor:
     if ids.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"token ids must be int64 or int32, got {ids.dtype}")
-    if not 1 <= len(qtypes) <= 8 or len(qtypes) != len(qbytes):
-        raise ValueError(f"1..8 candidates with their blocks expected, got {len(qtypes)} types and {len(qbytes)} tensors")
-    if rows < 0 or cols < 0 or cols > padded_cols or padded_cols % 256:
-        raise ValueError(f"table of {rows} rows: {padded_cols} stored columns must be a multiple of 256 that holds {cols}")
-    for qt, qb in zip(qtypes, qbytes):
-        if qt not in GGML_TYPE:
-            raise ValueError(f"Unknown quant type: {qt}. Supported: {list(GGML_TYPE)}")
-        be, bb = format_info(qt)
-        if qb.dtype != torch.uint8 or not qb.is_contiguous() or qb.numel() != rows * (padded_cols // be) * bb:
-            raise ValueError(f"{qt}: contiguous uint8 blocks of {rows * (padded_cols // be) * bb} bytes expected, got "
-                             f"{qb.dtype} {tuple(qb.shape)}")
     return ids.contiguous()
 
 
+def _table_operands(qtypes, qbytes, rows: int, padded_cols: int, cols: int):
+    """The checked candidates' arrays for the C ABI: K, types, pointers."""
+    K = len(qtypes)
+    if not 1 <= K <= 8 or K != len(qbytes):
+        raise ValueError(f"1..8 candidates with their blocks expected, got {K} types and {len(qbytes)} tensors")
+    if rows < 0 or cols < 0 or cols > padded_cols or padded_cols % 256:
+        raise ValueError(f"table of {rows} rows: {padded_cols} stored columns must be a multiple of 256 that holds {cols}")
+    types, ptrs = (_int * K)(), (_vp * K)()
+    for i, (qt, qb) in enumerate(zip(qtypes, qbytes)):
+        be, bb = _geometry(qt)
+        if qb.dtype != torch.uint8 or not qb.is_contiguous() or qb.numel() != rows * (padded_cols // be) * bb:
+            raise ValueError(f"{qt}: contiguous uint8 blocks of {rows * (padded_cols // be) * bb} bytes expected, got "
+                             f"{qb.dtype} {tuple(qb.shape)}")
+        types[i] = GGML_TYPE[qt]
+        ptrs[i] = qb.data_ptr()
+    return K, types, ptrs
+
+
+def embed_plan(ids: torch.Tensor, rows: int, vocab_start: int | None = None) -> torch.Tensor:
+    """Plan of the token ids over a table of ``rows`` rows (uint8, its layout is the C header's): the tokens sorted by
+    row and cut into pieces of equal rows, for ``embed_mix`` and ``embed_gategrad`` of the same ids and table."""
+    dev = _device_of(ids)
+    ids = _ids_operand(ids)
+    T = ids.numel()
+    plan = torch.empty(_lib.vq_embed_plan_bytes(T), dtype=torch.uint8, device=ids.device)
+    _check(_lib.vq_embed_plan(ids.data_ptr(), ids.dtype == torch.int32, T, vocab_start or 0, rows, plan.data_ptr(),
+                              plan.numel(), _raw_stream(dev)))
+    return plan
+
+
 def embed_mix(ids: torch.Tensor, qtypes, qbytes, probs: torch.Tensor, rows: int, padded_cols: int, cols: int,
-              scale: float = 1.0, vocab_start: int | None = None) -> torch.Tensor:
+              scale: float = 1.0, vocab_start: int | None = None, plan: torch.Tensor | None = None) -> torch.Tensor:
     """Rows scale * sum_k probs[k] W_k[ids] of a table of packed candidates -> bf16 [*ids.shape, cols].  With
     ``vocab_start`` the table holds the vocabulary from there on and tokens of other shards get rows of zeros;
-    without it such ids are reported by ``device_error`` as well."""
-    ids = _table_operands(ids, qtypes, qbytes, rows, padded_cols, cols)
-    if probs.numel() != len(qtypes):
-        raise ValueError(f"{len(qtypes)} probabilities expected, got {tuple(probs.shape)}")
-    _require_cuda(probs)
-    _require_one_device(ids, probs)
-    K, types, ptrs = _cand_arrays(qtypes, qbytes)
-    p = probs.detach().to(torch.float32).contiguous()
+    without it such ids are reported by ``device_error`` as well.  With the ids' ``plan`` a row is decoded once for
+    up to 16 tokens that name it, else once per token."""
+    dev = _device_of(ids, probs, *qbytes)
+    ids = _ids_operand(ids)
+    K, types, ptrs = _table_operands(qtypes, qbytes, rows, padded_cols, cols)
+    if probs.numel() != K:
+        raise ValueError(f"{K} probabilities expected, got {tuple(probs.shape)}")
+    if probs.dtype != torch.float32 or not probs.is_contiguous():
+        probs = probs.detach().to(torch.float32).contiguous()
     out = torch.empty(*ids.shape, cols, dtype=torch.bfloat16, device=ids.device)
-    _check(_lib.vq_embed_mix(K, types, ptrs, p.data_ptr(), ids.data_ptr(), int(ids.dtype == torch.int32), ids.numel(),
-                             vocab_start or 0, rows, padded_cols, cols, float(scale), int(vocab_start is None),
-                             out.data_ptr(), cols, _stream(ids)))
+    _check(_lib.vq_embed_mix(K, types, ptrs, probs.data_ptr(), ids.data_ptr(), ids.dtype == torch.int32, ids.numel(),
+                             _ptr(plan), 0 if plan is None else plan.numel(), vocab_start or 0, rows, padded_cols, cols,
+                             scale, vocab_start is None, out.data_ptr(), cols, _raw_stream(dev)))
     return out
 
 
-def token_sort(ids: torch.Tensor, rows: int, vocab_start: int = 0):
-    """(keys, order), int32 [T]: the tokens' rows in ascending order (``rows`` for ids outside the table, last) and
-    the position that each came from; equal tokens keep their order."""
-    _require_cuda(ids)
-    if ids.dtype not in (torch.int64, torch.int32):
-        raise ValueError(f"token ids must be int64 or int32, got {ids.dtype}")
-    ids = ids.contiguous().reshape(-1)
-    T = ids.numel()
-    buf = torch.empty(4, T, dtype=torch.int32, device=ids.device)
-    _check(_lib.vq_token_sort(ids.data_ptr(), int(ids.dtype == torch.int32), T, vocab_start, rows, buf[0].data_ptr(),
-                              buf[1].data_ptr(), buf[2].data_ptr(), buf[3].data_ptr(), _stream(ids)))
-    return buf[0], buf[1]
-
-
-def embed_gategrad(dy: torch.Tensor, ids: torch.Tensor, qtypes, qbytes, rows: int, padded_cols: int, cols: int,
-                   scale: float = 1.0, vocab_start: int | None = None) -> torch.Tensor:
-    """grad[k] = scale * sum_t <dy[t], W_k[ids[t]]> (float32 [K]) for dy [*ids.shape, cols] in float32, bfloat16 or
-    float16; ids outside the table add nothing."""
-    ids = _table_operands(ids, qtypes, qbytes, rows, padded_cols, cols)
-    _require_cuda(dy)
-    _require_one_device(ids, dy)
+def embed_gategrad(dy: torch.Tensor, plan: torch.Tensor, qtypes, qbytes, rows: int, padded_cols: int, cols: int,
+                   scale: float = 1.0) -> torch.Tensor:
+    """grad[k] = scale * sum_t <dy[t], W_k[ids[t]]> (float32 [K]) for dy [..., cols] in float32, bfloat16 or float16 and
+    the plan of its ids; ids outside the table add nothing."""
+    dev = _device_of(dy, plan, *qbytes)
+    K, types, ptrs = _table_operands(qtypes, qbytes, rows, padded_cols, cols)
     code = _float_code(dy, "embed_gategrad")
-    if tuple(dy.shape) != (*ids.shape, cols):
-        raise ValueError(f"gradient of shape {(*ids.shape, cols)} expected, got {tuple(dy.shape)}")
-    T = ids.numel()
-    dy = dy.reshape(T, cols)
-    if dy.stride(-1) != 1 or dy.stride(0) < cols:
-        dy = dy.contiguous()
-    K, types, ptrs = _cand_arrays(qtypes, qbytes)
-    need = int(_lib.vq_embed_gategrad_workspace_bytes(T, K))
-    ws = torch.empty(max(need, 4), dtype=torch.uint8, device=ids.device)
-    g = torch.empty(K, dtype=torch.float32, device=ids.device)
-    _check(_lib.vq_embed_gategrad(K, types, ptrs, ids.data_ptr(), int(ids.dtype == torch.int32), T, vocab_start or 0,
-                                  rows, padded_cols, cols, float(scale), dy.data_ptr(), max(dy.stride(0), cols), code,
-                                  ws.data_ptr(), need, g.data_ptr(), _stream(ids)))
+    if dy.dim() < 1 or dy.shape[-1] != cols:
+        raise ValueError(f"gradient rows of {cols} columns expected, got {tuple(dy.shape)}")
+    if dy.dim() != 2:
+        dy = dy.reshape(-1, cols) if cols else dy.new_empty(0, 0)
+    T = dy.shape[0]
+    if plan.numel() != _lib.vq_embed_plan_bytes(T):
+        raise ValueError(f"the plan is not one of {T} tokens")
+    ld, unit = dy.stride()
+    if unit != 1 or ld < cols:
+        dy, ld = dy.contiguous(), cols
+    ws = torch.empty(_lib.vq_embed_gategrad_workspace_bytes(K), dtype=torch.uint8, device=dy.device)
+    g = torch.empty(K, dtype=torch.float32, device=dy.device)
+    _check(_lib.vq_embed_gategrad(K, types, ptrs, plan.data_ptr(), plan.numel(), T, rows, padded_cols, cols, scale,
+                                  dy.data_ptr(), ld, code, ws.data_ptr(), ws.numel(), g.data_ptr(), _raw_stream(dev)))
     return g
 
 
@@ -794,19 +835,22 @@ def clip_grad_norm(tensors, max_norm: float = float("inf"), norm_inf: bool = Fal
     n = len(tensors)
     if n == 0:
         raise ValueError("clip_grad_norm: no tensors")
-    _require_cuda(*tensors)
-    dev = tensors[0].device
-    norm = torch.empty((), dtype=torch.float32, device=dev)
+    # one list per property: a few hundred short tensors cost more here than on the GPU
+    dev = _device_of(tensors[0])
+    if any([t.get_device() != dev for t in tensors]):
+        _device_of(*tensors)
+    if not all([t.is_contiguous() for t in tensors]):
+        raise ValueError("clip_grad_norm: contiguous tensors expected")
     try:
-        codes = [_FLOAT_CODE[t.dtype] for t in tensors]
+        codes = array("i", [_FLOAT_CODE[t.dtype] for t in tensors])
     except KeyError as e:
         raise ValueError(f"clip_grad_norm: float32, bfloat16 or float16 expected, got {e.args[0]}") from None
-    for t in tensors:
-        if t.device != dev or not t.is_contiguous():
-            raise ValueError("clip_grad_norm: contiguous tensors on one device expected")
-    need = int(_lib.vq_clip_grad_norm_workspace_bytes(n))
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    _check(_lib.vq_clip_grad_norm(n, (_vp * n)(*[t.data_ptr() for t in tensors]),
-                                  (ctypes.c_int64 * n)(*[t.numel() for t in tensors]), (_int * n)(*codes),
-                                  float(max_norm), int(norm_inf), ws.data_ptr(), need, norm.data_ptr(), _stream(norm)))
+    ptrs = array("Q", [t.data_ptr() for t in tensors])
+    sizes = array("q", [t.numel() for t in tensors])
+    device = tensors[0].device
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    need = _lib.vq_clip_grad_norm_workspace_bytes(n)
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    _check(_lib.vq_clip_grad_norm(n, ptrs.buffer_info()[0], sizes.buffer_info()[0], codes.buffer_info()[0], max_norm,
+                                  norm_inf, ws.data_ptr(), need, norm.data_ptr(), _raw_stream(dev)))
     return norm

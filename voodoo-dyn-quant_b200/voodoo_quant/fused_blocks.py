@@ -103,21 +103,20 @@ class _QKNormRopeFn(Function):
 
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, cos, sin, eps: float, weight_offset: float):
-        qo, ko = _C.qk_norm_rope_fwd(q, k, q_weight, k_weight, cos, sin, eps, weight_offset)
-        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin)
-        ctx.args = (eps, weight_offset)
+        qo, ko, operands, ctx.layout = _C.qk_norm_rope_fwd(q, k, q_weight, k_weight, cos, sin, eps, weight_offset,
+                                                           saved=True)
+        ctx.save_for_backward(*operands)
+        ctx.weight_types = (q_weight.dtype, k_weight.dtype)
         return qo, ko
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gq: torch.Tensor, gk: torch.Tensor):
-        q, k, q_weight, k_weight, cos, sin = ctx.saved_tensors
-        eps, offset = ctx.args
         need = ctx.needs_input_grad
-        dq, dk, dwq, dwk = _C.qk_norm_rope_bwd(gq, gk, q, k, q_weight, k_weight, cos, sin, eps, offset,
+        dq, dk, dwq, dwk = _C.qk_norm_rope_bwd(gq, gk, ctx.saved_tensors, ctx.layout,
                                                want_weight_grads=need[2] or need[3])
-        return (dq if need[0] else None, dk if need[1] else None, dwq if need[2] else None, dwk if need[3] else None,
-                None, None, None, None)
+        return (dq if need[0] else None, dk if need[1] else None, dwq.to(ctx.weight_types[0]) if need[2] else None,
+                dwk.to(ctx.weight_types[1]) if need[3] else None, None, None, None, None)
 
 
 class _SwiGLUFn(Function):
@@ -195,6 +194,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     and sin are constants.  D and R are multiples of 16, D up to 512."""
     if cos.requires_grad or sin.requires_grad:
         raise ValueError("qk_norm_rope: cos and sin are constants; they cannot require a gradient")
+    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad
+                                         or k_weight.requires_grad)):
+        return _C.qk_norm_rope_fwd(q, k, q_weight, k_weight, cos, sin, eps, weight_offset)
     return _QKNormRopeFn.apply(q, k, q_weight, k_weight, cos, sin, float(eps), float(weight_offset))
 
 

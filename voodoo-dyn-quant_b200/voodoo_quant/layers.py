@@ -709,25 +709,31 @@ class _GatedEmbeddingRowsFunction(Function):
 
 
 class _GatedEmbeddingFunction(Function):
-    """Token rows of a gated table in one kernel, its gate gradient over the
-    sorted tokens in another (``vq_embed_mix``, ``vq_embed_gategrad``): no
-    gathered blocks, no decoded rows, no host round trip."""
+    """Token rows of a gated table in one kernel, its gate gradient in
+    another (``vq_embed_mix``, ``vq_embed_gategrad``), both over one plan of
+    the sorted tokens: no gathered blocks, no decoded rows of a candidate, no
+    host round trip."""
 
     @staticmethod
-    def forward(ctx, probs: torch.Tensor, ids: torch.Tensor, qtypes: tuple, rows: int, padded_cols: int, cols: int,
-                scale: float, vocab_start: int | None, dtype: torch.dtype, *qbytes: torch.Tensor):
-        ctx.save_for_backward(ids, *qbytes)
-        ctx.args = (qtypes, rows, padded_cols, cols, scale, vocab_start, probs.dtype, probs.shape)
-        # the mixture is bf16 everywhere on this path (W_mix); other types hold its bf16 values
-        return _C.embed_mix(ids, qtypes, qbytes, probs, rows, padded_cols, cols, scale, vocab_start).to(dtype)
+    def forward(ctx, probs: torch.Tensor, ids: torch.Tensor, table: tuple, vocab_start: int | None, dtype: torch.dtype):
+        plan = _C.embed_plan(ids, table[2], vocab_start)
+        ctx.save_for_backward(plan)
+        ctx.table, ctx.like = table, (probs.dtype, probs.shape)  # the candidates' blocks are constants
+        return _embedding_rows(probs, ids, table, vocab_start, dtype, plan)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g: torch.Tensor):
-        ids, *qbytes = ctx.saved_tensors
-        qtypes, rows, padded_cols, cols, scale, vocab_start, pdtype, pshape = ctx.args
-        gp = _C.embed_gategrad(g, ids, qtypes, qbytes, rows, padded_cols, cols, scale, vocab_start)
-        return (gp.to(pdtype).view(pshape), *[None] * (8 + len(qbytes)))
+        qtypes, qbytes, rows, padded_cols, cols, scale = ctx.table
+        gp = _C.embed_gategrad(g, ctx.saved_tensors[0], qtypes, qbytes, rows, padded_cols, cols, scale)
+        return gp.to(ctx.like[0]).view(ctx.like[1]), None, None, None, None
+
+
+def _embedding_rows(probs, ids, table, vocab_start, dtype, plan=None):
+    qtypes, qbytes, rows, padded_cols, cols, scale = table
+    out = _C.embed_mix(ids, qtypes, qbytes, probs, rows, padded_cols, cols, scale, vocab_start, plan)
+    # the mixture is bf16 everywhere on this path (W_mix); other types hold its bf16 values
+    return out if dtype == torch.bfloat16 else out.to(dtype)
 
 
 def gated_embedding(ids: torch.Tensor, probs: torch.Tensor, candidate_types, candidate_blocks, num_embeddings: int,
@@ -744,8 +750,10 @@ def gated_embedding(ids: torch.Tensor, probs: torch.Tensor, candidate_types, can
         raise ValueError(f"gated_embedding: float32, bfloat16 or float16 rows, got {dtype}")
     if vocab_start is not None and vocab_start < 0:
         raise ValueError(f"gated_embedding: vocab_start {vocab_start} is negative")
-    return _GatedEmbeddingFunction.apply(probs, ids, tuple(candidate_types), num_embeddings, _padded(embedding_dim),
-                                         embedding_dim, float(scale), vocab_start, dtype, *candidate_blocks)
+    table = (candidate_types, tuple(candidate_blocks), num_embeddings, _padded(embedding_dim), embedding_dim, float(scale))
+    if not (probs.requires_grad and torch.is_grad_enabled()):
+        return _embedding_rows(probs, ids, table, vocab_start, dtype)
+    return _GatedEmbeddingFunction.apply(probs, ids, table, vocab_start, dtype)
 
 
 # --------------------------------------------------------------------------- modules

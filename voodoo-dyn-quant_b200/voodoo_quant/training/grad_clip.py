@@ -33,17 +33,20 @@ def _dense(g: torch.Tensor) -> torch.Tensor | None:
 
 def _run(grads, max_norm: float, norm_type: float) -> torch.Tensor:
     norm_inf = _norm_is_inf(norm_type)
-    flat, copies = [], []
-    for g in grads:
-        if g.layout != torch.strided:
-            raise ValueError("clip_grad_norm_: dense gradients expected")
-        v = _dense(g)
-        if v is None:  # scaled as a copy
-            if any(st == 0 and n > 1 for st, n in zip(g.stride(), g.shape)):
-                raise ValueError("clip_grad_norm_: an expanded gradient shares memory with itself")
-            v = g.contiguous()
-            copies.append((g, v))
-        flat.append(v)
+    copies = []
+    flat = grads
+    if not all([g.layout is torch.strided and g.is_contiguous() for g in grads]):
+        flat = []
+        for g in grads:
+            if g.layout is not torch.strided:
+                raise ValueError("clip_grad_norm_: dense gradients expected")
+            v = _dense(g)
+            if v is None:  # scaled as a copy
+                if any(st == 0 and n > 1 for st, n in zip(g.stride(), g.shape)):
+                    raise ValueError("clip_grad_norm_: an expanded gradient shares memory with itself")
+                v = g.contiguous()
+                copies.append((g, v))
+            flat.append(v)
     norm = _C.clip_grad_norm(flat, max_norm, norm_inf)
     if not math.isinf(max_norm):
         for g, v in copies:
@@ -70,7 +73,7 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0,
     raises RuntimeError before anything is scaled.  Parameters without a gradient are skipped; ``norm_type`` 2 or inf;
     gradients that share memory are refused."""
     params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
-    grads = [p.grad for p in params if p.grad is not None]
+    grads = [g for g in [p.grad for p in params] if g is not None]
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative or NaN, got {max_norm}")
