@@ -13,8 +13,8 @@
 //
 // Eight lanes hold a unit (256 weights) of a row, a lane 32 consecutive
 // weights.  The lanes of a unit copy its packed bytes of every candidate into
-// their own slots of shared memory (16-byte asynchronous copies), the next
-// unit's while this one's are decoded, so that no block-wide barrier is needed.
+// their own slots of shared memory (16-byte asynchronous copies), so that no
+// block-wide barrier is needed; the SM's other warps decode meanwhile.
 #pragma once
 
 #include <type_traits>
@@ -27,7 +27,13 @@ namespace embed {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kUnits = 4;   // units of a warp
-constexpr int kStages = 2;  // of a warp's slots: the next units' bytes arrive while these are decoded
+#ifndef VQ_EMBED_MIX_BLOCKS
+#define VQ_EMBED_MIX_BLOCKS 3
+#endif
+#ifndef VQ_EMBED_GRAD_BLOCKS
+#define VQ_EMBED_GRAD_BLOCKS 3
+#endif
+constexpr int kMixBlocks = VQ_EMBED_MIX_BLOCKS, kGradBlocks = VQ_EMBED_GRAD_BLOCKS;  // resident per SM
 constexpr int kMaxBlocks = 1184;  // of a gradient launch: the partials it leaves
 
 // A unit's slot: the 16-byte aligned span of a 2-byte aligned unit, and a
@@ -49,25 +55,29 @@ __device__ __forceinline__ void async_wait() {
 }
 
 // Copies unit `unit` (of the whole table) of every candidate into slot `lu`
-// of the warp's buffer; lane c of the unit's eight takes every eighth vector.
+// of the warp's buffer; lane c of the unit's eight takes every eighth vector
+// (18 at most: a Q8_0 unit that starts inside a vector).
 __device__ __forceinline__ void stage_unit(const CandSet& cs, uint32_t buf, int lu, int c, long long unit) {
   for (int k = 0; k < cs.K; ++k) {
     const int ub = cs.ubytes[k], slot = slot_bytes(ub);
-    const uintptr_t a = reinterpret_cast<uintptr_t>(cs.ptr[k]) + static_cast<uintptr_t>(unit) * ub;
-    const uintptr_t a0 = a & ~uintptr_t(15);
-    const int n = static_cast<int>((a + ub + 15 - a0) >> 4);
-    const uint32_t dst = buf + lu * slot;
-    for (int v = c; v < n; v += 8) async_copy16(dst + 16 * v, reinterpret_cast<const void*>(a0 + 16 * v));
+    const uint8_t* a = cs.ptr[k] + unit * ub;
+    const int rel = static_cast<int>(reinterpret_cast<uintptr_t>(a) & 15u);
+    const uint8_t* src = a - rel + 16 * c;
+    const uint32_t dst = buf + lu * slot + 16 * c;
+    const int left = rel + ub - 16 * c;  // bytes from this lane's first vector on
+    if (left > 0) async_copy16(dst, src);
+    if (left > 128) async_copy16(dst + 128, src + 128);
+    if (left > 256) async_copy16(dst + 256, src + 256);
     buf += kUnits * slot;
   }
 }
 
-// The staged unit of candidate k, whose slots start at `region`.
-__device__ __forceinline__ URef staged(const CandSet& cs, const uint8_t* region, int k, int lu, long long unit) {
+// The staged unit of candidate k, whose slots start at `region`; `unit` modulo 2^32.
+__device__ __forceinline__ URef staged(const CandSet& cs, const uint8_t* region, int k, int lu, uint32_t unit) {
   const int ub = cs.ubytes[k];
-  const int rel = static_cast<int>((reinterpret_cast<uintptr_t>(cs.ptr[k]) + static_cast<uintptr_t>(unit) * ub) & 15u);
-  return URef{reinterpret_cast<const uint32_t*>(region + lu * slot_bytes(ub) + (rel & ~3)), rel & 3,
-              8u * static_cast<uint32_t>(rel & 3)};
+  const uint32_t rel = (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(cs.ptr[k])) + unit * ub) & 15u;
+  return URef{reinterpret_cast<const uint32_t*>(region + lu * slot_bytes(ub) + (rel & ~3u)), static_cast<int>(rel & 3u),
+              8u * (rel & 3u)};
 }
 
 struct Ids {
@@ -95,33 +105,24 @@ struct Plan {
 // on by many warps, each decoding its row again.
 constexpr int kPieceTokens = 16;
 
-// A team's unit: which of a row, and the tokens that want it.
-struct Unit {
-  long long row;     // of the table, -1: of another one
-  long long begin;   // tokens: places in the order, or (kRuns false) the token itself
-  long long end;
-  int u;             // unit of the row
-};
-
 // The units that eight lanes work on one after the other: unit u of piece
-// (or token) i, i * units_per_row + u ascending by a fixed stride.
+// (kRuns) or token i, i * units_per_row + u ascending by a fixed stride.
 template <bool kRuns>
 struct UnitWalk {
   Plan plan;
   Ids ids;
-  long long count;  // pieces, or tokens
-  long long vocab_start, rows;
-  int units_per_row;
-  long long i, di;
-  int u, du;
+  int count;  // pieces, or tokens
+  long long vocab_start;
+  int rows, units_per_row;
+  int i, di, u, du;
 
   __device__ __forceinline__ void start_at(long long first, long long stride) {
-    i = first / units_per_row;
-    u = static_cast<int>(first - i * units_per_row);
-    di = stride / units_per_row;
-    du = static_cast<int>(stride - di * units_per_row);
+    i = static_cast<int>(first / units_per_row);
+    u = static_cast<int>(first - static_cast<long long>(i) * units_per_row);
+    di = static_cast<int>(stride / units_per_row);
+    du = static_cast<int>(stride - static_cast<long long>(di) * units_per_row);
   }
-  __device__ __forceinline__ bool done() const { return i >= count; }
+  __device__ __forceinline__ bool on() const { return i < count; }
   __device__ __forceinline__ void step() {
     i += di;
     u += du;
@@ -130,23 +131,12 @@ struct UnitWalk {
       ++i;
     }
   }
-  __device__ __forceinline__ Unit get() const {
-    Unit n;
-    n.u = u;
-    if (i >= count) {
-      n.row = -1;
-      n.begin = n.end = 0;
-    } else if (kRuns) {
-      const int key = plan.key[i];
-      n.row = key < rows ? key : -1;
-      n.begin = plan.start[i];
-      n.end = plan.start[i + 1];
-    } else {
-      n.row = local_row(ids.at(i), vocab_start, rows);
-      n.begin = i;
-      n.end = i + 1;
-    }
-    return n;
+  // Row of the table, or -1 for a token of another one.
+  __device__ __forceinline__ int row() const {
+    if (!on()) return -1;
+    if (!kRuns) return static_cast<int>(local_row(ids.at(i), vocab_start, rows));
+    const int key = plan.key[i];
+    return key < rows ? key : -1;
   }
 };
 
@@ -158,46 +148,37 @@ struct UnitWalk {
 // is decoded once per piece of the plan and written to all its tokens;
 // otherwise once per token, with no plan to wait for.
 template <bool kRuns>
-__global__ void __launch_bounds__(kThreads, 2) embed_mix_kernel(CandSet cs, const float* __restrict__ probs, Ids ids,
-                                                                long long T, Plan plan, long long vocab_start,
-                                                                long long rows, int units_per_row, int cols, float scale,
-                                                                bool strict, __nv_bfloat16* __restrict__ out,
-                                                                long long ldo, int* err) {
+__global__ void __launch_bounds__(kThreads, kMixBlocks)
+    embed_mix_kernel(const __grid_constant__ CandSet cs, const float* __restrict__ probs, Ids ids, int T, Plan plan,
+                     long long vocab_start, int rows, int units_per_row, int cols, float scale, bool strict, bool vec,
+                     __nv_bfloat16* __restrict__ out, long long ldo, int* err) {
   extern __shared__ __align__(16) uint8_t esmem[];
   __shared__ float pk_s[kMaxCandidates];
   if (threadIdx.x < cs.K) pk_s[threadIdx.x] = probs[threadIdx.x];
   __syncthreads();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int lu = lane >> 3, c = lane & 7;
-  const int wbytes = warp_bytes(cs);
-  uint8_t* buf = esmem + warp * kStages * wbytes;
+  uint8_t* buf = esmem + warp * warp_bytes(cs);
   UnitWalk<kRuns> w{plan, ids, kRuns ? *plan.count : T, vocab_start, rows, units_per_row};
-  const long long stride = static_cast<long long>(gridDim.x) * kWarps * kUnits;
-  w.start_at((static_cast<long long>(blockIdx.x) * kWarps + warp) * kUnits + lu, stride);
+  w.start_at((static_cast<long long>(blockIdx.x) * kWarps + warp) * kUnits + lu,
+             static_cast<long long>(gridDim.x) * kWarps * kUnits);
   bool bad = false, fmt_ok = true;
-  Unit now = w.get();
-  if (now.row >= 0) stage_unit(cs, smem_u32(buf), lu, c, now.row * units_per_row + now.u);
-  async_commit();
-  w.step();
-  Unit next = w.get();
-  int st = 0;
-  while (__any_sync(0xffffffffu, now.begin < now.end)) {
-    if (next.row >= 0) stage_unit(cs, smem_u32(buf + (st ^ 1) * wbytes), lu, c, next.row * units_per_row + next.u);
+  for (; __any_sync(0xffffffffu, w.on()); w.step()) {
+    const int row = w.row();
+    const long long unit = static_cast<long long>(row) * units_per_row + w.u;
+    if (row >= 0) stage_unit(cs, smem_u32(buf), lu, c, unit);
     async_commit();
-    w.step();
-    const Unit after = w.get();
-    async_wait<1>();
-    __syncwarp();
     float2 acc[16];
 #pragma unroll
     for (int j = 0; j < 16; ++j) acc[j] = make_float2(0.f, 0.f);
     float cst[2] = {0.f, 0.f};
-    const int col = 256 * now.u + 32 * c;
-    if (now.row >= 0 && col < cols) {
-      const uint8_t* region = buf + st * wbytes;
-      const long long unit = now.row * units_per_row + now.u;
+    const int col = 256 * w.u + 32 * c;
+    async_wait<0>();
+    __syncwarp();
+    if (row >= 0 && col < cols) {
+      const uint8_t* region = buf;
       for (int k = 0; k < cs.K; ++k) {
-        const URef ur = staged(cs, region, k, lu, unit);
+        const URef ur = staged(cs, region, k, lu, static_cast<uint32_t>(unit));
         const float pk = pk_s[k];
         switch (cs.fmt[k]) {
           case kQ8_0: mix_chunk<kQ8_0>(ur, c, pk, acc, cst); break;
@@ -212,32 +193,32 @@ __global__ void __launch_bounds__(kThreads, 2) embed_mix_kernel(CandSet cs, cons
         region += kUnits * slot_bytes(cs.ubytes[k]);
       }
     }
-    bad |= now.row < 0 && now.begin < now.end;
-    if (col < cols) {
-      __align__(16) __nv_bfloat162 hv[16];
+    if (w.on()) {
+      bad |= row < 0;
+      if (col < cols) {
+        __align__(16) __nv_bfloat162 hv[16];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float cs0 = cst[j >> 3];
-        hv[j] = __floats2bfloat162_rn((acc[j].x + cs0) * scale, (acc[j].y + cs0) * scale);
-      }
-      for (long long i = now.begin; i < now.end; ++i) {
-        __nv_bfloat16* dst = out + (kRuns ? static_cast<long long>(plan.order[i]) : i) * ldo + col;
-        if (col + 32 <= cols && (reinterpret_cast<uintptr_t>(dst) & 15u) == 0) {
+        for (int j = 0; j < 16; ++j) {
+          const float cs0 = cst[j >> 3];
+          hv[j] = __floats2bfloat162_rn((acc[j].x + cs0) * scale, (acc[j].y + cs0) * scale);
+        }
+        const int begin = kRuns ? plan.start[w.i] : w.i, end = kRuns ? plan.start[w.i + 1] : w.i + 1;
+        for (int i = begin; i < end; ++i) {
+          __nv_bfloat16* dst = out + static_cast<long long>(kRuns ? plan.order[i] : i) * ldo + col;
+          if (vec && col + 32 <= cols) {
 #pragma unroll
-          for (int v = 0; v < 4; ++v) reinterpret_cast<uint4*>(dst)[v] = reinterpret_cast<const uint4*>(hv)[v];
-        } else {
+            for (int v = 0; v < 4; ++v) reinterpret_cast<uint4*>(dst)[v] = reinterpret_cast<const uint4*>(hv)[v];
+          } else {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            if (col + 2 * j < cols) dst[2 * j] = hv[j].x;
-            if (col + 2 * j + 1 < cols) dst[2 * j + 1] = hv[j].y;
+            for (int j = 0; j < 16; ++j) {
+              if (col + 2 * j < cols) dst[2 * j] = hv[j].x;
+              if (col + 2 * j + 1 < cols) dst[2 * j + 1] = hv[j].y;
+            }
           }
         }
       }
     }
     __syncwarp();  // the slots are filled again
-    now = next;
-    next = after;
-    st ^= 1;
   }
   if (bad && strict) report_error(err, kDevBadIndex, 30);
   if (!fmt_ok) report_error(err, kDevBadFormat, 3);
@@ -434,11 +415,12 @@ __device__ __forceinline__ float dot_chunk(const URef& u, int c, const float2 (&
   return d;
 }
 
-// Adds 32 values of a row of dy at column col (zeros past cols).
+// Adds 32 values of a row of dy at column col (zeros past cols); vec: the rows
+// are 16-byte aligned.
 template <typename T>
-__device__ __forceinline__ void add_row(const T* row, int col, int cols, float2 (&g)[16]) {
+__device__ __forceinline__ void add_row(const T* row, int col, int cols, bool vec, float2 (&g)[16]) {
   constexpr int kPer = 16 / sizeof(T);
-  if (col + 32 <= cols && (reinterpret_cast<uintptr_t>(row + col) & 15u) == 0) {
+  if (vec && col + 32 <= cols) {
     uint4 v[32 / kPer];
 #pragma unroll
     for (int j = 0; j < 32 / kPer; ++j) v[j] = __ldg(reinterpret_cast<const uint4*>(row + col) + j);
@@ -479,50 +461,44 @@ __device__ __forceinline__ void add_row(const T* row, int col, int cols, float2 
 // (an index that varies would put a register array into local memory), and
 // the block's are left in partials[blockIdx.x][K].
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) embed_gategrad_kernel(CandSet cs, Plan plan, long long rows,
-                                                                     int units_per_row, int cols,
-                                                                     const T* __restrict__ dy, long long lddy,
-                                                                     double* __restrict__ partials, int* err) {
+__global__ void __launch_bounds__(kThreads, kGradBlocks)
+    embed_gategrad_kernel(const __grid_constant__ CandSet cs, Plan plan, int rows, int units_per_row, int cols,
+                          const T* __restrict__ dy, long long lddy, bool vec, double* __restrict__ partials, int* err) {
   extern __shared__ __align__(16) uint8_t esmem[];
   double* acc = reinterpret_cast<double*>(esmem);  // [K][kThreads]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int lu = lane >> 3, c = lane & 7;
-  const int wbytes = warp_bytes(cs);
-  uint8_t* buf = esmem + cs.K * kThreads * sizeof(double) + warp * kStages * wbytes;
+  uint8_t* buf = esmem + cs.K * kThreads * sizeof(double) + warp * warp_bytes(cs);
   for (int k = 0; k < cs.K; ++k) acc[k * kThreads + threadIdx.x] = 0.0;
   UnitWalk<true> w{plan, Ids{nullptr, false}, *plan.count, 0, rows, units_per_row};
-  const long long stride = static_cast<long long>(gridDim.x) * kWarps * kUnits;
-  w.start_at((static_cast<long long>(blockIdx.x) * kWarps + warp) * kUnits + lu, stride);
+  w.start_at((static_cast<long long>(blockIdx.x) * kWarps + warp) * kUnits + lu,
+             static_cast<long long>(gridDim.x) * kWarps * kUnits);
   bool fmt_ok = true;
-  Unit now = w.get();
-  if (now.row >= 0) stage_unit(cs, smem_u32(buf), lu, c, now.row * units_per_row + now.u);
-  async_commit();
-  w.step();
-  Unit next = w.get();
-  int st = 0;
-  while (__any_sync(0xffffffffu, now.row >= 0)) {  // other shards' pieces come last
-    if (next.row >= 0) stage_unit(cs, smem_u32(buf + (st ^ 1) * wbytes), lu, c, next.row * units_per_row + next.u);
+  for (;; w.step()) {
+    const int row = w.row();
+    if (!__any_sync(0xffffffffu, row >= 0)) break;  // other shards' pieces come last
+    const long long unit = static_cast<long long>(row) * units_per_row + w.u;
+    if (row >= 0) stage_unit(cs, smem_u32(buf), lu, c, unit);
     async_commit();
-    w.step();
-    const Unit after = w.get();
-    const int col = 256 * now.u + 32 * c;
-    const bool on = now.row >= 0 && col < cols;
+    const int col = 256 * w.u + 32 * c;
+    const bool on = row >= 0 && col < cols;
     float2 g[16];
 #pragma unroll
     for (int j = 0; j < 16; ++j) g[j] = make_float2(0.f, 0.f);
-    if (on)
-      for (long long i = now.begin; i < now.end; ++i)
-        add_row<T>(dy + static_cast<long long>(plan.order[i]) * lddy, col, cols, g);
+    if (on) {
+      const int end = plan.start[w.i + 1];
+      for (int i = plan.start[w.i]; i < end; ++i)
+        add_row<T>(dy + static_cast<long long>(plan.order[i]) * lddy, col, cols, vec, g);
+    }
     float gs[2] = {0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < 16; ++j) gs[j >> 3] += g[j].x + g[j].y;
-    async_wait<1>();
+    async_wait<0>();
     __syncwarp();
     if (on) {
-      const uint8_t* region = buf + st * wbytes;
-      const long long unit = now.row * units_per_row + now.u;
+      const uint8_t* region = buf;
       for (int k = 0; k < cs.K; ++k) {
-        const URef ur = staged(cs, region, k, lu, unit);
+        const URef ur = staged(cs, region, k, lu, static_cast<uint32_t>(unit));
         float d = 0.f;
         switch (cs.fmt[k]) {
           case kQ8_0: d = dot_chunk<kQ8_0>(ur, c, g, gs); break;
@@ -539,11 +515,7 @@ __global__ void __launch_bounds__(kThreads, 2) embed_gategrad_kernel(CandSet cs,
       }
     }
     __syncwarp();  // the slots are filled again
-    now = next;
-    next = after;
-    st ^= 1;
   }
-  async_wait<0>();
   if (!fmt_ok) report_error(err, kDevBadFormat, 4);
   __syncthreads();
   for (int k = warp; k < cs.K; k += kWarps) {

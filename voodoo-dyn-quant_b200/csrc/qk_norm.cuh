@@ -34,7 +34,15 @@ constexpr int kMaxDim = 512;  // 32 lanes of 16 values
 #ifndef VQ_QK_BWD_BLOCKS_WIDE
 #define VQ_QK_BWD_BLOCKS_WIDE 3
 #endif
-// Resident blocks per SM; fp32 tables take twice the registers in the backward.
+#ifndef VQ_QK_FWD_BLOCKS_WIDE
+#define VQ_QK_FWD_BLOCKS_WIDE 4
+#endif
+#ifndef VQ_QK_DEPTH
+#define VQ_QK_DEPTH 4
+#endif
+constexpr int kDepth = VQ_QK_DEPTH;  // steps of the ring: one being computed, the others on their way
+// Resident blocks per SM; fp32 heads or tables take twice the registers.
+constexpr int kFwdBlocksWide = VQ_QK_FWD_BLOCKS_WIDE;
 constexpr int kFwdBlocks = VQ_QK_FWD_BLOCKS, kBwdBlocks = VQ_QK_BWD_BLOCKS, kBwdBlocksWide = VQ_QK_BWD_BLOCKS_WIDE;
 // Blocks of one launch at most: the rows of the weight-gradient partials.
 constexpr int kMaxBlocks = 2368;
@@ -132,7 +140,8 @@ struct Shape {
   bool w_f32;
 };
 
-// Eight weights from column c, with the offset.
+// Eight weights from column c, with the offset (read once a position in the
+// forward, where they would take registers from the loop: they are in L1).
 template <typename T>
 __device__ __forceinline__ F8 weights(const void* w, bool f32, int c, float offset) {
   F8 f;
@@ -159,98 +168,194 @@ __device__ __forceinline__ float sum_squares(const F8& a, const F8& b) {
   return s.x + s.y;
 }
 
-__device__ __forceinline__ float team_sum(float v, int team) {
-  for (int o = team >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+// Sum over the lanes of a head.  kTeam: log2 of their number, -1: only known at run time.
+template <int kTeam>
+__device__ __forceinline__ float team_sum(float v, int team_log2) {
+  if constexpr (kTeam >= 0) {
+#pragma unroll
+    for (int o = (1 << kTeam) >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  } else {
+    for (int o = (1 << team_log2) >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  }
   return v;
 }
 
-// What both kernels share: the lane's places in a head, and its walk over
-// the items (position, piece of its heads) of its side with the heads of the
-// next step on their way while this one's are computed.
+__device__ __forceinline__ void async_copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Shared memory of a block: kDepth steps of every thread's own values.
 template <typename T, bool kGrad>
+constexpr int ring_bytes() {
+  return kDepth * (kGrad ? 4 : 2) * 8 * static_cast<int>(sizeof(T)) * kThreads;
+}
+
+// What both kernels share: the lane's places in a head, and its walk over
+// the items (position, piece of its heads) of its side.  A thread copies the
+// values of the steps to come into a ring of its own in shared memory
+// (asynchronous copies, read back by the same thread: no barrier), since the
+// registers that plain loads ahead would take hold too few bytes in flight:
+// at one step ahead the kernels ran at the memory's latency (72 us forward
+// for 16384 x 40 heads of 128, 106 us backward).  Lanes past the end of a
+// head, and teams past the last head, read one that exists and leave nothing:
+// that is cheaper than holding their loads back.
+template <typename T, bool kGrad, int kTeam>
 struct Walk {
+  static constexpr int kVecs = static_cast<int>(sizeof(T)) / 2;  // 16-byte vectors of eight values
+  static constexpr uint32_t kStep = (kGrad ? 4 : 2) * kVecs * 16 * kThreads;  // bytes of a step, all threads
+  static_assert((kDepth & (kDepth - 1)) == 0, "the ring wraps by masking");
   const Side<T>& side;
   const Shape& sh;
-  int team, per_warp, slot, a, b;
+  int team_log2, per_warp, slot, a, b, H, iters;
   bool live, turned;
-  unsigned items, stride, item;
-  const T *xp, *gp;  // next heads to fetch
-  int h;             // the one to fetch
-  long long xstep, gstep;
-  Raw8<T> x1, x2, g1, g2;
+  // Where an item lies: its piece of the position's heads, and the position
+  // (place in the sequence, batch entry); kept by additions, since a division
+  // an item cost more than its heads' arithmetic.
+  struct At {
+    unsigned item, c, s, b;
+  };
+  At at, by, ahead;  // of the current item, of a stride, of the item to copy next
+  unsigned items, chunks, S;
+  int f_left, f_h;
+  const T *xp, *gp;  // heads of the position to copy next, at this lane's place
+  long long xh, gh;
+  uint32_t ring, f_off, r_off;
+  const uint8_t* ring_p;
 
-  __device__ __forceinline__ Walk(const Side<T>& side_, const Shape& sh_, unsigned block) : side(side_), sh(sh_) {
+  __device__ __forceinline__ Walk(const Side<T>& side_, const Shape& sh_, unsigned block, uint8_t* smem)
+      : side(side_), sh(sh_) {
     const int lane = threadIdx.x & 31;
-    team = 1 << sh.team_log2;
-    per_warp = 32 >> sh.team_log2;
-    slot = lane >> sh.team_log2;
-    const int i = lane & (team - 1);
+    team_log2 = kTeam >= 0 ? kTeam : sh.team_log2;
+    per_warp = 32 >> team_log2;
+    slot = lane >> team_log2;
+    const int i = lane & ((1 << team_log2) - 1);
     live = 16 * i < sh.D;
     turned = 16 * i < sh.R;
-    a = turned ? 8 * i : 16 * i;
-    b = turned ? sh.R / 2 + 8 * i : 16 * i + 8;
-    items = sh.positions * static_cast<unsigned>(side.chunks);
-    stride = static_cast<unsigned>(side.blocks) * kWarps;
-    item = block * kWarps + (threadIdx.x >> 5);
-    xstep = per_warp * side.xh;
-    gstep = per_warp * side.gh;
+    a = turned ? 8 * i : live ? 16 * i : 0;
+    b = turned ? sh.R / 2 + 8 * i : a + 8;
+    H = side.H;
+    iters = side.iters;
+    xh = side.xh;
+    gh = side.gh;
+    S = sh.S;
+    chunks = static_cast<unsigned>(side.chunks);
+    items = sh.positions * chunks;
+    by = place(static_cast<unsigned>(side.blocks) * kWarps);
+    // one value a warp, in the open, lets the compiler branch on it without masks
+    at = place(block * kWarps + __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0));
+    ahead = at;
+    ring_p = smem + 16 * threadIdx.x;
+    ring = smem_u32(ring_p);
+    f_off = r_off = 0;
+    f_left = 0;
+    if (at.item < items) aim();
+#pragma unroll
+    for (int s = 0; s < kDepth - 1; ++s) copy_step();
   }
 
-  // Position (batch entry, place in the sequence) and first head of an item.
-  __device__ __forceinline__ void place(unsigned it, unsigned& bi, unsigned& si, int& h0) const {
-    const unsigned pos = it / static_cast<unsigned>(side.chunks);
-    h0 = static_cast<int>(it - pos * side.chunks) * side.iters * per_warp + slot;
-    bi = pos / sh.S;
-    si = pos - bi * sh.S;
+  __device__ __forceinline__ At place(unsigned item) const {
+    At p;
+    p.item = item;
+    const unsigned pos = chunks > 1 ? item / chunks : item;
+    p.c = item - pos * chunks;
+    p.b = pos / S;
+    p.s = pos - p.b * S;
+    return p;
   }
-
-  __device__ __forceinline__ void aim(unsigned bi, unsigned si, int h0) {
-    h = h0;
-    xp = side.x + bi * side.xb + si * side.xs + h * side.xh + a;
-    if (kGrad) gp = side.g + bi * side.gb + si * side.gs + h * side.gh + a;
-  }
-
-  __device__ __forceinline__ void fetch() {
-    if (live && h < side.H) {
-      x1.load(xp);
-      x2.load(xp + (b - a));
-      if (kGrad) {
-        g1.load(gp);
-        g2.load(gp + (b - a));
-      }
-    } else {
-      x1.zero();
-      x2.zero();
-      if (kGrad) {
-        g1.zero();
-        g2.zero();
-      }
+  // Moves an item on by the stride; false at the end.
+  __device__ __forceinline__ bool next(At& p) const {
+    if (items - p.item <= by.item) return false;
+    p.item += by.item;
+    p.c += by.c;
+    p.s += by.s;
+    p.b += by.b;
+    if (p.c >= chunks) {
+      p.c -= chunks;
+      ++p.s;
     }
-    h += per_warp;
-    xp += xstep;
-    if (kGrad) gp += gstep;
+    if (p.s >= S) {
+      p.s -= S;
+      ++p.b;
+    }
+    return true;
   }
+  __device__ __forceinline__ int first_head(const At& p) const { return static_cast<int>(p.c) * iters * per_warp + slot; }
+
+  __device__ __forceinline__ void aim() {
+    f_h = first_head(ahead);
+    xp = side.x + ahead.b * side.xb + ahead.s * side.xs + a;
+    if (kGrad) gp = side.g + ahead.b * side.gb + ahead.s * side.gs + a;
+    f_left = iters;
+  }
+
+  __device__ __forceinline__ void copy8(int part, const T* p) {
+    const uint32_t d = ring + f_off + part * (16 * kThreads);
+    async_copy16(d, p);
+    if (kVecs == 2) async_copy16(d + 16 * kThreads, p + 4);
+  }
+
+  // Starts the copies of the next step, if there is one; a group either way.
+  __device__ __forceinline__ void copy_step() {
+    if (f_left > 0) {
+      const int h = min(f_h, H - 1);
+      const T* p = xp + h * xh;
+      copy8(0, p);
+      copy8(kVecs, p + (b - a));
+      if (kGrad) {
+        const T* e = gp + h * gh;
+        copy8(2 * kVecs, e);
+        copy8(3 * kVecs, e + (b - a));
+      }
+      f_h += per_warp;
+      if (--f_left == 0 && next(ahead)) aim();
+    }
+    async_commit();
+    f_off = (f_off + kStep) & (kDepth * kStep - 1);
+  }
+
+  __device__ __forceinline__ F8 read8(int part) const {
+    const uint8_t* p = ring_p + r_off + part * (16 * kThreads);
+    Raw8<T> r;
+    if constexpr (kVecs == 2) {
+      r.a = *reinterpret_cast<const float4*>(p);
+      r.b = *reinterpret_cast<const float4*>(p + 16 * kThreads);
+    } else {
+      r.q = *reinterpret_cast<const uint4*>(p);
+    }
+    return widen(r);
+  }
+
+  // Makes the current step's values readable (read8) after starting those of a later one.
+  __device__ __forceinline__ void arrive() {
+    copy_step();
+    async_wait<kDepth - 1>();
+  }
+  __device__ __forceinline__ void leave() { r_off = (r_off + kStep) & (kDepth * kStep - 1); }
 };
 
 // Forward.  With A = (offset + w) cos and B = the partner's (offset + w) sin,
 // held for all heads of a position, a pair is r (x1 A1 - x2 B1),
 // r (x2 A2 + x1 B2).  One warp per item, grid-stride within a side; the first
 // q.blocks blocks serve the queries, the rest the keys.  TC: type of the tables.
-template <typename T, typename TC>
-__global__ void __launch_bounds__(kThreads, kFwdBlocks)
+template <typename T, typename TC, int kTeam>
+__global__ void __launch_bounds__(kThreads, sizeof(TC) == 4 ? kFwdBlocksWide : kFwdBlocks)
     qk_norm_rope_fwd_kernel(const __grid_constant__ Side<T> q, const __grid_constant__ Side<T> k,
                             const __grid_constant__ Shape sh) {
+  extern __shared__ __align__(16) uint8_t qsmem[];
   const bool is_q = blockIdx.x < static_cast<unsigned>(q.blocks);
   const Side<T>& side = is_q ? q : k;
-  Walk<T, false> w(side, sh, is_q ? blockIdx.x : blockIdx.x - q.blocks);
-  if (w.item >= w.items) return;
-  const float inv_d = 1.f / static_cast<float>(sh.D);
-  unsigned bi, si;
-  int h0;
-  w.place(w.item, bi, si, h0);
-  w.aim(bi, si, h0);
-  w.fetch();
-  for (;;) {
+  Walk<T, false, kTeam> w(side, sh, is_q ? blockIdx.x : blockIdx.x - q.blocks, qsmem);
+  const float inv_d = 1.f / static_cast<float>(sh.D), eps = sh.eps;
+  const long long ostep = static_cast<long long>(w.per_warp) * sh.D;
+  bool more = w.at.item < w.items;
+  while (more) {
+    const unsigned bi = w.at.b, si = w.at.s;
+    int h = w.first_head(w.at);
     F8 a1, a2, b1, b2;
 #pragma unroll
     for (int j = 0; j < 4; ++j) a1.v[j] = a2.v[j] = b1.v[j] = b2.v[j] = both(0.f);
@@ -276,22 +381,15 @@ __global__ void __launch_bounds__(kThreads, kFwdBlocks)
         }
       }
     }
-    int hh = h0;
-    T* op = side.out + ((static_cast<long long>(bi) * sh.S + si) * side.H + hh) * sh.D + w.a;
-    const long long ostep = static_cast<long long>(w.per_warp) * sh.D;
-    const bool more = w.items - w.item > w.stride;
-    for (int it = side.iters; it > 0; --it) {
-      const Raw8<T> r1 = w.x1, r2 = w.x2;
-      if (it > 1) {
-        w.fetch();
-      } else if (more) {
-        w.item += w.stride;
-        w.place(w.item, bi, si, h0);
-        w.aim(bi, si, h0);
-        w.fetch();
-      }
-      const F8 x1 = widen(r1), x2 = widen(r2);
-      const float r = rsqrtf(fmaf(team_sum(sum_squares(x1, x2), w.team), inv_d, sh.eps));
+    T* op = side.out + ((static_cast<long long>(bi) * sh.S + si) * w.H + h) * sh.D + w.a;
+    more = w.next(w.at);
+#pragma unroll 1
+    for (int it = w.iters; it > 0; --it) {
+      w.arrive();
+      const F8 x1 = w.read8(0), x2 = w.read8(w.kVecs);
+      w.leave();
+      const float ss = w.live ? sum_squares(x1, x2) : 0.f;
+      const float r = rsqrtf(fmaf(team_sum<kTeam>(ss, w.team_log2), inv_d, eps));
       F8 o1, o2;
       if (w.turned) {
 #pragma unroll
@@ -306,27 +404,28 @@ __global__ void __launch_bounds__(kThreads, kFwdBlocks)
           o2.v[j] = __fmul2_rn(both(r), __fmul2_rn(x2.v[j], a2.v[j]));
         }
       }
-      if (w.live && hh < side.H) {
+      if (w.live && h < w.H) {
         store8<T>(op, o1);
         store8<T>(op + (w.b - w.a), o2);
       }
-      hh += w.per_warp;
+      h += w.per_warp;
       op += ostep;
     }
-    if (!more) break;
   }
 }
 
 // Backward, on the same items.  kWeights: also leave this block's sum of
 // g * n, of its side's weight gradient, in partials[blockIdx.x][D].
-template <typename T, typename TC, bool kWeights>
+template <typename T, typename TC, bool kWeights, int kTeam>
 __global__ void __launch_bounds__(kThreads, sizeof(TC) == 4 ? kBwdBlocksWide : kBwdBlocks)
     qk_norm_rope_bwd_kernel(const __grid_constant__ Side<T> q, const __grid_constant__ Side<T> k,
                             const __grid_constant__ Shape sh, float* __restrict__ partials) {
+  extern __shared__ __align__(16) uint8_t qsmem[];
   const bool is_q = blockIdx.x < static_cast<unsigned>(q.blocks);
   const Side<T>& side = is_q ? q : k;
-  Walk<T, true> w(side, sh, is_q ? blockIdx.x : blockIdx.x - q.blocks);
-  const float inv_d = 1.f / static_cast<float>(sh.D);
+  Walk<T, true, kTeam> w(side, sh, is_q ? blockIdx.x : blockIdx.x - q.blocks, qsmem);
+  const float inv_d = 1.f / static_cast<float>(sh.D), eps = sh.eps;
+  const long long ostep = static_cast<long long>(w.per_warp) * sh.D;
   F8 w1, w2, dw1, dw2;
 #pragma unroll
   for (int j = 0; j < 4; ++j) w1.v[j] = w2.v[j] = dw1.v[j] = dw2.v[j] = both(0.f);
@@ -334,15 +433,10 @@ __global__ void __launch_bounds__(kThreads, sizeof(TC) == 4 ? kBwdBlocksWide : k
     w1 = weights<T>(side.w, sh.w_f32, w.a, sh.offset);
     w2 = weights<T>(side.w, sh.w_f32, w.b, sh.offset);
   }
-  unsigned bi = 0, si = 0;
-  int h0 = 0;
-  bool more = w.item < w.items;
-  if (more) {
-    w.place(w.item, bi, si, h0);
-    w.aim(bi, si, h0);
-    w.fetch();
-  }
+  bool more = w.at.item < w.items;
   while (more) {
+    const unsigned bi = w.at.b, si = w.at.s;
+    int h = w.first_head(w.at);
     Raw8<TC> c1r, c2r, s1r, s2r;
     c1r.zero(), c2r.zero(), s1r.zero(), s2r.zero();
     if (w.turned) {
@@ -354,23 +448,16 @@ __global__ void __launch_bounds__(kThreads, sizeof(TC) == 4 ? kBwdBlocksWide : k
       s1r.load(sp + w.a);
       s2r.load(sp + w.b);
     }
-    int hh = h0;
-    T* op = side.out + ((static_cast<long long>(bi) * sh.S + si) * side.H + hh) * sh.D + w.a;
-    const long long ostep = static_cast<long long>(w.per_warp) * sh.D;
-    more = w.items - w.item > w.stride;
-    for (int it = side.iters; it > 0; --it) {
-      const Raw8<T> r1 = w.x1, r2 = w.x2, e1 = w.g1, e2 = w.g2;
-      if (it > 1) {
-        w.fetch();
-      } else if (more) {
-        w.item += w.stride;
-        w.place(w.item, bi, si, h0);
-        w.aim(bi, si, h0);
-        w.fetch();
-      }
-      F8 n1 = widen(r1), n2 = widen(r2);
-      const float r = rsqrtf(fmaf(team_sum(sum_squares(n1, n2), w.team), inv_d, sh.eps));
-      F8 g1 = widen(e1), g2 = widen(e2);
+    T* op = side.out + ((static_cast<long long>(bi) * sh.S + si) * w.H + h) * sh.D + w.a;
+    more = w.next(w.at);
+#pragma unroll 1
+    for (int it = w.iters; it > 0; --it) {
+      w.arrive();
+      F8 n1 = w.read8(0), n2 = w.read8(w.kVecs), g1 = w.read8(2 * w.kVecs), g2 = w.read8(3 * w.kVecs);
+      w.leave();
+      const float ss = w.live ? sum_squares(n1, n2) : 0.f;
+      const float r = rsqrtf(fmaf(team_sum<kTeam>(ss, w.team_log2), inv_d, eps));
+      const float rw = h < w.H ? r : 0.f;  // a team past the last head adds nothing to the weights' sum
       if (w.turned) {
         c1r.stay(), c2r.stay(), s1r.stay(), s2r.stay();
         const F8 c1 = widen(c1r), c2 = widen(c2r), s1 = widen(s1r), s2 = widen(s2r);
@@ -384,8 +471,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(TC) == 4 ? kBwdBlocksWide : k
       float2 dot = both(0.f);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        n1.v[j] = __fmul2_rn(n1.v[j], both(r));
-        n2.v[j] = __fmul2_rn(n2.v[j], both(r));
+        n1.v[j] = __fmul2_rn(n1.v[j], both(rw));
+        n2.v[j] = __fmul2_rn(n2.v[j], both(rw));
         if (kWeights) {
           dw1.v[j] = __ffma2_rn(g1.v[j], n1.v[j], dw1.v[j]);
           dw2.v[j] = __ffma2_rn(g2.v[j], n2.v[j], dw2.v[j]);
@@ -395,17 +482,17 @@ __global__ void __launch_bounds__(kThreads, sizeof(TC) == 4 ? kBwdBlocksWide : k
         dot = __ffma2_rn(g1.v[j], n1.v[j], dot);
         dot = __ffma2_rn(g2.v[j], n2.v[j], dot);
       }
-      const float m = -team_sum(dot.x + dot.y, w.team) * inv_d;
+      const float m = -team_sum<kTeam>(w.live ? dot.x + dot.y : 0.f, w.team_log2) * inv_d;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         n1.v[j] = __fmul2_rn(both(r), __ffma2_rn(n1.v[j], both(m), g1.v[j]));
         n2.v[j] = __fmul2_rn(both(r), __ffma2_rn(n2.v[j], both(m), g2.v[j]));
       }
-      if (w.live && hh < side.H) {
+      if (w.live && h < w.H) {
         store8<T>(op, n1);
         store8<T>(op + (w.b - w.a), n2);
       }
-      hh += w.per_warp;
+      h += w.per_warp;
       op += ostep;
     }
   }
@@ -414,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(TC) == 4 ? kBwdBlocksWide : k
     __shared__ float red[kWarps][kMaxDim];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      for (int o = w.team; o < 32; o <<= 1) {
+      for (int o = 1 << w.team_log2; o < 32; o <<= 1) {
         dw1.v[j].x += __shfl_xor_sync(0xffffffffu, dw1.v[j].x, o);
         dw1.v[j].y += __shfl_xor_sync(0xffffffffu, dw1.v[j].y, o);
         dw2.v[j].x += __shfl_xor_sync(0xffffffffu, dw2.v[j].x, o);

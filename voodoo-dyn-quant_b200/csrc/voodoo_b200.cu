@@ -19,6 +19,7 @@
 #include <atomic>
 #include <cstring>
 #include <mutex>
+#include <type_traits>
 
 #include "common.cuh"
 #include "formats.cuh"
@@ -1247,21 +1248,32 @@ int launch_qk(const QkArgs& a, const QkPlan& p, float* partials, cudaStream_t st
   sh.eps = a.eps, sh.offset = a.offset;
   sh.w_f32 = a.w_f32;
   const int grid = p.q_blocks + p.k_blocks;
-  if constexpr (!kBackward) {
-    if (a.cs_f32)
-      qk_norm_rope_fwd_kernel<T, float><<<grid, kThreads, 0, st>>>(q, k, sh);
-    else
-      qk_norm_rope_fwd_kernel<T, T><<<grid, kThreads, 0, st>>>(q, k, sh);
-  } else if (a.cs_f32) {
-    if (partials != nullptr)
-      qk_norm_rope_bwd_kernel<T, float, true><<<grid, kThreads, 0, st>>>(q, k, sh, partials);
-    else
-      qk_norm_rope_bwd_kernel<T, float, false><<<grid, kThreads, 0, st>>>(q, k, sh, partials);
+  constexpr int smem = ring_bytes<T, kBackward>();
+  auto start = [&](auto kern, auto... more) {
+    cudaError_t e = cudaSuccess;
+    if (smem > 32 * 1024) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess) kern<<<grid, kThreads, smem, st>>>(q, k, sh, more...);
+    return e;
+  };
+  // the usual head dimensions (33 to 256) know their team's size at compile time
+  auto launch = [&](auto team) {
+    constexpr int kTeam = decltype(team)::value;
+    if constexpr (!kBackward) return start(qk_norm_rope_fwd_kernel<T, T, kTeam>);
+    else if (partials != nullptr) return start(qk_norm_rope_bwd_kernel<T, T, true, kTeam>, partials);
+    else return start(qk_norm_rope_bwd_kernel<T, T, false, kTeam>, partials);
+  };
+  if (a.cs_f32 && sizeof(T) != 4) {
+    if constexpr (!kBackward) VQ_CUDA(start(qk_norm_rope_fwd_kernel<T, float, -1>));
+    else if (partials != nullptr) VQ_CUDA(start(qk_norm_rope_bwd_kernel<T, float, true, -1>, partials));
+    else VQ_CUDA(start(qk_norm_rope_bwd_kernel<T, float, false, -1>, partials));
+  } else if (p.team_log2 == 2) {
+    VQ_CUDA(launch(std::integral_constant<int, 2>{}));
+  } else if (p.team_log2 == 3) {
+    VQ_CUDA(launch(std::integral_constant<int, 3>{}));
+  } else if (p.team_log2 == 4) {
+    VQ_CUDA(launch(std::integral_constant<int, 4>{}));
   } else {
-    if (partials != nullptr)
-      qk_norm_rope_bwd_kernel<T, T, true><<<grid, kThreads, 0, st>>>(q, k, sh, partials);
-    else
-      qk_norm_rope_bwd_kernel<T, T, false><<<grid, kThreads, 0, st>>>(q, k, sh, partials);
+    VQ_CUDA(launch(std::integral_constant<int, -1>{}));
   }
   VQ_CUDA(cudaGetLastError());
   return 0;
@@ -1290,7 +1302,9 @@ int vq_qk_norm_rope_fwd(const void* q, const int64_t* q_strides, int64_t Hq, con
   if ((Hq > 0 && (q_out == nullptr || !aligned16(q_out))) || (Hk > 0 && (k_out == nullptr || !aligned16(k_out))))
     return fail(VQ_ERR_INVALID, "outputs must be 16-byte aligned pointers");
   QkPlan p;
-  if (int rc = qk_plan(&p, B * S, Hq, Hk, D, vq::qknorm::kFwdBlocks)) return rc;
+  if (int rc = qk_plan(&p, B * S, Hq, Hk, D,
+                       cs_f32 || dtype == 0 ? vq::qknorm::kFwdBlocksWide : vq::qknorm::kFwdBlocks))
+    return rc;
   const QkArgs a{q,  k,  nullptr, nullptr, q_weight, k_weight, cos, sin, q_strides, k_strides, nullptr, nullptr, cs_strides,
                  Hq, Hk, B,       S,       D,        R,        weight_f32 != 0, cs_f32 != 0, eps, weight_offset, q_out, k_out};
   return launch_qk_dtype<false>(a, p, dtype, nullptr, static_cast<cudaStream_t>(stream));
@@ -1416,10 +1430,11 @@ int launch_embed_gategrad(const vq::CandSet& cs, const vq::embed::Plan& plan, lo
                           int cols, const void* dy, long long lddy, double* partials, int* blocks, int* err,
                           cudaStream_t st) {
   using namespace vq::embed;
-  const int smem = cs.K * kThreads * static_cast<int>(sizeof(double)) + kWarps * kStages * warp_bytes(cs);
+  const int smem = cs.K * kThreads * static_cast<int>(sizeof(double)) + kWarps * warp_bytes(cs);
   if (int rc = one_wave(embed_gategrad_kernel<T>, smem, tokens * upr, blocks)) return rc;
-  embed_gategrad_kernel<T><<<*blocks, kThreads, smem, st>>>(cs, plan, rows, upr, cols, static_cast<const T*>(dy), lddy,
-                                                            partials, err);
+  const bool vec = aligned16(dy) && lddy * sizeof(T) % 16 == 0;
+  embed_gategrad_kernel<T><<<*blocks, kThreads, smem, st>>>(cs, plan, static_cast<int>(rows), upr, cols,
+                                                            static_cast<const T*>(dy), lddy, vec, partials, err);
   VQ_CUDA(cudaGetLastError());
   return 0;
 }
@@ -1483,15 +1498,16 @@ int vq_embed_mix(int K, const int* types, const void* const* blocks, const float
   int* err = nullptr;
   if (int rc = device_error_ptr(&err)) return rc;
   using namespace vq::embed;
-  const int smem = kWarps * kStages * warp_bytes(cs);
+  const int smem = kWarps * warp_bytes(cs);
   const int upr = static_cast<int>(padded_cols / 256);
   auto kern = plan != nullptr ? embed_mix_kernel<true> : embed_mix_kernel<false>;
   int grid = 0;
   if (int rc = one_wave(kern, smem, T * upr, &grid)) return rc;
   const Plan pl = plan != nullptr ? plan_at(const_cast<void*>(plan), PlanLayout(T)) : Plan{};
   kern<<<grid, kThreads, smem, static_cast<cudaStream_t>(stream)>>>(
-      cs, probs, Ids{ids, ids_i32 != 0}, T, pl, vocab_start, rows, upr, static_cast<int>(cols), scale, strict != 0,
-      static_cast<__nv_bfloat16*>(out), ldo, err);
+      cs, probs, Ids{ids, ids_i32 != 0}, static_cast<int>(T), pl, vocab_start, static_cast<int>(rows), upr,
+      static_cast<int>(cols), scale, strict != 0, aligned16(out) && ldo % 8 == 0, static_cast<__nv_bfloat16*>(out), ldo,
+      err);
   VQ_CUDA(cudaGetLastError());
   return 0;
 }
