@@ -355,7 +355,7 @@ int vq_qk_norm_rope_bwd(const void* gq, const int64_t* gq_strides, const void* g
 /* ---- gated embedding ----
  * Plan of T token ids (int64, or int32 when ids_i32) over a table of `rows` rows that holds the vocabulary from
  * vocab_start on: the tokens in the order of their rows (stable; ids outside the table last), cut into pieces of equal
- * rows and at most 16 tokens.  `plan` (vq_embed_plan_bytes(T), 16-byte aligned) holds int32: the number of pieces P
+ * rows and at most 8 tokens (one begins at every 1024th place).  `plan` (vq_embed_plan_bytes(T), 16-byte aligned) holds int32: the number of pieces P
  * at byte 0; order[T] from byte 256; then, each from a multiple of 256 bytes, start[P] with T behind the last, and
  * the pieces' rows key[P] (`rows` for ids outside the table). */
 size_t vq_embed_plan_bytes(int64_t T);

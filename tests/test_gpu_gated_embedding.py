@@ -112,7 +112,8 @@ def test_lookup_and_gradient_against_64_bits(cuda, T, V, D, types, scale, start,
     assert _C.device_error() == 0
 
 
-@pytest.mark.parametrize("T,rows", [(1, 1), (5, 3), (1024, 511), (1025, 512), (4097, 70000), (20000, 200), (70001, 151936)])
+@pytest.mark.parametrize("T,rows", [(1, 1), (5, 3), (1024, 511), (1025, 512), (4097, 70000), (16384, 151936), (20000, 200),
+                                    (70001, 151936)])
 def test_plan_is_a_stable_sort_in_pieces(cuda, T, rows):
     from voodoo_quant import _C
 
@@ -124,8 +125,9 @@ def test_plan_is_a_stable_sort_in_pieces(cuda, T, rows):
     want, order = torch.sort(keys, stable=True)
     head = torch.ones(T, dtype=torch.bool)
     head[1:] = want[1:] != want[:-1]
-    head |= torch.arange(T) % 16 == 0
-    at = head.nonzero()[:, 0]
+    head |= torch.arange(T) % 1024 == 0
+    begin = torch.where(head, torch.arange(T), torch.zeros(T, dtype=torch.long)).cummax(0).values
+    at = ((torch.arange(T) - begin) % 8 == 0).nonzero()[:, 0]
     step = (4 * T + 255) // 256 * 64
     for dt in (torch.int64, torch.int32):
         plan = _C.embed_plan(ids.to(dt).to(cuda), rows, start).view(torch.int32).cpu().long()

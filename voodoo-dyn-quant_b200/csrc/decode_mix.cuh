@@ -129,10 +129,39 @@ struct URef {
   }
   __device__ __forceinline__ uint32_t b16(int off) const { return w(off) & 0xFFFFu; }
   __device__ __forceinline__ uint32_t b8(int off) const { return w(off) & 0xFFu; }
+  // eight words from wq(i) on
+  __device__ __forceinline__ void wq8(int i, int extra, uint32_t (&q)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = wq(i + j, extra);
+  }
+};
+
+// The same of a unit that starts at a word (kVec: at a 16-byte vector) of
+// shared memory: no joining of words, and runs of words read as vectors.  The
+// bits that `extra` shifts in from the next word are zeros here; every field
+// is masked out of them.
+template <bool kVec>
+struct URefAligned {
+  const uint32_t* s;
+  __device__ __forceinline__ uint32_t wq(int i, int extra = 0) const { return s[i] >> extra; }
+  __device__ __forceinline__ uint32_t b16(int off) const { return (s[off >> 2] >> (8 * (off & 3))) & 0xFFFFu; }
+  __device__ __forceinline__ uint32_t b8(int off) const { return (s[off >> 2] >> (8 * (off & 3))) & 0xFFu; }
+  __device__ __forceinline__ void wq8(int i, int extra, uint32_t (&q)[8]) const {
+    if (kVec) {
+      const uint4 a = *reinterpret_cast<const uint4*>(s + i), b = *reinterpret_cast<const uint4*>(s + i + 4);
+      const uint32_t v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) q[j] = v[j] >> extra;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) q[j] = s[i + j] >> extra;
+    }
+  }
 };
 
 // Scale and min of K-quant sub-block j from the 12-byte table at unit byte 4.
-__device__ __forceinline__ void k4_scale_min_u(const URef& u, int j, uint32_t& sc, uint32_t& mn) {
+template <class U>
+__device__ __forceinline__ void k4_scale_min_u(const U& u, int j, uint32_t& sc, uint32_t& mn) {
   if (j < 4) {
     sc = u.b8(4 + j) & 63u;
     mn = u.b8(8 + j) & 63u;
@@ -169,14 +198,16 @@ template <>
 struct MixChunk<kQ4_K> {
   static constexpr bool kMin = true;
   static constexpr float kSub = 8388608.0f;
-  __device__ __forceinline__ static void get(const URef& u, int c, float (&a)[2], float (&b)[2], uint32_t (&qb)[8]) {
+  template <class U>
+  __device__ __forceinline__ static void get(const U& u, int c, float (&a)[2], float (&b)[2], uint32_t (&qb)[8]) {
     const uint32_t w0 = u.wq(0);
     uint32_t sc, mn;
     k4_scale_min_u(u, c, sc, mn);
     a[0] = a[1] = __fmul_rn(h2f(w0), u2f(sc));
     b[0] = b[1] = -__fmul_rn(h2f(w0 >> 16), u2f(mn));
+    u.wq8(4 + 8 * (c >> 1), 4 * (c & 1), qb);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) qb[j] = u.wq(4 + 8 * (c >> 1) + j, 4 * (c & 1)) & 0x0F0F0F0Fu;
+    for (int j = 0; j < 8; ++j) qb[j] &= 0x0F0F0F0Fu;
   }
 };
 
@@ -184,15 +215,18 @@ template <>
 struct MixChunk<kQ5_K> {
   static constexpr bool kMin = true;
   static constexpr float kSub = 8388608.0f;
-  __device__ __forceinline__ static void get(const URef& u, int c, float (&a)[2], float (&b)[2], uint32_t (&qb)[8]) {
+  template <class U>
+  __device__ __forceinline__ static void get(const U& u, int c, float (&a)[2], float (&b)[2], uint32_t (&qb)[8]) {
     const uint32_t w0 = u.wq(0);
     uint32_t sc, mn;
     k4_scale_min_u(u, c, sc, mn);
     a[0] = a[1] = __fmul_rn(h2f(w0), u2f(sc));
     b[0] = b[1] = -__fmul_rn(h2f(w0 >> 16), u2f(mn));
+    uint32_t high[8];
+    u.wq8(12 + 8 * (c >> 1), 4 * (c & 1), qb);
+    u.wq8(4, c, high);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      qb[j] = (u.wq(12 + 8 * (c >> 1) + j, 4 * (c & 1)) & 0x0F0F0F0Fu) | ((u.wq(4 + j, c) & 0x01010101u) << 4);
+    for (int j = 0; j < 8; ++j) qb[j] = (qb[j] & 0x0F0F0F0Fu) | ((high[j] & 0x01010101u) << 4);
   }
 };
 
@@ -220,7 +254,8 @@ template <>
 struct MixChunk<kQ2_K> {
   static constexpr bool kMin = true;
   static constexpr float kSub = 8388608.0f;
-  __device__ __forceinline__ static void get(const URef& u, int c, float (&a)[2], float (&b)[2], uint32_t (&qb)[8]) {
+  template <class U>
+  __device__ __forceinline__ static void get(const U& u, int c, float (&a)[2], float (&b)[2], uint32_t (&qb)[8]) {
     const int h = c >> 2, sft = c & 3;
     const uint32_t sw = u.b16(2 * c);  // scale bytes 2c, 2c+1
     const uint32_t wd = u.wq(20);
@@ -229,8 +264,9 @@ struct MixChunk<kQ2_K> {
     b[0] = -__fmul_rn(dmin, u2f((sw >> 4) & 15u));
     a[1] = __fmul_rn(d, u2f((sw >> 8) & 15u));
     b[1] = -__fmul_rn(dmin, u2f((sw >> 12) & 15u));
+    u.wq8(4 + 8 * h, 2 * sft, qb);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) qb[j] = u.wq(4 + 8 * h + j, 2 * sft) & 0x03030303u;
+    for (int j = 0; j < 8; ++j) qb[j] &= 0x03030303u;
   }
 };
 
@@ -259,7 +295,8 @@ template <>
 struct MixChunk<kIQ4_XS> {
   static constexpr bool kMin = false;
   static constexpr float kSub = 8388736.0f;  // 2^23 + 128
-  __device__ __forceinline__ static void get(const URef& u, int c, float (&a)[2], float (&b)[2], uint32_t (&qb)[8]) {
+  template <class U>
+  __device__ __forceinline__ static void get(const U& u, int c, float (&a)[2], float (&b)[2], uint32_t (&qb)[8]) {
     const uint32_t w0 = u.wq(0);
     const uint32_t ls = ((u.b8(4 + (c >> 1)) >> (4 * (c & 1))) & 15u) | ((((w0 >> 16) >> (2 * c)) & 3u) << 4);
     a[0] = a[1] = __fmul_rn(h2f(w0), u2f(ls) - 32.0f);

@@ -72,12 +72,52 @@ __device__ __forceinline__ void stage_unit(const CandSet& cs, uint32_t buf, int 
   }
 }
 
-// The staged unit of candidate k, whose slots start at `region`; `unit` modulo 2^32.
-__device__ __forceinline__ URef staged(const CandSet& cs, const uint8_t* region, int k, int lu, uint32_t unit) {
+// How a candidate's units are decoded: its format, and whether they start at
+// words or 16-byte vectors, so that its fields can be read whole.  Dense
+// numbers, for a jump table.
+enum Decode : int { kDQ8, kDQ3, kDQ6, kDQ2, kDIQ4, kDQ4, kDQ5, kDQ2Words, kDIQ4Words, kDQ4Vectors, kDQ5Vectors };
+
+inline int decode_code(int fmt, const uint8_t* p) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+  switch (fmt) {
+    case kQ8_0: return kDQ8;
+    case kQ3_K: return kDQ3;
+    case kQ6_K: return kDQ6;
+    case kQ2_K: return a % 4 == 0 ? kDQ2Words : kDQ2;      // 84 bytes a unit
+    case kIQ4_XS: return a % 4 == 0 ? kDIQ4Words : kDIQ4;  // 136
+    case kQ4_K: return a % 16 == 0 ? kDQ4Vectors : kDQ4;   // 144
+    default: return a % 16 == 0 ? kDQ5Vectors : kDQ5;      // Q5_K: 176
+  }
+}
+
+template <int F>
+using Format = std::integral_constant<int, F>;
+
+// Calls op(format, unit) for the staged unit of candidate k (whose cs.fmt is
+// its decode_code), whose slots start at `region`; `unit` counts modulo 2^32.
+template <class Op>
+__device__ __forceinline__ void with_unit(const CandSet& cs, const uint8_t* region, int k, int lu, uint32_t unit,
+                                          const Op& op) {
   const int ub = cs.ubytes[k];
   const uint32_t rel = (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(cs.ptr[k])) + unit * ub) & 15u;
-  return URef{reinterpret_cast<const uint32_t*>(region + lu * slot_bytes(ub) + (rel & ~3u)), static_cast<int>(rel & 3u),
-              8u * (rel & 3u)};
+  const uint32_t* s = reinterpret_cast<const uint32_t*>(region + lu * slot_bytes(ub) + (rel & ~3u));
+  const URef any{s, static_cast<int>(rel & 3u), 8u * (rel & 3u)};
+  const URefAligned<false> words{s};
+  const URefAligned<true> vectors{s};
+  switch (cs.fmt[k]) {
+    case kDQ8: op(Format<kQ8_0>{}, any); break;
+    case kDQ3: op(Format<kQ3_K>{}, any); break;
+    case kDQ6: op(Format<kQ6_K>{}, any); break;
+    case kDQ2: op(Format<kQ2_K>{}, any); break;
+    case kDIQ4: op(Format<kIQ4_XS>{}, any); break;
+    case kDQ4: op(Format<kQ4_K>{}, any); break;
+    case kDQ5: op(Format<kQ5_K>{}, any); break;
+    case kDQ2Words: op(Format<kQ2_K>{}, words); break;
+    case kDIQ4Words: op(Format<kIQ4_XS>{}, words); break;
+    case kDQ4Vectors: op(Format<kQ4_K>{}, vectors); break;
+    case kDQ5Vectors: op(Format<kQ5_K>{}, vectors); break;
+    default: break;
+  }
 }
 
 struct Ids {
@@ -95,15 +135,20 @@ __device__ __forceinline__ long long local_row(long long id, long long vocab_sta
 }
 
 // The tokens of a call in the order of their rows, cut into pieces of equal
-// rows (token_plan_kernel): piece i holds the tokens order[start[i]] to
-// order[start[i + 1] - 1], all naming row key[i].
+// rows: piece i holds the tokens order[start[i]] to order[start[i + 1] - 1],
+// all naming row key[i].  A piece begins where a row does, at every 1024th
+// place of the order (a tile of the sort, which then needs no carry from the
+// one before) and kPieceTokens after the piece before it.
 struct Plan {
   int *order, *start, *key, *count;
 };
 
 // Most tokens of a piece: a token that fills much of a batch is then worked
-// on by many warps, each decoding its row again.
-constexpr int kPieceTokens = 16;
+// on by many warps, each decoding its row again.  8 is what a unit's lanes
+// read in one load; 16 and 32 decode less (16384 tokens of text: 6300 and
+// 5800 pieces, not 7300) but measured 91 and 95 us for the lookup against 88,
+// the warps that got the long pieces ending last.
+constexpr int kPieceTokens = 8;
 
 // The units that eight lanes work on one after the other: unit u of piece
 // (kRuns) or token i, i * units_per_row + u ascending by a fixed stride.
@@ -131,16 +176,55 @@ struct UnitWalk {
       ++i;
     }
   }
-  // Row of the table, or -1 for a token of another one.
-  __device__ __forceinline__ int row() const {
-    if (!on()) return -1;
-    if (!kRuns) return static_cast<int>(local_row(ids.at(i), vocab_start, rows));
-    const int key = plan.key[i];
-    return key < rows ? key : -1;
+  // Row of the table (-1: a token of another one), unit, and the tokens: places in the order from begin to end.
+  struct At {
+    int row, u, begin, end;
+  };
+  __device__ __forceinline__ At get() const {
+    At a{-1, u, 0, 0};
+    if (!on()) return a;
+    if (kRuns) {
+      const int key = plan.key[i];
+      a.begin = plan.start[i];
+      a.end = plan.start[i + 1];
+      a.row = key < rows ? key : -1;
+    } else {
+      a.row = static_cast<int>(local_row(ids.at(i), vocab_start, rows));
+      a.begin = i;
+      a.end = i + 1;
+    }
+    return a;
   }
 };
 
 // ---------------------------------------------------------------- lookup
+// mix_chunk's arithmetic, one value an instruction: pairs (f32x2) cost more
+// moves into aligned registers here than they save (DECIDE).
+template <int F, class U>
+__device__ __forceinline__ void mix_unit(const U& u, int c, float pk, float (&acc)[32], float (&cst)[2]) {
+  float a[2], b[2];
+  uint32_t qb[8];
+  MixChunk<F>::get(u, c, a, b, qb);
+  const float pa[2] = {pk * a[0], pk * a[1]};
+  if (MixChunk<F>::kMin) {
+    cst[0] = fmaf(pk, b[0], cst[0]);
+    cst[1] = fmaf(pk, b[1], cst[1]);
+  }
+#ifdef VQ_SCALAR
+#pragma unroll
+  for (int j = 0; j < 32; ++j)
+    acc[j] = fmaf(pa[j >> 4], magic_byte(qb[j >> 2], j & 3) - MixChunk<F>::kSub, acc[j]);
+#else
+  const float2 nsub = make_float2(-MixChunk<F>::kSub, -MixChunk<F>::kSub);
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const float2 q = __fadd2_rn(make_float2(magic_byte(qb[j >> 1], 2 * (j & 1)), magic_byte(qb[j >> 1], 2 * (j & 1) + 1)), nsub);
+    const float2 r = __ffma2_rn(make_float2(pa[j >> 3], pa[j >> 3]), q, make_float2(acc[2 * j], acc[2 * j + 1]));
+    acc[2 * j] = r.x, acc[2 * j + 1] = r.y;
+  }
+#endif
+}
+
 // Rows of ids outside [vocab_start, vocab_start + rows) are written as zeros
 // (another shard's tokens); `strict` also reports them.  The mixture is
 // mix_units_kernel's, in the same order, so for scale 1 the rows are those of
@@ -162,78 +246,72 @@ __global__ void __launch_bounds__(kThreads, kMixBlocks)
   UnitWalk<kRuns> w{plan, ids, kRuns ? *plan.count : T, vocab_start, rows, units_per_row};
   w.start_at((static_cast<long long>(blockIdx.x) * kWarps + warp) * kUnits + lu,
              static_cast<long long>(gridDim.x) * kWarps * kUnits);
-  bool bad = false, fmt_ok = true;
-  for (; __any_sync(0xffffffffu, w.on()); w.step()) {
-    const int row = w.row();
-    const long long unit = static_cast<long long>(row) * units_per_row + w.u;
-    if (row >= 0) stage_unit(cs, smem_u32(buf), lu, c, unit);
+  bool bad = false;
+  const bool scaled = scale != 1.f;
+  for (;; w.step()) {
+    const auto now = w.get();
+    if (!__any_sync(0xffffffffu, now.begin < now.end)) break;
+    const long long unit = static_cast<long long>(now.row) * units_per_row + now.u;
+    if (now.row >= 0) stage_unit(cs, smem_u32(buf), lu, c, unit);
     async_commit();
-    float2 acc[16];
+    const int len = now.end - now.begin;
+    // lane c holds the unit's c-th token
+    const int mine = kRuns ? (c < len ? plan.order[now.begin + c] : 0) : now.begin;
+    float acc[32];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) acc[j] = make_float2(0.f, 0.f);
+    for (int j = 0; j < 32; ++j) acc[j] = 0.f;
     float cst[2] = {0.f, 0.f};
-    const int col = 256 * w.u + 32 * c;
+    const int col = 256 * now.u + 32 * c;
     async_wait<0>();
     __syncwarp();
-    if (row >= 0 && col < cols) {
+    if (now.row >= 0 && col < cols) {
       const uint8_t* region = buf;
       for (int k = 0; k < cs.K; ++k) {
-        const URef ur = staged(cs, region, k, lu, static_cast<uint32_t>(unit));
         const float pk = pk_s[k];
-        switch (cs.fmt[k]) {
-          case kQ8_0: mix_chunk<kQ8_0>(ur, c, pk, acc, cst); break;
-          case kQ2_K: mix_chunk<kQ2_K>(ur, c, pk, acc, cst); break;
-          case kQ3_K: mix_chunk<kQ3_K>(ur, c, pk, acc, cst); break;
-          case kQ4_K: mix_chunk<kQ4_K>(ur, c, pk, acc, cst); break;
-          case kQ5_K: mix_chunk<kQ5_K>(ur, c, pk, acc, cst); break;
-          case kQ6_K: mix_chunk<kQ6_K>(ur, c, pk, acc, cst); break;
-          case kIQ4_XS: mix_chunk<kIQ4_XS>(ur, c, pk, acc, cst); break;
-          default: fmt_ok = false;
-        }
+        with_unit(cs, region, k, lu, static_cast<uint32_t>(unit), [&](auto f, const auto& u) {
+          mix_unit<decltype(f)::value>(u, c, pk, acc, cst);
+        });
         region += kUnits * slot_bytes(cs.ubytes[k]);
       }
     }
-    if (w.on()) {
-      bad |= row < 0;
-      if (col < cols) {
-        __align__(16) __nv_bfloat162 hv[16];
+    bad |= now.row < 0 && len > 0;
+    __align__(16) __nv_bfloat162 hv[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float cs0 = cst[j >> 3];
+      const float x = acc[2 * j] + cs0, y = acc[2 * j + 1] + cs0;
+      hv[j] = scaled ? __floats2bfloat162_rn(x * scale, y * scale) : __floats2bfloat162_rn(x, y);
+    }
+    const int most = kRuns ? __reduce_max_sync(0xffffffffu, len) : 1;
+    for (int i = 0; i < most; ++i) {
+      const int tok = kRuns ? __shfl_sync(0xffffffffu, mine, (lane & 24) + i) : mine;
+      if (i >= len || col >= cols) continue;
+      __nv_bfloat16* dst = out + static_cast<long long>(tok) * ldo + col;
+      if (vec && col + 32 <= cols) {
+#pragma unroll
+        for (int v = 0; v < 4; ++v) reinterpret_cast<uint4*>(dst)[v] = reinterpret_cast<const uint4*>(hv)[v];
+      } else {
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          const float cs0 = cst[j >> 3];
-          hv[j] = __floats2bfloat162_rn((acc[j].x + cs0) * scale, (acc[j].y + cs0) * scale);
-        }
-        const int begin = kRuns ? plan.start[w.i] : w.i, end = kRuns ? plan.start[w.i + 1] : w.i + 1;
-        for (int i = begin; i < end; ++i) {
-          __nv_bfloat16* dst = out + static_cast<long long>(kRuns ? plan.order[i] : i) * ldo + col;
-          if (vec && col + 32 <= cols) {
-#pragma unroll
-            for (int v = 0; v < 4; ++v) reinterpret_cast<uint4*>(dst)[v] = reinterpret_cast<const uint4*>(hv)[v];
-          } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              if (col + 2 * j < cols) dst[2 * j] = hv[j].x;
-              if (col + 2 * j + 1 < cols) dst[2 * j + 1] = hv[j].y;
-            }
-          }
+          if (col + 2 * j < cols) dst[2 * j] = hv[j].x;
+          if (col + 2 * j + 1 < cols) dst[2 * j + 1] = hv[j].y;
         }
       }
     }
     __syncwarp();  // the slots are filled again
   }
   if (bad && strict) report_error(err, kDevBadIndex, 30);
-  if (!fmt_ok) report_error(err, kDevBadFormat, 3);
 }
 
 // ---------------------------------------------------------------- plan
-// Stable radix sort of the tokens' local rows by one cluster, nine bits a
-// pass, and the pieces of equal rows.  Tokens of other shards get the key
-// `rows` and so end up last.  Each CTA owns a contiguous slice of a pass's
-// input and ranks it a tile of 1024 tokens at a time: within a warp by
-// matching digits, over the warps and tiles by counts; the slices' counts
-// meet through distributed shared memory.  Latency bound: a dozen barriers
-// and the round trips between them.
+// Stable radix sort of the tokens' local rows, nine bits a pass, and the
+// pieces.  Tokens of other shards get the key `rows` and so end up last.
+// Latency bound: barriers and the round trips between them.
 constexpr int kSortThreads = 1024;
-constexpr int kSortCtas = 8;  // largest portable cluster
+#ifndef VQ_CTAS
+#define VQ_CTAS 16
+#endif
+constexpr int kSortCtas = VQ_CTAS;  // the largest cluster (8 is the portable limit)
 constexpr int kDigitBits = 9;
 constexpr int kBins = 1 << kDigitBits;
 constexpr int kSortSmem = 32 * kBins * 2;
@@ -241,10 +319,156 @@ constexpr int kKeepTiles = 2;  // tiles whose keys and ranks stay in registers b
 
 __device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
   int v;
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr));
   return v;
 }
 
+// Exclusive scan over the digits of a block (thread d < kBins holds digit d's
+// total; wsum: 32 ints of scratch).  One barrier inside.
+__device__ __forceinline__ int digit_scan(int total, int* wsum) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int x = total;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) wsum[warp] = x;
+  __syncthreads();
+  int ahead = 0;
+#pragma unroll
+  for (int w = 0; w < kBins / 32; ++w) ahead += w < warp ? wsum[w] : 0;
+  return ahead + x - total;
+}
+
+// Turns each digit's counts by warp into the sums over the warps before, and
+// returns the digit's total (threads < kBins).
+__device__ __forceinline__ int warp_prefix(uint16_t* wcount) {
+  int run = 0;
+  if (threadIdx.x < kBins) {
+#pragma unroll 16
+    for (int w = 0; w < 32; ++w) {
+      const int n = wcount[w * kBins + threadIdx.x];
+      wcount[w * kBins + threadIdx.x] = static_cast<uint16_t>(run);
+      run += n;
+    }
+  }
+  return run;
+}
+
+// Up to 1024 * kItems tokens: one block sorts in shared memory, a warp holding
+// 32 * kItems consecutive places, without the cluster's barriers.
+template <int kItems>
+__global__ void __launch_bounds__(kSortThreads) token_plan_block_kernel(Ids ids, int T, long long vocab_start, int rows,
+                                                                        int passes, Plan plan) {
+  extern __shared__ __align__(16) uint8_t ssmem[];
+  uint16_t* wcount = reinterpret_cast<uint16_t*>(ssmem);              // [32 warps][kBins]
+  int* skey = reinterpret_cast<int*>(ssmem + kSortSmem);              // [1024 * kItems]
+  uint16_t* sidx = reinterpret_cast<uint16_t*>(skey + kSortThreads * kItems);
+  __shared__ int base[kBins];
+  __shared__ int wsum[32];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int first = warp * 32 * kItems + lane;  // this lane's places: first + 32 r
+  int key[kItems], idx[kItems], rank[kItems];
+#pragma unroll
+  for (int r = 0; r < kItems; ++r) {
+    const int i = first + 32 * r;
+    idx[r] = i;
+    const long long row = i < T ? local_row(ids.at(i), vocab_start, rows) : -1;
+    // places past the end sort behind everything (the sort is stable)
+    key[r] = i >= T ? (1 << (kDigitBits * passes)) - 1 : row < 0 ? rows : static_cast<int>(row);
+  }
+  for (int p = 0; p < passes; ++p) {
+    const int shift = p * kDigitBits;
+    uint4* z = reinterpret_cast<uint4*>(wcount);
+    for (int v = tid; v < kSortSmem / 16; v += kSortThreads) z[v] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    uint16_t* mine = wcount + warp * kBins;
+#pragma unroll
+    for (int r = 0; r < kItems; ++r) {
+      const int d = (key[r] >> shift) & (kBins - 1);
+      const uint32_t same = __match_any_sync(0xffffffffu, d);
+      const int before = mine[d];
+      __syncwarp();
+      const int ahead = __popc(same & ((1u << lane) - 1u));
+      if (ahead == 0) mine[d] = static_cast<uint16_t>(before + __popc(same));
+      __syncwarp();
+      rank[r] = before + ahead;
+    }
+    __syncthreads();
+    const int total = warp_prefix(wcount);
+    const int at0 = digit_scan(total, wsum);
+    if (tid < kBins) base[tid] = at0;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kItems; ++r) {
+      const int d = (key[r] >> shift) & (kBins - 1);
+      const int at = base[d] + mine[d] + rank[r];
+      skey[at] = key[r];
+      sidx[at] = static_cast<uint16_t>(idx[r]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kItems; ++r) {
+      key[r] = skey[first + 32 * r];
+      idx[r] = sidx[first + 32 * r];
+    }
+  }
+  // pieces: the last place before each warp's where a row or a tile begins ...
+  uint32_t heads[kItems];
+  int last = -1;
+#pragma unroll
+  for (int r = 0; r < kItems; ++r) {
+    const int i = first + 32 * r;
+    if (i < T) plan.order[i] = idx[r];
+    heads[r] = __ballot_sync(0xffffffffu, i % kSortThreads == 0 || skey[i] != skey[i - 1]);
+    if (heads[r]) last = i - lane + 31 - __clz(heads[r]);
+  }
+  if (lane == 0) wsum[warp] = last;
+  __syncthreads();
+  int from = -1;
+#pragma unroll
+  for (int w = 0; w < 32; ++w) from = w < warp ? max(from, wsum[w]) : from;
+  // ... every kPieceTokens places from which a piece begins
+  uint32_t starts[kItems];
+  int n = 0;
+#pragma unroll
+  for (int r = 0; r < kItems; ++r) {
+    const int i = first + 32 * r;
+    const uint32_t upto = heads[r] & (0xffffffffu >> (31 - lane));
+    const int begin = upto ? i - lane + 31 - __clz(upto) : from;
+    starts[r] = __ballot_sync(0xffffffffu, i < T && (i - begin) % kPieceTokens == 0);
+    n += __popc(starts[r]);
+    if (heads[r]) from = i - lane + 31 - __clz(heads[r]);
+  }
+  __syncthreads();
+  if (lane == 0) wsum[warp] = n;
+  __syncthreads();
+  int at = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < 32; ++w) {
+    at += w < warp ? wsum[w] : 0;
+    all += wsum[w];
+  }
+#pragma unroll
+  for (int r = 0; r < kItems; ++r) {
+    if ((starts[r] >> lane) & 1u) {
+      const int q = at + __popc(starts[r] & ((1u << lane) - 1u));
+      plan.start[q] = first + 32 * r;
+      plan.key[q] = key[r];
+    }
+    at += __popc(starts[r]);
+  }
+  if (tid == 0) {
+    plan.start[all] = T;
+    *plan.count = all;
+  }
+}
+
+// More tokens: one cluster.  Each CTA owns a contiguous slice (of whole
+// tiles) of a pass's input and ranks it a tile of 1024 tokens at a time:
+// within a warp by matching digits, over the warps and tiles by counts; the
+// slices' counts meet through distributed shared memory.
 __global__ void __launch_bounds__(kSortThreads) token_plan_kernel(Ids ids, int T, long long vocab_start, int rows,
                                                                   int passes, Plan plan, int* keys, int* keys_tmp,
                                                                   int* order_tmp) {
@@ -260,7 +484,8 @@ __global__ void __launch_bounds__(kSortThreads) token_plan_kernel(Ids ids, int T
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(nctas));
   const int rank = static_cast<int>(cluster_ctarank());
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int slice = (T + static_cast<int>(nctas) - 1) / static_cast<int>(nctas);
+  const int tiles = (T + kSortThreads - 1) / kSortThreads;
+  const int slice = (tiles + static_cast<int>(nctas) - 1) / static_cast<int>(nctas) * kSortThreads;
   const int b = min(T, rank * slice), e = min(T, b + slice);
   for (int p = 0; p < passes; ++p) {
     const bool to_tmp = ((passes - 1 - p) & 1) != 0;
@@ -285,15 +510,7 @@ __global__ void __launch_bounds__(kSortThreads) token_plan_kernel(Ids ids, int T
       const int ahead = __popc(same & ((1u << lane) - 1u));
       if (in && ahead == 0) wcount[warp * kBins + d] = static_cast<uint16_t>(__popc(same));
       __syncthreads();
-      int run = 0;
-      if (tid < kBins) {
-#pragma unroll 8
-        for (int w = 0; w < 32; ++w) {
-          const int n = wcount[w * kBins + tid];
-          wcount[w * kBins + tid] = static_cast<uint16_t>(run);
-          run += n;
-        }
-      }
+      const int run = warp_prefix(wcount);
       __syncthreads();
       const int r = in ? count[d] + wcount[warp * kBins + d] + ahead : 0;
       __syncthreads();
@@ -319,25 +536,15 @@ __global__ void __launch_bounds__(kSortThreads) token_plan_kernel(Ids ids, int T
     // first place of each digit of this slice: smaller digits, then the same digit in earlier slices
     int total = 0, before = 0;
     if (tid < kBins) {
-      for (int r = 0; r < static_cast<int>(nctas); ++r) {
-        const int h = ld_cluster_s32(map_to_rank(smem_u32(&count[tid]), r));
+#pragma unroll
+      for (int r = 0; r < kSortCtas; ++r) {  // in flight together
+        const int h = r < static_cast<int>(nctas) ? ld_cluster_s32(map_to_rank(smem_u32(&count[tid]), r)) : 0;
         before += r < rank ? h : 0;
         total += h;
       }
     }
-    int x = total;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    if (lane == 31) wsum[warp] = x;
-    __syncthreads();
-    if (tid < kBins) {
-      int ahead = 0;
-      for (int w = 0; w < warp; ++w) ahead += wsum[w];
-      base[tid] = ahead + x - total + before;
-    }
+    const int at0 = digit_scan(total, wsum);
+    if (tid < kBins) base[tid] = at0 + before;
     __syncthreads();
 #pragma unroll
     for (int t = 0; t < kKeepTiles; ++t) {
@@ -356,38 +563,65 @@ __global__ void __launch_bounds__(kSortThreads) token_plan_kernel(Ids ids, int T
     }
     cluster_sync();  // this pass's keys are written, and nobody reads the counts any more
   }
-  // pieces: where a row begins, and every kPieceTokens-th place of the order
-  auto begins = [&](int i) -> bool {
-    return i < e && (i % kPieceTokens == 0 || __ldcg(keys + i) != __ldcg(keys + i - 1));
+  // pieces, a tile at a time; first their number
+  auto starts_of = [&](int i) -> uint32_t {
+    const bool in = i < e;
+    const uint32_t heads =
+        __ballot_sync(0xffffffffu, in && (i % kSortThreads == 0 || __ldcg(keys + i) != __ldcg(keys + i - 1)));
+    if (lane == 0) wsum[warp] = heads ? i + 31 - __clz(heads) : -1;
+    __syncthreads();
+    int from = -1;
+#pragma unroll
+    for (int w = 0; w < 32; ++w) from = w < warp ? max(from, wsum[w]) : from;
+    __syncthreads();
+    const uint32_t upto = heads & (0xffffffffu >> (31 - lane));
+    const int begin = upto ? i - lane + 31 - __clz(upto) : from;
+    return __ballot_sync(0xffffffffu, in && (i - begin) % kPieceTokens == 0);
   };
   int mine = 0;
-  for (int i0 = b; i0 < e; i0 += kSortThreads) mine += __syncthreads_count(begins(i0 + tid));
-  if (tid == 0) pieces = mine;
+  uint32_t kept[kKeepTiles];
+#pragma unroll
+  for (int t = 0; t < kKeepTiles; ++t) {
+    kept[t] = b + t * kSortThreads < e ? starts_of(b + t * kSortThreads + tid) : 0;
+    mine += __popc(kept[t]);
+  }
+  for (int i0 = b + kKeepTiles * kSortThreads; i0 < e; i0 += kSortThreads) mine += __popc(starts_of(i0 + tid));
+  __syncthreads();
+  if (lane == 0) wsum[warp] = mine;
+  __syncthreads();
+  if (tid == 0) {
+    int n = 0;
+    for (int w = 0; w < 32; ++w) n += wsum[w];
+    pieces = n;
+  }
   cluster_sync();
   int at = 0, all = 0;
-  for (int r = 0; r < static_cast<int>(nctas); ++r) {
-    const int n = ld_cluster_s32(map_to_rank(smem_u32(&pieces), r));
+#pragma unroll
+  for (int r = 0; r < kSortCtas; ++r) {
+    const int n = r < static_cast<int>(nctas) ? ld_cluster_s32(map_to_rank(smem_u32(&pieces), r)) : 0;
     at += r < rank ? n : 0;
     all += n;
   }
-  for (int i0 = b; i0 < e; i0 += kSortThreads) {
-    const int i = i0 + tid;
-    const bool f = begins(i);
-    const uint32_t m = __ballot_sync(0xffffffffu, f);
+  auto write_starts = [&](int i, uint32_t m) {
     if (lane == 0) wsum[warp] = __popc(m);
     __syncthreads();
     int ahead = __popc(m & ((1u << lane) - 1u)), sum = 0;
+#pragma unroll
     for (int w = 0; w < 32; ++w) {
       ahead += w < warp ? wsum[w] : 0;
       sum += wsum[w];
     }
-    if (f) {
+    if ((m >> lane) & 1u) {
       plan.start[at + ahead] = i;
       plan.key[at + ahead] = __ldcg(keys + i);
     }
     at += sum;
     __syncthreads();
-  }
+  };
+#pragma unroll
+  for (int t = 0; t < kKeepTiles; ++t)
+    if (b + t * kSortThreads < e) write_starts(b + t * kSortThreads + tid, kept[t]);
+  for (int i0 = b + kKeepTiles * kSortThreads; i0 < e; i0 += kSortThreads) write_starts(i0 + tid, starts_of(i0 + tid));
   if (rank == 0 && tid == 0) {
     plan.start[all] = T;
     *plan.count = all;
@@ -396,21 +630,30 @@ __global__ void __launch_bounds__(kSortThreads) token_plan_kernel(Ids ids, int T
 }
 
 // ---------------------------------------------------------------- gradient
-template <int F>
-__device__ __forceinline__ float dot_chunk(const URef& u, int c, const float2 (&g)[16], const float (&gs)[2]) {
+template <int F, class U>
+__device__ __forceinline__ float dot_unit(const U& u, int c, const float (&g)[32], const float (&gs)[2]) {
   float a[2], b[2];
   uint32_t qb[8];
   MixChunk<F>::get(u, c, a, b, qb);
-  const float2 nsub = make_float2(-MixChunk<F>::kSub, -MixChunk<F>::kSub);
-  float2 s[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+  float s[4] = {0.f, 0.f, 0.f, 0.f};  // two chains a half
+#ifdef VQ_SCALAR
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float2 q01 = __fadd2_rn(make_float2(magic_byte(qb[j], 0), magic_byte(qb[j], 1)), nsub);
-    const float2 q23 = __fadd2_rn(make_float2(magic_byte(qb[j], 2), magic_byte(qb[j], 3)), nsub);
-    s[j >> 2] = __ffma2_rn(g[2 * j], q01, s[j >> 2]);
-    s[j >> 2] = __ffma2_rn(g[2 * j + 1], q23, s[j >> 2]);
+  for (int j = 0; j < 32; ++j)
+    s[(j >> 4) * 2 + (j & 1)] = fmaf(g[j], magic_byte(qb[j >> 2], j & 3) - MixChunk<F>::kSub, s[(j >> 4) * 2 + (j & 1)]);
+#else
+  const float2 nsub = make_float2(-MixChunk<F>::kSub, -MixChunk<F>::kSub);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float2 t = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int j = 8 * h; j < 8 * h + 8; ++j) {
+      const float2 q = __fadd2_rn(make_float2(magic_byte(qb[j >> 1], 2 * (j & 1)), magic_byte(qb[j >> 1], 2 * (j & 1) + 1)), nsub);
+      t = __ffma2_rn(make_float2(g[2 * j], g[2 * j + 1]), q, t);
+    }
+    s[2 * h] = t.x, s[2 * h + 1] = t.y;
   }
-  float d = a[0] * (s[0].x + s[0].y) + a[1] * (s[1].x + s[1].y);
+#endif
+  float d = a[0] * (s[0] + s[1]) + a[1] * (s[2] + s[3]);
   if (MixChunk<F>::kMin) d = fmaf(b[0], gs[0], fmaf(b[1], gs[1], d));
   return d;
 }
@@ -418,7 +661,7 @@ __device__ __forceinline__ float dot_chunk(const URef& u, int c, const float2 (&
 // Adds 32 values of a row of dy at column col (zeros past cols); vec: the rows
 // are 16-byte aligned.
 template <typename T>
-__device__ __forceinline__ void add_row(const T* row, int col, int cols, bool vec, float2 (&g)[16]) {
+__device__ __forceinline__ void add_row(const T* row, int col, int cols, bool vec, float (&g)[32]) {
   constexpr int kPer = 16 / sizeof(T);
   if (vec && col + 32 <= cols) {
     uint4 v[32 / kPer];
@@ -430,26 +673,21 @@ __device__ __forceinline__ void add_row(const T* row, int col, int cols, bool ve
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if constexpr (sizeof(T) == 4) {
-          float2& d = g[2 * j + (i >> 1)];
-          (i & 1 ? d.y : d.x) += __uint_as_float(w[i]);
+          g[4 * j + i] += __uint_as_float(w[i]);
+        } else if constexpr (std::is_same<T, __half>::value) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+          g[8 * j + 2 * i] += f.x;
+          g[8 * j + 2 * i + 1] += f.y;
         } else {
-          const float2 f = [&] {
-            if constexpr (std::is_same<T, __half>::value)
-              return __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-            else
-              return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
-          }();
-          g[4 * j + i].x += f.x;
-          g[4 * j + i].y += f.y;
+          g[8 * j + 2 * i] += __uint_as_float(w[i] << 16);
+          g[8 * j + 2 * i + 1] += __uint_as_float(w[i] & 0xffff0000u);
         }
       }
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      if (col + 2 * j < cols) g[j].x += static_cast<float>(row[col + 2 * j]);
-      if (col + 2 * j + 1 < cols) g[j].y += static_cast<float>(row[col + 2 * j + 1]);
-    }
+    for (int j = 0; j < 32; ++j)
+      if (col + j < cols) g[j] += static_cast<float>(row[col + j]);
   }
 }
 
@@ -473,50 +711,42 @@ __global__ void __launch_bounds__(kThreads, kGradBlocks)
   UnitWalk<true> w{plan, Ids{nullptr, false}, *plan.count, 0, rows, units_per_row};
   w.start_at((static_cast<long long>(blockIdx.x) * kWarps + warp) * kUnits + lu,
              static_cast<long long>(gridDim.x) * kWarps * kUnits);
-  bool fmt_ok = true;
   for (;; w.step()) {
-    const int row = w.row();
-    if (!__any_sync(0xffffffffu, row >= 0)) break;  // other shards' pieces come last
-    const long long unit = static_cast<long long>(row) * units_per_row + w.u;
-    if (row >= 0) stage_unit(cs, smem_u32(buf), lu, c, unit);
+    const auto now = w.get();
+    if (!__any_sync(0xffffffffu, now.row >= 0)) break;  // other shards' pieces come last
+    const long long unit = static_cast<long long>(now.row) * units_per_row + now.u;
+    if (now.row >= 0) stage_unit(cs, smem_u32(buf), lu, c, unit);
     async_commit();
-    const int col = 256 * w.u + 32 * c;
-    const bool on = row >= 0 && col < cols;
-    float2 g[16];
+    const int col = 256 * now.u + 32 * c;
+    const bool on = now.row >= 0 && col < cols;
+    const int len = now.row >= 0 ? now.end - now.begin : 0;
+    const int mine = c < len ? plan.order[now.begin + c] : 0;  // lane c holds the unit's c-th token
+    float g[32];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) g[j] = make_float2(0.f, 0.f);
-    if (on) {
-      const int end = plan.start[w.i + 1];
-      for (int i = plan.start[w.i]; i < end; ++i)
-        add_row<T>(dy + static_cast<long long>(plan.order[i]) * lddy, col, cols, vec, g);
+    for (int j = 0; j < 32; ++j) g[j] = 0.f;
+    const int most = __reduce_max_sync(0xffffffffu, len);
+    for (int i = 0; i < most; ++i) {
+      const int tok = __shfl_sync(0xffffffffu, mine, (lane & 24) + i);
+      if (i < len && on) add_row<T>(dy + static_cast<long long>(tok) * lddy, col, cols, vec, g);
     }
     float gs[2] = {0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < 16; ++j) gs[j >> 3] += g[j].x + g[j].y;
+    for (int j = 0; j < 32; ++j) gs[j >> 4] += g[j];
     async_wait<0>();
     __syncwarp();
     if (on) {
       const uint8_t* region = buf;
       for (int k = 0; k < cs.K; ++k) {
-        const URef ur = staged(cs, region, k, lu, static_cast<uint32_t>(unit));
         float d = 0.f;
-        switch (cs.fmt[k]) {
-          case kQ8_0: d = dot_chunk<kQ8_0>(ur, c, g, gs); break;
-          case kQ2_K: d = dot_chunk<kQ2_K>(ur, c, g, gs); break;
-          case kQ3_K: d = dot_chunk<kQ3_K>(ur, c, g, gs); break;
-          case kQ4_K: d = dot_chunk<kQ4_K>(ur, c, g, gs); break;
-          case kQ5_K: d = dot_chunk<kQ5_K>(ur, c, g, gs); break;
-          case kQ6_K: d = dot_chunk<kQ6_K>(ur, c, g, gs); break;
-          case kIQ4_XS: d = dot_chunk<kIQ4_XS>(ur, c, g, gs); break;
-          default: fmt_ok = false;
-        }
+        with_unit(cs, region, k, lu, static_cast<uint32_t>(unit), [&](auto f, const auto& u) {
+          d = dot_unit<decltype(f)::value>(u, c, g, gs);
+        });
         acc[k * kThreads + threadIdx.x] += static_cast<double>(d);
         region += kUnits * slot_bytes(cs.ubytes[k]);
       }
     }
     __syncwarp();  // the slots are filled again
   }
-  if (!fmt_ok) report_error(err, kDevBadFormat, 4);
   __syncthreads();
   for (int k = warp; k < cs.K; k += kWarps) {
     double t = 0.0;

@@ -1364,6 +1364,13 @@ int vq_qk_norm_rope_bwd(const void* gq, const int64_t* gq_strides, const void* g
 namespace {
 
 // ---- gated embedding ----
+// The candidates with the alignment of their blocks in the formats' codes.
+int build_table(vq::CandSet* cs, int K, const int* types, const void* const* blocks) {
+  if (int rc = build_candset(cs, K, types, blocks)) return rc;
+  for (int k = 0; k < K; ++k) cs->fmt[k] = vq::embed::decode_code(cs->fmt[k], cs->ptr[k]);
+  return 0;
+}
+
 int check_table(int64_t T, int64_t vocab_start, int64_t rows, int64_t padded_cols, int64_t cols) {
   if (T < 0 || rows < 0 || cols < 0 || vocab_start < 0) return fail(VQ_ERR_INVALID, "negative shape or vocabulary start");
   if (padded_cols < cols || padded_cols % 256 != 0)
@@ -1457,22 +1464,37 @@ int vq_embed_plan(const void* ids, int ids_i32, int64_t T, int64_t vocab_start, 
   int bits = 1;
   while ((rows >> bits) != 0) ++bits;
   const int passes = (bits + kDigitBits - 1) / kDigitBits;
-  const int ctas = static_cast<int>(T >= static_cast<int64_t>(kSortCtas) * kSortThreads ? kSortCtas
-                                                                                        : (T + kSortThreads - 1) / kSortThreads);
   const PlanLayout l(T);
   char* c = static_cast<char*>(plan);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const Ids in{ids, ids_i32 != 0};
+  auto one_block = [&](auto items) {
+    constexpr int kItems = decltype(items)::value;
+    constexpr int smem = kSortSmem + kSortThreads * kItems * 6;
+    VQ_CUDA(cudaFuncSetAttribute(token_plan_block_kernel<kItems>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    token_plan_block_kernel<kItems><<<1, kSortThreads, smem, st>>>(in, static_cast<int>(T), vocab_start,
+                                                                   static_cast<int>(rows), passes, plan_at(plan, l));
+    VQ_CUDA(cudaGetLastError());
+    return 0;
+  };
+  if (T <= kSortThreads) return one_block(std::integral_constant<int, 1>{});
+  if (T <= 4 * kSortThreads) return one_block(std::integral_constant<int, 4>{});
+  const int ctas = T >= static_cast<int64_t>(kSortCtas) * kSortThreads
+                       ? kSortCtas
+                       : static_cast<int>((T + kSortThreads - 1) / kSortThreads);
+  VQ_CUDA(cudaFuncSetAttribute(token_plan_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas));
   cfg.blockDim = dim3(kSortThreads);
   cfg.dynamicSmemBytes = kSortSmem;
-  cfg.stream = static_cast<cudaStream_t>(stream);
+  cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = static_cast<unsigned>(ctas);
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  VQ_CUDA(cudaLaunchKernelEx(&cfg, token_plan_kernel, Ids{ids, ids_i32 != 0}, static_cast<int>(T),
+  VQ_CUDA(cudaLaunchKernelEx(&cfg, token_plan_kernel, in, static_cast<int>(T),
                              static_cast<long long>(vocab_start), static_cast<int>(rows), passes, plan_at(plan, l),
                              reinterpret_cast<int*>(c + l.keys), reinterpret_cast<int*>(c + l.keys_tmp),
                              reinterpret_cast<int*>(c + l.order_tmp)));
@@ -1485,7 +1507,7 @@ int vq_embed_mix(int K, const int* types, const void* const* blocks, const float
                  int64_t cols, float scale, int strict, void* out, int64_t ldo, void* stream) {
   DeviceScope scope(out);
   vq::CandSet cs;
-  if (int rc = build_candset(&cs, K, types, blocks)) return rc;
+  if (int rc = build_table(&cs, K, types, blocks)) return rc;
   if (int rc = check_table(T, vocab_start, rows, padded_cols, cols)) return rc;
   if (int rc = check_matrix(out, T, cols, ldo, "out")) return rc;
   if (T == 0 || cols == 0) return 0;
@@ -1521,7 +1543,7 @@ int vq_embed_gategrad(int K, const int* types, const void* const* blocks, const 
                       int dy_dtype, void* workspace, size_t workspace_bytes, float* grad, void* stream) {
   DeviceScope scope(grad);
   vq::CandSet cs;
-  if (int rc = build_candset(&cs, K, types, blocks)) return rc;
+  if (int rc = build_table(&cs, K, types, blocks)) return rc;
   if (int rc = check_table(T, 0, rows, padded_cols, cols)) return rc;
   if (int rc = check_matrix(dy, T, cols, lddy, "dy")) return rc;
   if (dy_dtype < 0 || dy_dtype > 2) return fail(VQ_ERR_INVALID, "dtype %d (0 = float32, 1 = bfloat16, 2 = float16)", dy_dtype);

@@ -789,7 +789,7 @@ def embed_mix(ids: torch.Tensor, qtypes, qbytes, probs: torch.Tensor, rows: int,
     """Rows scale * sum_k probs[k] W_k[ids] of a table of packed candidates -> bf16 [*ids.shape, cols].  With
     ``vocab_start`` the table holds the vocabulary from there on and tokens of other shards get rows of zeros;
     without it such ids are reported by ``device_error`` as well.  With the ids' ``plan`` a row is decoded once for
-    up to 16 tokens that name it, else once per token."""
+    up to 8 tokens that name it, else once per token."""
     dev = _device_of(ids, probs, *qbytes)
     ids = _ids_operand(ids)
     K, types, ptrs = _table_operands(qtypes, qbytes, rows, padded_cols, cols)
