@@ -383,12 +383,12 @@ int vq_embed_gategrad(int K, const int* types, const void* const* blocks, const 
 
 /* ---- global norm and clipping ----
  * norm[0] = sqrt(sum of squares) (or, with norm_inf, the largest magnitude) over n contiguous tensors (HOST arrays:
- * device pointers, element counts, dtypes 0 = float32, 1 = bfloat16, 2 = float16), and every value times
+ * device pointers, sizes in bytes, dtypes 0 = float32, 1 = bfloat16, 2 = float16), and every value times
  * min(1, max_norm / (norm + 1e-6)) in place.  max_norm = infinity only takes the norm.  Tensors of no elements are
  * skipped; tensors that share memory are refused.  Replaces torch.nn.utils.clip_grad_norm_ in
  * voodoo_quant/training/trainer.py:2607-2616.  `workspace`: vq_clip_grad_norm_workspace_bytes(n), 8-byte aligned. */
 size_t vq_clip_grad_norm_workspace_bytes(int n);
-int vq_clip_grad_norm(int n, const void* const* ptrs, const int64_t* numel, const int* dtypes, float max_norm,
+int vq_clip_grad_norm(int n, const void* const* ptrs, const int64_t* bytes, const int* dtypes, float max_norm,
                       int norm_inf, void* workspace, size_t workspace_bytes, float* norm, void* stream);
 
 #ifdef __cplusplus

@@ -6,7 +6,7 @@ one bf16 rounding (2^-8) of the value plus the fp32 chain -- K candidates,
 each a product and a sum, of magnitudes below three times the row's largest
 weight (code times scale and the block's offset are each within twice the
 largest), so below 2e-5 of it for K <= 8.  Gradient: chains of at most 64
-roundings of 2^-24 (a run of 32 rows of dy, then a sub-block of 32 weights)
+roundings of 2^-24 (a piece's 8 rows of dy, then a sub-block of 32 weights)
 relative to the sum of |dy| times three times the row's largest weight; the
 runs are joined in 64 bits.
 """
@@ -151,13 +151,14 @@ def test_one_token_for_all_and_one_shard_without_any(cuda):
     ids = torch.full((T,), 7)
     g = torch.Generator(device="cpu").manual_seed(1)
     dy = torch.randn(T, D, generator=g).to(torch.bfloat16)
-    grad = _C.embed_gategrad(dy.to(cuda), _C.embed_plan(ids.to(cuda), V), types, blocks, V, D, D)
+    table = _C.EmbedTable(types, blocks, V, D, D)
+    grad = _C.embed_gategrad(dy.to(cuda), table, _C.embed_plan(ids.to(cuda), V))
     _check_grad(grad, dy, ids, dec, 1.0, 0, V)
     plan = _C.embed_plan(ids.to(cuda), V, 100)
-    none = _C.embed_gategrad(dy.to(cuda), plan, types, blocks, V, D, D)
+    none = _C.embed_gategrad(dy.to(cuda), table, plan)
     assert torch.equal(none, torch.zeros_like(none))
     for q in (plan, None):
-        assert not _C.embed_mix(ids.to(cuda), types, blocks, p.to(cuda), V, D, D, vocab_start=100, plan=q).any()
+        assert not _C.embed_mix(ids.to(cuda), table, p.to(cuda), vocab_start=100, plan=q).any()
     assert _C.device_error() == 0
 
 
@@ -171,15 +172,16 @@ def test_ids_outside_the_table(cuda):
     ids = torch.tensor([3, -1, 19, 20, 2 ** 40, -2 ** 62, 0])
     good = (ids >= 0) & (ids < V)
     assert _C.device_error() == 0
+    table = _C.EmbedTable(types, blocks, V, D, D)
     plan = _C.embed_plan(ids.to(cuda), V)
     for q in (plan, None):
-        out = _C.embed_mix(ids.to(cuda), types, blocks, p.to(cuda), V, D, D, plan=q)
+        out = _C.embed_mix(ids.to(cuda), table, p.to(cuda), plan=q)
         assert _C.device_error() == (4 << 16 | 30) and _C.device_error() == 0
         _check_lookup(out[good.to(cuda)], ids[good], dec, p, 1.0, 0, V)
         assert not out[~good.to(cuda)].any()
     dy = torch.ones(7, D, dtype=torch.bfloat16)
     dy[1] = float("nan")  # of an id that is not in the table
-    grad = _C.embed_gategrad(dy.to(cuda), plan, types, blocks, V, D, D)
+    grad = _C.embed_gategrad(dy.to(cuda), table, plan)
     _check_grad(grad, dy, ids, dec, 1.0, 0, V)
 
 
@@ -216,12 +218,12 @@ def test_unaligned_blocks(cuda):
         _, _, blocks, dec, p = _table(V, D, [qt], 6, cuda)
         ids = _ids(T, V, 7)
         one = torch.ones(1, device=cuda)
-        want = _C.embed_mix(ids.to(cuda), [qt], blocks, one, V, D, D)
+        want = _C.embed_mix(ids.to(cuda), _C.EmbedTable([qt], blocks, V, D, D), one)
         for off in (2, 6, 14):
             buf = torch.empty(blocks[0].numel() + 16, dtype=torch.uint8, device=cuda)
             b = buf[off:off + blocks[0].numel()]
             b.copy_(blocks[0].reshape(-1))
-            assert torch.equal(_C.embed_mix(ids.to(cuda), [qt], [b], one, V, D, D), want)
+            assert torch.equal(_C.embed_mix(ids.to(cuda), _C.EmbedTable([qt], [b], V, D, D), one), want)
 
 
 def test_streams_graphs_and_repeats(cuda):
@@ -234,11 +236,11 @@ def test_streams_graphs_and_repeats(cuda):
     sets = [(_ids(T, V, s).to(cuda), torch.randn(T, D, generator=torch.Generator().manual_seed(s)).to(torch.bfloat16).to(cuda))
             for s in (1, 2)]
     pd = p.to(cuda)
+    table = _C.EmbedTable(types, blocks, V, D, D)
 
     def call(ids, dy):
         plan = _C.embed_plan(ids, V)
-        return (_C.embed_mix(ids, types, blocks, pd, V, D, D), _C.embed_mix(ids, types, blocks, pd, V, D, D, plan=plan),
-                _C.embed_gategrad(dy, plan, types, blocks, V, D, D))
+        return (_C.embed_mix(ids, table, pd), _C.embed_mix(ids, table, pd, plan=plan), _C.embed_gategrad(dy, table, plan))
 
     want = [call(*s) for s in sets]
     again = [call(*s) for s in sets]

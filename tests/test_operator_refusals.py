@@ -117,16 +117,16 @@ def test_gated_embedding_refuses():
 def test_clip_refuses():
     lib = _lib()
 
-    def clip(ptrs, numel, codes, max_norm=1.0, ws=ONE, nbytes=1 << 20, norm=ONE):
+    def clip(ptrs, nbytes_of, codes, max_norm=1.0, ws=ONE, nbytes=1 << 20, norm=ONE):
         n = len(ptrs)
-        return lib.vq_clip_grad_norm(n, (ctypes.c_void_p * n)(*ptrs), (ctypes.c_int64 * n)(*numel),
+        return lib.vq_clip_grad_norm(n, (ctypes.c_void_p * n)(*ptrs), (ctypes.c_int64 * n)(*nbytes_of),
                                      (ctypes.c_int * n)(*codes), max_norm, 0, ws, nbytes, norm, None)
 
     for args, kw, text in (
             (([ONE], [4], [0]), dict(max_norm=-1.0), "max_norm"), (([ONE], [4], [0]), dict(max_norm=math.nan), "max_norm"),
-            (([ONE], [-4], [0]), {}, "bad size"), (([ONE], [4], [3]), {}, "dtype"), (([None], [4], [0]), {}, "null"),
+            (([ONE], [-4], [0]), {}, "bad size"), (([ONE], [3], [1]), {}, "bad size"), (([ONE], [4], [3]), {}, "dtype"), (([None], [4], [0]), {}, "null"),
             (([ONE + 2], [4], [0]), {}, "misaligned"), (([ONE + 1], [4], [1]), {}, "misaligned"),
-            (([ONE, ONE], [4, 4], [0, 0]), {}, "share memory"), (([ONE + 16, ONE], [4, 9], [1, 1]), {}, "share memory"),
+            (([ONE, ONE], [4, 4], [0, 0]), {}, "share memory"), (([ONE + 16, ONE], [8, 18], [1, 1]), {}, "share memory"),
             (([ONE], [4], [0]), dict(nbytes=8), "workspace"), (([ONE], [4], [0]), dict(ws=None), "workspace"),
             (([ONE], [4], [0]), dict(norm=None), "null")):
         _refused(clip(*args, **kw), text)

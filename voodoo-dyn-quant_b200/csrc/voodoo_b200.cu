@@ -1588,12 +1588,12 @@ struct Range {
 constexpr long long kClipSmallValues = 16384;
 
 template <int N>
-void fill_table(vq::clip::Table<N>* t, const void* const* ptrs, const int64_t* numel, const int* dtypes, int n) {
+void fill_table(vq::clip::Table<N>* t, const void* const* ptrs, const int64_t* bytes_of, const int* dtypes, int n) {
   long long chunks = 0;
   t->n = n;
   for (int i = 0; i < n; ++i) {
     const uintptr_t p = reinterpret_cast<uintptr_t>(ptrs[i]);
-    const long long bytes = numel[i] * (dtypes[i] == vq::clip::kF32 ? 4 : 2);
+    const long long bytes = bytes_of[i];
     t->ptr[i] = p;
     t->bytes[i] = bytes;
     t->dtype[i] = static_cast<uint8_t>(dtypes[i]);
@@ -1605,24 +1605,24 @@ void fill_table(vq::clip::Table<N>* t, const void* const* ptrs, const int64_t* n
 }
 
 template <int N, bool kMax>
-int launch_clip(const void* const* ptrs, const int64_t* numel, const int* dtypes, int n, long long total,
+int launch_clip(const void* const* ptrs, const int64_t* bytes, const int* dtypes, int n, long long total,
                 float max_norm, double* partials, int max_partials, float* norm, cudaStream_t st) {
   using namespace vq::clip;
   static_assert(sizeof(Table<N>) + 64 <= 32764, "kernel parameters");
   Table<N> tab;
   if (n <= N && total <= kClipSmallValues) {
-    fill_table(&tab, ptrs, numel, dtypes, n);
+    fill_table(&tab, ptrs, bytes, dtypes, n);
     small_kernel<N, kMax><<<1, kSmallThreads, 0, st>>>(tab, max_norm, max_norm != INFINITY, norm);
     VQ_CUDA(cudaGetLastError());
     return 0;
   }
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
-  int cap = kBlocksPerSm * sms < vq::clip::kMaxBlocks ? kBlocksPerSm * sms : vq::clip::kMaxBlocks;
+  const int cap = kBlocksPerSm * sms < vq::clip::kMaxBlocks ? kBlocksPerSm * sms : vq::clip::kMaxBlocks;
   int used = 0;
   for (int i = 0; i < n; i += N) {
     const int m = n - i < N ? n - i : N;
-    fill_table(&tab, ptrs + i, numel + i, dtypes + i, m);
+    fill_table(&tab, ptrs + i, bytes + i, dtypes + i, m);
     const int grid = tab.chunks < cap ? tab.chunks : cap;
     if (used + grid > max_partials) return fail(VQ_ERR_INVALID, "workspace too small");
     norm_kernel<N, kMax><<<grid, kThreads, 0, st>>>(tab, partials + used);
@@ -1633,8 +1633,9 @@ int launch_clip(const void* const* ptrs, const int64_t* numel, const int* dtypes
   const bool scale = max_norm != INFINITY;
   for (int i = scale ? (n - 1) / N * N : 0; i >= 0; i -= N) {
     const int m = n - i < N ? n - i : N;
-    if (scale && n > N) fill_table(&tab, ptrs + i, numel + i, dtypes + i, m);
-    const int grid = !scale ? 1 : tab.chunks < cap ? tab.chunks : cap;
+    if (scale && n > N) fill_table(&tab, ptrs + i, bytes + i, dtypes + i, m);
+    const int wave = kScaleBlocksPerSm * sms;
+    const int grid = !scale ? 1 : tab.chunks < wave ? tab.chunks : wave;
     scale_kernel<N, kMax><<<grid, kThreads, 0, st>>>(tab, partials, used, max_norm, scale, i == 0 ? norm : nullptr);
     VQ_CUDA(cudaGetLastError());
   }
@@ -1651,14 +1652,14 @@ size_t vq_clip_grad_norm_workspace_bytes(int n) {
   return launches * vq::clip::kMaxBlocks * sizeof(double);
 }
 
-int vq_clip_grad_norm(int n, const void* const* ptrs, const int64_t* numel, const int* dtypes, float max_norm,
+int vq_clip_grad_norm(int n, const void* const* ptrs, const int64_t* bytes, const int* dtypes, float max_norm,
                       int norm_inf, void* workspace, size_t workspace_bytes, float* norm, void* stream) {
   DeviceScope scope(norm);
   if (n < 0) return fail(VQ_ERR_INVALID, "negative count");
   if (norm == nullptr) return fail(VQ_ERR_INVALID, "null pointer");
   if (!(max_norm >= 0.f)) return fail(VQ_ERR_INVALID, "max_norm must not be negative or NaN");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (n > 0 && (ptrs == nullptr || numel == nullptr || dtypes == nullptr)) return fail(VQ_ERR_INVALID, "null array");
+  if (n > 0 && (ptrs == nullptr || bytes == nullptr || dtypes == nullptr)) return fail(VQ_ERR_INVALID, "null array");
   if (n > (1 << 20)) return fail(VQ_ERR_INVALID, "too many tensors");
   // the tensors that hold something, checked, with their ranges in order
   Range* r = static_cast<Range*>(std::malloc(static_cast<size_t>(n + 1) * sizeof(Range)));
@@ -1673,15 +1674,15 @@ int vq_clip_grad_norm(int n, const void* const* ptrs, const int64_t* numel, cons
   int m = 0;
   long long total = 0;
   for (int i = 0; i < n; ++i) {
-    if (numel[i] < 0 || numel[i] > (1LL << 40)) return fail(VQ_ERR_INVALID, "tensor %d: bad size", i);
     if (dtypes[i] < 0 || dtypes[i] > 2) return fail(VQ_ERR_INVALID, "tensor %d: dtype %d (0 = float32, 1 = bfloat16, 2 = float16)", i, dtypes[i]);
-    if (numel[i] == 0) continue;
     const int es = dtypes[i] == 0 ? 4 : 2;
+    if (bytes[i] < 0 || bytes[i] > (1LL << 40) || bytes[i] % es != 0) return fail(VQ_ERR_INVALID, "tensor %d: bad size", i);
+    if (bytes[i] == 0) continue;
     const uintptr_t b = reinterpret_cast<uintptr_t>(ptrs[i]);
     if (b == 0 || b % es != 0) return fail(VQ_ERR_INVALID, "tensor %d: null or misaligned pointer", i);
-    p[m] = ptrs[i], c[m] = numel[i], d[m] = dtypes[i];
-    r[m] = Range{b, b + static_cast<uintptr_t>(numel[i]) * es};
-    total += numel[i];
+    p[m] = ptrs[i], c[m] = bytes[i], d[m] = dtypes[i];
+    r[m] = Range{b, b + static_cast<uintptr_t>(bytes[i])};
+    total += bytes[i] / es;
     ++m;
   }
   if (total > (1LL << 42)) return fail(VQ_ERR_INVALID, "too many values");

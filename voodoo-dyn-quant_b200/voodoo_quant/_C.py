@@ -14,6 +14,7 @@ from __future__ import annotations
 import ctypes
 import os
 from array import array
+from operator import attrgetter
 from pathlib import Path
 
 import torch
@@ -754,22 +755,35 @@ def _ids_operand(ids: torch.Tensor) -> torch.Tensor:
     return ids.contiguous()
 
 
-def _table_operands(qtypes, qbytes, rows: int, padded_cols: int, cols: int):
-    """The checked candidates' arrays for the C ABI: K, types, pointers."""
-    K = len(qtypes)
-    if not 1 <= K <= 8 or K != len(qbytes):
-        raise ValueError(f"1..8 candidates with their blocks expected, got {K} types and {len(qbytes)} tensors")
-    if rows < 0 or cols < 0 or cols > padded_cols or padded_cols % 256:
-        raise ValueError(f"table of {rows} rows: {padded_cols} stored columns must be a multiple of 256 that holds {cols}")
-    types, ptrs = (_int * K)(), (_vp * K)()
-    for i, (qt, qb) in enumerate(zip(qtypes, qbytes)):
-        be, bb = _geometry(qt)
-        if qb.dtype != torch.uint8 or not qb.is_contiguous() or qb.numel() != rows * (padded_cols // be) * bb:
-            raise ValueError(f"{qt}: contiguous uint8 blocks of {rows * (padded_cols // be) * bb} bytes expected, got "
-                             f"{qb.dtype} {tuple(qb.shape)}")
-        types[i] = GGML_TYPE[qt]
-        ptrs[i] = qb.data_ptr()
-    return K, types, ptrs
+class EmbedTable:
+    """The checked packed candidates of an embedding table: what ``embed_mix`` and ``embed_gategrad`` pass on.  Holds
+    the blocks; nothing of it outlives the call (or the backward) that made it."""
+
+    __slots__ = ("blocks", "rows", "padded_cols", "cols", "device", "K", "types", "ptrs")
+
+    def __init__(self, qtypes, qbytes, rows: int, padded_cols: int, cols: int):
+        K = len(qtypes)
+        if not 1 <= K <= 8 or K != len(qbytes):
+            raise ValueError(f"1..8 candidates with their blocks expected, got {K} types and {len(qbytes)} tensors")
+        if rows < 0 or cols < 0 or cols > padded_cols or padded_cols % 256:
+            raise ValueError(f"table of {rows} rows: {padded_cols} stored columns must be a multiple of 256 that holds "
+                             f"{cols}")
+        self.device = _device_of(*qbytes)
+        self.blocks, self.rows, self.padded_cols, self.cols, self.K = tuple(qbytes), rows, padded_cols, cols, K
+        self.types, self.ptrs = (_int * K)(), (_vp * K)()
+        for i, (qt, qb) in enumerate(zip(qtypes, qbytes)):
+            be, bb = _geometry(qt)
+            if qb.dtype != torch.uint8 or not qb.is_contiguous() or qb.numel() != rows * (padded_cols // be) * bb:
+                raise ValueError(f"{qt}: contiguous uint8 blocks of {rows * (padded_cols // be) * bb} bytes expected, got "
+                                 f"{qb.dtype} {tuple(qb.shape)}")
+            self.types[i] = GGML_TYPE[qt]
+            self.ptrs[i] = qb.data_ptr()
+
+    def check(self, *ts: torch.Tensor) -> None:
+        for t in ts:
+            if t.get_device() != self.device:
+                _require_cuda(*ts)
+                raise ValueError(f"tensors on cuda:{self.device} expected, got {t.device}")
 
 
 def embed_plan(ids: torch.Tensor, rows: int, vocab_start: int | None = None) -> torch.Tensor:
@@ -778,75 +792,88 @@ def embed_plan(ids: torch.Tensor, rows: int, vocab_start: int | None = None) -> 
     dev = _device_of(ids)
     ids = _ids_operand(ids)
     T = ids.numel()
-    plan = torch.empty(_lib.vq_embed_plan_bytes(T), dtype=torch.uint8, device=ids.device)
+    need = _lib.vq_embed_plan_bytes(T)
+    plan = torch.empty(need, dtype=torch.uint8, device=ids.device)
     _check(_lib.vq_embed_plan(ids.data_ptr(), ids.dtype == torch.int32, T, vocab_start or 0, rows, plan.data_ptr(),
-                              plan.numel(), _raw_stream(dev)))
+                              need, _raw_stream(dev)))
     return plan
 
 
-def embed_mix(ids: torch.Tensor, qtypes, qbytes, probs: torch.Tensor, rows: int, padded_cols: int, cols: int,
-              scale: float = 1.0, vocab_start: int | None = None, plan: torch.Tensor | None = None) -> torch.Tensor:
+def embed_mix(ids: torch.Tensor, table: EmbedTable, probs: torch.Tensor, scale: float = 1.0,
+              vocab_start: int | None = None, plan: torch.Tensor | None = None) -> torch.Tensor:
     """Rows scale * sum_k probs[k] W_k[ids] of a table of packed candidates -> bf16 [*ids.shape, cols].  With
     ``vocab_start`` the table holds the vocabulary from there on and tokens of other shards get rows of zeros;
     without it such ids are reported by ``device_error`` as well.  With the ids' ``plan`` a row is decoded once for
     up to 8 tokens that name it, else once per token."""
-    dev = _device_of(ids, probs, *qbytes)
+    table.check(ids, probs)
     ids = _ids_operand(ids)
-    K, types, ptrs = _table_operands(qtypes, qbytes, rows, padded_cols, cols)
-    if probs.numel() != K:
-        raise ValueError(f"{K} probabilities expected, got {tuple(probs.shape)}")
+    if probs.numel() != table.K:
+        raise ValueError(f"{table.K} probabilities expected, got {tuple(probs.shape)}")
     if probs.dtype != torch.float32 or not probs.is_contiguous():
         probs = probs.detach().to(torch.float32).contiguous()
+    cols = table.cols
     out = torch.empty(*ids.shape, cols, dtype=torch.bfloat16, device=ids.device)
-    _check(_lib.vq_embed_mix(K, types, ptrs, probs.data_ptr(), ids.data_ptr(), ids.dtype == torch.int32, ids.numel(),
-                             _ptr(plan), 0 if plan is None else plan.numel(), vocab_start or 0, rows, padded_cols, cols,
-                             scale, vocab_start is None, out.data_ptr(), cols, _raw_stream(dev)))
+    _check(_lib.vq_embed_mix(table.K, table.types, table.ptrs, probs.data_ptr(), ids.data_ptr(), ids.dtype == torch.int32,
+                             ids.numel(), _ptr(plan), 0 if plan is None else plan.numel(), vocab_start or 0, table.rows,
+                             table.padded_cols, cols, scale, vocab_start is None, out.data_ptr(), cols,
+                             _raw_stream(table.device)))
     return out
 
 
-def embed_gategrad(dy: torch.Tensor, plan: torch.Tensor, qtypes, qbytes, rows: int, padded_cols: int, cols: int,
-                   scale: float = 1.0) -> torch.Tensor:
+def embed_gategrad(dy: torch.Tensor, table: EmbedTable, plan: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     """grad[k] = scale * sum_t <dy[t], W_k[ids[t]]> (float32 [K]) for dy [..., cols] in float32, bfloat16 or float16 and
     the plan of its ids; ids outside the table add nothing."""
-    dev = _device_of(dy, plan, *qbytes)
-    K, types, ptrs = _table_operands(qtypes, qbytes, rows, padded_cols, cols)
+    table.check(dy, plan)
+    K, cols = table.K, table.cols
     code = _float_code(dy, "embed_gategrad")
     if dy.dim() < 1 or dy.shape[-1] != cols:
         raise ValueError(f"gradient rows of {cols} columns expected, got {tuple(dy.shape)}")
     if dy.dim() != 2:
         dy = dy.reshape(-1, cols) if cols else dy.new_empty(0, 0)
     T = dy.shape[0]
-    if plan.numel() != _lib.vq_embed_plan_bytes(T):
+    nplan = plan.numel()
+    if nplan != _lib.vq_embed_plan_bytes(T):
         raise ValueError(f"the plan is not one of {T} tokens")
     ld, unit = dy.stride()
     if unit != 1 or ld < cols:
         dy, ld = dy.contiguous(), cols
-    ws = torch.empty(_lib.vq_embed_gategrad_workspace_bytes(K), dtype=torch.uint8, device=dy.device)
+    need = _lib.vq_embed_gategrad_workspace_bytes(K)
+    ws = torch.empty(need, dtype=torch.uint8, device=dy.device)
     g = torch.empty(K, dtype=torch.float32, device=dy.device)
-    _check(_lib.vq_embed_gategrad(K, types, ptrs, plan.data_ptr(), plan.numel(), T, rows, padded_cols, cols, scale,
-                                  dy.data_ptr(), ld, code, ws.data_ptr(), ws.numel(), g.data_ptr(), _raw_stream(dev)))
+    _check(_lib.vq_embed_gategrad(K, table.types, table.ptrs, plan.data_ptr(), nplan, T, table.rows, table.padded_cols,
+                                  cols, scale, dy.data_ptr(), ld, code, ws.data_ptr(), need, g.data_ptr(),
+                                  _raw_stream(table.device)))
     return g
 
 
 # ---------------------------------------------------------------- global norm and clipping
+_dtype_of, _nbytes_of = attrgetter("dtype"), attrgetter("nbytes")
+
+
+class NotContiguous(ValueError):
+    """A tensor is sparse or has strides of its own."""
+
+
 def clip_grad_norm(tensors, max_norm: float = float("inf"), norm_inf: bool = False) -> torch.Tensor:
     """Global 2-norm (or largest magnitude) of dense, non-overlapping CUDA tensors as a float32 scalar on their device,
     and every value times min(1, max_norm / (norm + 1e-6)) in place; an infinite ``max_norm`` leaves them as they are."""
     n = len(tensors)
     if n == 0:
         raise ValueError("clip_grad_norm: no tensors")
-    # one list per property: a few hundred short tensors cost more here than on the GPU
+    # one pass per property: a few hundred short tensors cost more here than on the GPU
     dev = _device_of(tensors[0])
-    if any([t.get_device() != dev for t in tensors]):
+    if set(map(torch.Tensor.get_device, tensors)) != {dev}:
         _device_of(*tensors)
-    if not all([t.is_contiguous() for t in tensors]):
-        raise ValueError("clip_grad_norm: contiguous tensors expected")
-    try:
-        codes = array("i", [_FLOAT_CODE[t.dtype] for t in tensors])
-    except KeyError as e:
-        raise ValueError(f"clip_grad_norm: float32, bfloat16 or float16 expected, got {e.args[0]}") from None
-    ptrs = array("Q", [t.data_ptr() for t in tensors])
-    sizes = array("q", [t.numel() for t in tensors])
+    if not all(map(torch.Tensor.is_contiguous, tensors)):  # nor is a sparse one
+        raise NotContiguous("clip_grad_norm: contiguous tensors expected")
+    types = set(map(_dtype_of, tensors))
+    for d in types:
+        if d not in _FLOAT_CODE:
+            raise ValueError(f"clip_grad_norm: float32, bfloat16 or float16 expected, got {d}")
+    codes = array("i", [_FLOAT_CODE[types.pop()]]) * n if len(types) == 1 else \
+        array("i", [_FLOAT_CODE[t.dtype] for t in tensors])
+    ptrs = array("Q", map(torch.Tensor.data_ptr, tensors))
+    sizes = array("q", map(_nbytes_of, tensors))
     device = tensors[0].device
     norm = torch.empty((), dtype=torch.float32, device=device)
     need = _lib.vq_clip_grad_norm_workspace_bytes(n)

@@ -715,23 +715,22 @@ class _GatedEmbeddingFunction(Function):
     host round trip."""
 
     @staticmethod
-    def forward(ctx, probs: torch.Tensor, ids: torch.Tensor, table: tuple, vocab_start: int | None, dtype: torch.dtype):
-        plan = _C.embed_plan(ids, table[2], vocab_start)
+    def forward(ctx, probs: torch.Tensor, ids: torch.Tensor, table: "_C.EmbedTable", scale: float,
+                vocab_start: int | None, dtype: torch.dtype):
+        plan = _C.embed_plan(ids, table.rows, vocab_start)
         ctx.save_for_backward(plan)
-        ctx.table, ctx.like = table, (probs.dtype, probs.shape)  # the candidates' blocks are constants
-        return _embedding_rows(probs, ids, table, vocab_start, dtype, plan)
+        ctx.table, ctx.scale, ctx.like = table, scale, (probs.dtype, probs.shape)  # the candidates are constants
+        return _embedding_rows(probs, ids, table, scale, vocab_start, dtype, plan)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g: torch.Tensor):
-        qtypes, qbytes, rows, padded_cols, cols, scale = ctx.table
-        gp = _C.embed_gategrad(g, ctx.saved_tensors[0], qtypes, qbytes, rows, padded_cols, cols, scale)
-        return gp.to(ctx.like[0]).view(ctx.like[1]), None, None, None, None
+        gp = _C.embed_gategrad(g, ctx.table, ctx.saved_tensors[0], ctx.scale)
+        return gp.to(ctx.like[0]).view(ctx.like[1]), None, None, None, None, None
 
 
-def _embedding_rows(probs, ids, table, vocab_start, dtype, plan=None):
-    qtypes, qbytes, rows, padded_cols, cols, scale = table
-    out = _C.embed_mix(ids, qtypes, qbytes, probs, rows, padded_cols, cols, scale, vocab_start, plan)
+def _embedding_rows(probs, ids, table, scale, vocab_start, dtype, plan=None):
+    out = _C.embed_mix(ids, table, probs, scale, vocab_start, plan)
     # the mixture is bf16 everywhere on this path (W_mix); other types hold its bf16 values
     return out if dtype == torch.bfloat16 else out.to(dtype)
 
@@ -750,10 +749,11 @@ def gated_embedding(ids: torch.Tensor, probs: torch.Tensor, candidate_types, can
         raise ValueError(f"gated_embedding: float32, bfloat16 or float16 rows, got {dtype}")
     if vocab_start is not None and vocab_start < 0:
         raise ValueError(f"gated_embedding: vocab_start {vocab_start} is negative")
-    table = (candidate_types, tuple(candidate_blocks), num_embeddings, _padded(embedding_dim), embedding_dim, float(scale))
+    table = _C.EmbedTable(candidate_types, candidate_blocks, num_embeddings, _padded(embedding_dim), embedding_dim)
+    scale = float(scale)
     if not (probs.requires_grad and torch.is_grad_enabled()):
-        return _embedding_rows(probs, ids, table, vocab_start, dtype)
-    return _GatedEmbeddingFunction.apply(probs, ids, table, vocab_start, dtype)
+        return _embedding_rows(probs, ids, table, scale, vocab_start, dtype)
+    return _GatedEmbeddingFunction.apply(probs, ids, table, scale, vocab_start, dtype)
 
 
 # --------------------------------------------------------------------------- modules

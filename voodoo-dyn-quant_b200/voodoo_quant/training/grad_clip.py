@@ -24,6 +24,8 @@ def _norm_is_inf(norm_type: float) -> bool:
 
 def _dense(g: torch.Tensor) -> torch.Tensor | None:
     """A contiguous view of all of g's memory, or None where g has gaps or overlaps."""
+    if g.layout is not torch.strided:
+        raise ValueError(f"clip_grad_norm_: dense gradients expected, got {g.layout}")
     if g.is_contiguous():
         return g
     order = sorted(range(g.dim()), key=lambda d: (g.stride(d), g.shape[d]), reverse=True)
@@ -33,20 +35,19 @@ def _dense(g: torch.Tensor) -> torch.Tensor | None:
 
 def _run(grads, max_norm: float, norm_type: float) -> torch.Tensor:
     norm_inf = _norm_is_inf(norm_type)
-    copies = []
-    flat = grads
-    if not all([g.layout is torch.strided and g.is_contiguous() for g in grads]):
-        flat = []
-        for g in grads:
-            if g.layout is not torch.strided:
-                raise ValueError("clip_grad_norm_: dense gradients expected")
-            v = _dense(g)
-            if v is None:  # scaled as a copy
-                if any(st == 0 and n > 1 for st, n in zip(g.stride(), g.shape)):
-                    raise ValueError("clip_grad_norm_: an expanded gradient shares memory with itself")
-                v = g.contiguous()
-                copies.append((g, v))
-            flat.append(v)
+    try:
+        return _C.clip_grad_norm(grads, max_norm, norm_inf)  # checks that they are contiguous
+    except _C.NotContiguous:
+        pass
+    flat, copies = [], []
+    for g in grads:
+        v = _dense(g)
+        if v is None:  # scaled as a copy
+            if any(st == 0 and n > 1 for st, n in zip(g.stride(), g.shape)):
+                raise ValueError("clip_grad_norm_: an expanded gradient shares memory with itself")
+            v = g.contiguous()
+            copies.append((g, v))
+        flat.append(v)
     norm = _C.clip_grad_norm(flat, max_norm, norm_inf)
     if not math.isinf(max_norm):
         for g, v in copies:

@@ -131,8 +131,9 @@ class Q8Embedding(nn.Module):
         from voodoo_quant.layers import _STATIC_STATE
 
         if self.qweight.is_cuda:  # decode, scale and place the tokens' rows in one kernel
-            return _C.embed_mix(ids, ["Q8_0"], [self.qweight], self._one, self.num_embeddings, self.embedding_dim,
-                                self.embedding_dim, self.scale)
+            D = self.embedding_dim
+            table = _C.EmbedTable(["Q8_0"], [self.qweight], self.num_embeddings, D, D)
+            return _C.embed_mix(ids, table, self._one, self.scale)
         e = self._rows(ids, _STATIC_STATE.enabled)
         return e if self.scale == 1.0 else (e.float() * self.scale).to(e.dtype)
 
