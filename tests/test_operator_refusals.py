@@ -175,3 +175,19 @@ def test_scaled_embeddings_keep_their_factor_on_cpu_paths():
     assert embed_scale(e) == 1.0
     e.embed_scale = 31.62
     assert embed_scale(e) == float(torch.tensor(31.62).bfloat16())
+
+
+def test_head_norm_models_build_and_fuse_on_cpu():
+    """The synthetic decoder with head norms is built from Qwen3 blocks; patched blocks run their own forward off the
+    fused path."""
+    pytest.importorskip("transformers")
+    from voodoo_quant.fused_blocks import fuse_llama_blocks, fuse_qwen3_blocks
+    from voodoo_quant.training import synthetic as S
+
+    shape = S.SHAPES["tiny-qk"]
+    a, b = (S.build_llama(shape, "cpu", seed=2) for _ in range(2))
+    assert fuse_llama_blocks(b) == 0
+    assert fuse_qwen3_blocks(b, causal_batches=True) == 2 * 7 + 1 + 1
+    x = torch.randint(0, shape.vocab, (1, 16))
+    with torch.no_grad():
+        assert torch.equal(a(input_ids=x, use_cache=False).logits, b(input_ids=x, use_cache=False).logits)
