@@ -6,10 +6,12 @@
 //           = scale * sum over runs of equal id of <sum of the run's dy, W_k[id]>
 //
 // Neither writes a decoded row of a candidate: the lookup decodes and mixes a
-// token's packed rows in registers, the gradient sums the rows of dy of equal
-// tokens first (token_plan_kernel brings them together) and multiplies the
-// decoded weights into that sum as it decodes them.  Both are bound by HBM
-// (packed rows, and T x D of out or dy), closely followed by the decoding.
+// packed row in registers and writes it to all tokens of a piece, the gradient
+// sums a piece's rows of dy first and multiplies the decoded weights into that
+// sum as it decodes them.  What they cannot do without is the packed rows and
+// T x D of out or dy (16384 x 4096 of text, six candidates: 35 us of HBM each);
+// the decoding bounds them, some 245 instructions for 32 weights of a
+// candidate (82 us the lookup, 81 us the gradient).
 //
 // Eight lanes hold a unit (256 weights) of a row, a lane 32 consecutive
 // weights.  The lanes of a unit copy its packed bytes of every candidate into
@@ -26,15 +28,12 @@ namespace embed {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kUnits = 4;   // units of a warp
-#ifndef VQ_EMBED_MIX_BLOCKS
-#define VQ_EMBED_MIX_BLOCKS 3
-#endif
-#ifndef VQ_EMBED_GRAD_BLOCKS
-#define VQ_EMBED_GRAD_BLOCKS 3
-#endif
-constexpr int kMixBlocks = VQ_EMBED_MIX_BLOCKS, kGradBlocks = VQ_EMBED_GRAD_BLOCKS;  // resident per SM
-constexpr int kMaxBlocks = 1184;  // of a gradient launch: the partials it leaves
+constexpr int kUnits = 4;  // units of a warp
+// Resident blocks per SM, and so 80 registers a thread: decoding keeps every
+// pipe half busy and waits for its own results, so warps count (16384 x 4096
+// text, six candidates: 82 us with 3, 95 with 2; 4 blocks spill and take 113).
+constexpr int kBlocksPerSm = 3;
+constexpr int kMaxBlocks = 1184;  // of a launch: the partials that the gradient leaves
 
 // A unit's slot: the 16-byte aligned span of a 2-byte aligned unit, and a
 // word more for the field reads that join two words.
@@ -198,8 +197,7 @@ struct UnitWalk {
 };
 
 // ---------------------------------------------------------------- lookup
-// mix_chunk's arithmetic, one value an instruction: pairs (f32x2) cost more
-// moves into aligned registers here than they save (DECIDE).
+// mix_chunk on any reference of a unit: the same operations in the same order.
 template <int F, class U>
 __device__ __forceinline__ void mix_unit(const U& u, int c, float pk, float (&acc)[32], float (&cst)[2]) {
   float a[2], b[2];
@@ -210,19 +208,14 @@ __device__ __forceinline__ void mix_unit(const U& u, int c, float pk, float (&ac
     cst[0] = fmaf(pk, b[0], cst[0]);
     cst[1] = fmaf(pk, b[1], cst[1]);
   }
-#ifdef VQ_SCALAR
-#pragma unroll
-  for (int j = 0; j < 32; ++j)
-    acc[j] = fmaf(pa[j >> 4], magic_byte(qb[j >> 2], j & 3) - MixChunk<F>::kSub, acc[j]);
-#else
   const float2 nsub = make_float2(-MixChunk<F>::kSub, -MixChunk<F>::kSub);
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
-    const float2 q = __fadd2_rn(make_float2(magic_byte(qb[j >> 1], 2 * (j & 1)), magic_byte(qb[j >> 1], 2 * (j & 1) + 1)), nsub);
+    const int i = 2 * (j & 1);
+    const float2 q = __fadd2_rn(make_float2(magic_byte(qb[j >> 1], i), magic_byte(qb[j >> 1], i + 1)), nsub);
     const float2 r = __ffma2_rn(make_float2(pa[j >> 3], pa[j >> 3]), q, make_float2(acc[2 * j], acc[2 * j + 1]));
     acc[2 * j] = r.x, acc[2 * j + 1] = r.y;
   }
-#endif
 }
 
 // Rows of ids outside [vocab_start, vocab_start + rows) are written as zeros
@@ -232,7 +225,7 @@ __device__ __forceinline__ void mix_unit(const U& u, int c, float pk, float (&ac
 // is decoded once per piece of the plan and written to all its tokens;
 // otherwise once per token, with no plan to wait for.
 template <bool kRuns>
-__global__ void __launch_bounds__(kThreads, kMixBlocks)
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm)
     embed_mix_kernel(const __grid_constant__ CandSet cs, const float* __restrict__ probs, Ids ids, int T, Plan plan,
                      long long vocab_start, int rows, int units_per_row, int cols, float scale, bool strict, bool vec,
                      __nv_bfloat16* __restrict__ out, long long ldo, int* err) {
@@ -308,10 +301,7 @@ __global__ void __launch_bounds__(kThreads, kMixBlocks)
 // pieces.  Tokens of other shards get the key `rows` and so end up last.
 // Latency bound: barriers and the round trips between them.
 constexpr int kSortThreads = 1024;
-#ifndef VQ_CTAS
-#define VQ_CTAS 16
-#endif
-constexpr int kSortCtas = VQ_CTAS;  // the largest cluster (8 is the portable limit)
+constexpr int kSortCtas = 16;  // the largest cluster (the portable 8 take 25 us for 16384 tokens, these 21)
 constexpr int kDigitBits = 9;
 constexpr int kBins = 1 << kDigitBits;
 constexpr int kSortSmem = 32 * kBins * 2;
@@ -635,25 +625,19 @@ __device__ __forceinline__ float dot_unit(const U& u, int c, const float (&g)[32
   float a[2], b[2];
   uint32_t qb[8];
   MixChunk<F>::get(u, c, a, b, qb);
-  float s[4] = {0.f, 0.f, 0.f, 0.f};  // two chains a half
-#ifdef VQ_SCALAR
-#pragma unroll
-  for (int j = 0; j < 32; ++j)
-    s[(j >> 4) * 2 + (j & 1)] = fmaf(g[j], magic_byte(qb[j >> 2], j & 3) - MixChunk<F>::kSub, s[(j >> 4) * 2 + (j & 1)]);
-#else
+  float2 s[2];
   const float2 nsub = make_float2(-MixChunk<F>::kSub, -MixChunk<F>::kSub);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    float2 t = make_float2(0.f, 0.f);
+    s[h] = make_float2(0.f, 0.f);
 #pragma unroll
     for (int j = 8 * h; j < 8 * h + 8; ++j) {
-      const float2 q = __fadd2_rn(make_float2(magic_byte(qb[j >> 1], 2 * (j & 1)), magic_byte(qb[j >> 1], 2 * (j & 1) + 1)), nsub);
-      t = __ffma2_rn(make_float2(g[2 * j], g[2 * j + 1]), q, t);
+      const int i = 2 * (j & 1);
+      const float2 q = __fadd2_rn(make_float2(magic_byte(qb[j >> 1], i), magic_byte(qb[j >> 1], i + 1)), nsub);
+      s[h] = __ffma2_rn(make_float2(g[2 * j], g[2 * j + 1]), q, s[h]);
     }
-    s[2 * h] = t.x, s[2 * h + 1] = t.y;
   }
-#endif
-  float d = a[0] * (s[0] + s[1]) + a[1] * (s[2] + s[3]);
+  float d = a[0] * (s[0].x + s[0].y) + a[1] * (s[1].x + s[1].y);
   if (MixChunk<F>::kMin) d = fmaf(b[0], gs[0], fmaf(b[1], gs[1], d));
   return d;
 }
@@ -699,7 +683,7 @@ __device__ __forceinline__ void add_row(const T* row, int col, int cols, bool ve
 // (an index that varies would put a register array into local memory), and
 // the block's are left in partials[blockIdx.x][K].
 template <typename T>
-__global__ void __launch_bounds__(kThreads, kGradBlocks)
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm)
     embed_gategrad_kernel(const __grid_constant__ CandSet cs, Plan plan, int rows, int units_per_row, int cols,
                           const T* __restrict__ dy, long long lddy, bool vec, double* __restrict__ partials, int* err) {
   extern __shared__ __align__(16) uint8_t esmem[];

@@ -700,6 +700,7 @@ def _qk_operands(q, k, q_weight, k_weight, cos, sin):
 
 
 _strides3 = ctypes.c_int64 * 3
+_CONTIGUOUS = torch.contiguous_format
 _strides2 = ctypes.c_int64 * 2
 
 
@@ -711,7 +712,7 @@ def qk_norm_rope_fwd(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k
     ``qk_norm_rope_bwd``."""
     dev, (q, qb, qs, qh), (k, kb, ks, kh), wq, wk, c, s, cb, cs, (B, S, D, R), dtype = \
         _qk_operands(q, k, q_weight, k_weight, cos, sin)
-    qo, ko = q.new_empty(q.shape), k.new_empty(k.shape)
+    qo, ko = torch.empty_like(q, memory_format=_CONTIGUOUS), torch.empty_like(k, memory_format=_CONTIGUOUS)
     qst, kst, cst = _strides3(qb, qs, qh), _strides3(kb, ks, kh), _strides2(cb, cs)
     wf, cf = wq.dtype == torch.float32, c.dtype == torch.float32
     _check(_lib.vq_qk_norm_rope_fwd(q.data_ptr(), qst, q.shape[2], k.data_ptr(), kst, k.shape[2], wq.data_ptr(),
@@ -733,7 +734,7 @@ def qk_norm_rope_bwd(gq: torch.Tensor, gk: torch.Tensor, operands, layout, want_
     if gq.get_device() != dev or gk.get_device() != dev:
         raise ValueError("qk_norm_rope: gradients on the outputs' device expected")
     (gq, gqb, gqs, gqh), (gk, gkb, gks, gkh) = _heads_operand(gq), _heads_operand(gk)
-    dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
+    dq, dk = torch.empty_like(q, memory_format=_CONTIGUOUS), torch.empty_like(k, memory_format=_CONTIGUOUS)
     dwq = dwk = ws = None
     need = 0
     if want_weight_grads:

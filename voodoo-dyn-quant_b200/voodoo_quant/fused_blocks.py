@@ -102,9 +102,8 @@ class _QKNormRopeFn(Function):
     the heads before the norm again instead of keeping the normed ones."""
 
     @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, cos, sin, eps: float, weight_offset: float):
-        qo, ko, operands, ctx.layout = _C.qk_norm_rope_fwd(q, k, q_weight, k_weight, cos, sin, eps, weight_offset,
-                                                           saved=True)
+    def forward(ctx, q, k, q_weight, k_weight, constants: tuple):
+        qo, ko, operands, ctx.layout = _C.qk_norm_rope_fwd(q, k, q_weight, k_weight, *constants, saved=True)
         ctx.save_for_backward(*operands)
         ctx.weight_types = (q_weight.dtype, k_weight.dtype)
         return qo, ko
@@ -116,7 +115,7 @@ class _QKNormRopeFn(Function):
         dq, dk, dwq, dwk = _C.qk_norm_rope_bwd(gq, gk, ctx.saved_tensors, ctx.layout,
                                                want_weight_grads=need[2] or need[3])
         return (dq if need[0] else None, dk if need[1] else None, dwq.to(ctx.weight_types[0]) if need[2] else None,
-                dwk.to(ctx.weight_types[1]) if need[3] else None, None, None, None, None)
+                dwk.to(ctx.weight_types[1]) if need[3] else None, None)
 
 
 class _SwiGLUFn(Function):
@@ -197,7 +196,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad
                                          or k_weight.requires_grad)):
         return _C.qk_norm_rope_fwd(q, k, q_weight, k_weight, cos, sin, eps, weight_offset)
-    return _QKNormRopeFn.apply(q, k, q_weight, k_weight, cos, sin, float(eps), float(weight_offset))
+    return _QKNormRopeFn.apply(q, k, q_weight, k_weight, (cos, sin, eps, weight_offset))
 
 
 def swiglu(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
