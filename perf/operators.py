@@ -344,6 +344,8 @@ def _plain_clip(st):
 
 # ------------------------------------------------------------------ the framework's calls
 def _package():
+    if "voodoo_quant" in sys.modules:
+        return
     p = str(Path("voodoo-dyn-quant_b200").resolve())
     if p not in sys.path:
         sys.path.insert(0, p)
