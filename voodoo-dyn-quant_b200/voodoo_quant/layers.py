@@ -14,6 +14,9 @@ assignment after training.  What changes is where the work happens:
   g_k = <dY^T X, W_k> in the dW GEMM's epilogue without materialising dW.
   Autograd then applies the softmax Jacobian to reach the gates, exactly as
   in the reference (``_MixedWeightFunction.backward``, :355-363).
+* Embedding: ``vq_embed_mix`` looks the tokens' mixed rows up in the packed
+  blocks, ``vq_embed_gategrad`` reduces their gate gradients
+  (``gated_embedding``; reference ``_MixedEmbeddingRowFunctionLazy``, :670-750).
 
 The candidate cache on disk keeps the reference format and paths
 (``_combined_cache_path``, ``_tensor_hash``, :884-943): a ``combined_lazy``
@@ -80,9 +83,10 @@ def set_ptqr(enabled: bool) -> None:
 class _StaticState:
     """Static-shape mode (off by default): no host round trip and no
     data-dependent shape in the step's host code, so that the whole forward
-    and backward can be recorded as one CUDA graph.  Embedding lookups then
-    decode one row per token, repeats included, instead of the unique rows
-    (``torch.unique`` reads its output size on the host); a vocabulary shard
+    and backward can be recorded as one CUDA graph.  The GPU's fused embedding
+    lookup needs none either way; the routed lookup (PTQR) then
+    decodes one row per token, repeats included, instead of the unique rows
+    (``torch.unique`` reads its output size on the host); its vocabulary shard
     looks every token up at a clamped row and zeroes the rows that belong to
     other shards instead of gathering its own tokens (boolean indexing).
     Values are unchanged: the gated embedding's backward is a dot product per
