@@ -115,6 +115,17 @@ def test_lookup_and_gradient_against_64_bits(cuda, T, V, D, types, scale, start,
 @pytest.mark.parametrize("T,rows", [(1, 1), (5, 3), (1024, 511), (1025, 512), (4097, 70000), (16384, 151936), (20000, 200),
                                     (70001, 151936)])
 def test_plan_is_a_stable_sort_in_pieces(cuda, T, rows):
+    _check_plan(cuda, T, rows)
+
+
+@pytest.mark.parametrize("T", [1, 1000, 1025, 4500])
+@pytest.mark.parametrize("rows", [(1 << 27) - 1, 1 << 27, 1 << 30])
+def test_plan_of_the_most_rows(cuda, T, rows):
+    """The last sizes of three digits of nine bits, and four digits."""
+    _check_plan(cuda, T, rows)
+
+
+def _check_plan(cuda, T, rows):
     from voodoo_quant import _C
 
     g = torch.Generator(device="cpu").manual_seed(T)

@@ -365,8 +365,8 @@ __global__ void __launch_bounds__(kSortThreads) token_plan_block_kernel(Ids ids,
     const int i = first + 32 * r;
     idx[r] = i;
     const long long row = i < T ? local_row(ids.at(i), vocab_start, rows) : -1;
-    // places past the end sort behind everything (the sort is stable)
-    key[r] = i >= T ? (1 << (kDigitBits * passes)) - 1 : row < 0 ? rows : static_cast<int>(row);
+    // places past the end sort behind everything (the sort is stable): all bits of the passes set
+    key[r] = i >= T ? 0x7fffffff : row < 0 ? rows : static_cast<int>(row);
   }
   for (int p = 0; p < passes; ++p) {
     const int shift = p * kDigitBits;
