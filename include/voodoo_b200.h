@@ -52,7 +52,8 @@ int vq_format_info(int ggml_type, int* block_elems /* host */, int* block_bytes 
 /* Synchronise `stream`, then return and clear the device error word in *code
  * (host): 0 = none; (1 << 16 | where) = an mbarrier wait gave up after its
  * time limit; (2 << 16) = a kernel met an unknown format; (4 << 16 | where) =
- * a lookup met a token id outside its table. */
+ * a lookup met a token id outside its table; (5 << 16 | where) = a plan made
+ * for another number of tokens or rows. */
 int vq_device_error(void* stream, int* code /* host */);
 
 /* K0 -- bit-exact dequantisation of one packed candidate into float32
@@ -355,9 +356,10 @@ int vq_qk_norm_rope_bwd(const void* gq, const int64_t* gq_strides, const void* g
 /* ---- gated embedding ----
  * Plan of T token ids (int64, or int32 when ids_i32) over a table of `rows` rows that holds the vocabulary from
  * vocab_start on: the tokens in the order of their rows (stable; ids outside the table last), cut into pieces of equal
- * rows and at most 8 tokens (one begins at every 1024th place).  `plan` (vq_embed_plan_bytes(T), 16-byte aligned) holds int32: the number of pieces P
- * at byte 0; order[T] from byte 256; then, each from a multiple of 256 bytes, start[P] with T behind the last, and
- * the pieces' rows key[P] (`rows` for ids outside the table). */
+ * rows and at most 8 tokens (one begins at every 1024th place).  `plan` (vq_embed_plan_bytes(T), 16-byte aligned)
+ * holds int32: the number of pieces P, T and `rows` at byte 0; order[T] from byte 256; then, each from a multiple of
+ * 256 bytes, start[P] with T behind the last, and the pieces' rows key[P] (`rows` for ids outside the table).  A
+ * lookup or gradient of another T or `rows` reports the plan (vq_device_error) and takes no token of it. */
 size_t vq_embed_plan_bytes(int64_t T);
 int vq_embed_plan(const void* ids, int ids_i32, int64_t T, int64_t vocab_start, int64_t rows, void* plan,
                   size_t plan_bytes, void* stream);

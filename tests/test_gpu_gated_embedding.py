@@ -145,7 +145,7 @@ def _check_plan(cuda, T, rows):
         P = int(plan[0])
         second = 64 + step
         third = second + (4 * (T + 1) + 255) // 256 * 64
-        assert P == at.numel()
+        assert P == at.numel() and plan[1] == T and plan[2] == rows
         assert torch.equal(plan[64:64 + T], order)
         assert torch.equal(plan[second:second + P], at) and plan[second + P] == T
         assert torch.equal(plan[third:third + P], want[at])
@@ -194,6 +194,25 @@ def test_ids_outside_the_table(cuda):
     dy[1] = float("nan")  # of an id that is not in the table
     grad = _C.embed_gategrad(dy.to(cuda), table, plan)
     _check_grad(grad, dy, ids, dec, 1.0, 0, V)
+
+
+def test_a_plan_of_other_tokens_or_rows_is_reported(cuda):
+    """Plans whose size alone does not tell them apart: nothing is read or written by them."""
+    from voodoo_quant import _C
+
+    types = ["Q5_K", "Q3_K"]
+    V, D = 40, 256
+    _, _, blocks, _, p = _table(V, D, types, 4, cuda)
+    table = _C.EmbedTable(types, blocks, V, D, D)
+    ids = torch.arange(20).to(cuda)
+    dy = torch.ones(20, D, dtype=torch.bfloat16, device=cuda)
+    assert _C.device_error() == 0
+    for plan in (_C.embed_plan(torch.arange(25).to(cuda), V), _C.embed_plan(torch.arange(19).to(cuda), V),
+                 _C.embed_plan(ids, V + 100)):
+        _C.embed_mix(ids, table, p.to(cuda), plan=plan)
+        assert _C.device_error() == (5 << 16 | 31)
+        assert not _C.embed_gategrad(dy, table, plan).any()
+        assert _C.device_error() == (5 << 16 | 31) and _C.device_error() == 0
 
 
 def test_strided_gradients_and_multidimensional_ids(cuda):

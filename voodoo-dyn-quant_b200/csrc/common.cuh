@@ -21,6 +21,7 @@ enum DeviceError : int {
   kDevBadFormat = 2,    // unknown block format reached a kernel
   kDevBadSmemAlign = 3, // dynamic shared memory not 1024-byte aligned
   kDevBadIndex = 4,     // a token id outside the table of a lookup
+  kDevBadPlan = 5,      // a lookup met a plan of other tokens or rows
 };
 
 // Every spin on an mbarrier gives up after this long, records

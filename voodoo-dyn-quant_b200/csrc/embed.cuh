@@ -139,7 +139,19 @@ __device__ __forceinline__ long long local_row(long long id, long long vocab_sta
 // place of the order (a tile of the sort, which then needs no carry from the
 // one before) and kPieceTokens after the piece before it.
 struct Plan {
-  int *order, *start, *key, *count;
+  int *order, *start, *key, *count;  // count[1], count[2]: the tokens and rows that the plan was made for
+
+  __device__ __forceinline__ void finish(int pieces, int tokens, int rows) const {
+    start[pieces] = tokens;
+    *reinterpret_cast<int4*>(count) = make_int4(pieces, tokens, rows, 0);
+  }
+  // Pieces to walk; none where the plan is not one of these tokens and rows.
+  __device__ __forceinline__ int pieces(int tokens, int rows, int* err) const {
+    const int4 h = *reinterpret_cast<const int4*>(count);
+    if (h.y == tokens && h.z == rows) return h.x;  // its places and keys lie in what this call reads and writes
+    report_error(err, kDevBadPlan, 31);
+    return 0;
+  }
 };
 
 // Most tokens of a piece: a token that fills much of a batch is then worked
@@ -236,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int lu = lane >> 3, c = lane & 7;
   uint8_t* buf = esmem + warp * warp_bytes(cs);
-  UnitWalk<kRuns> w{plan, ids, kRuns ? *plan.count : T, vocab_start, rows, units_per_row};
+  UnitWalk<kRuns> w{plan, ids, kRuns ? plan.pieces(T, rows, err) : T, vocab_start, rows, units_per_row};
   w.start_at((static_cast<long long>(blockIdx.x) * kWarps + warp) * kUnits + lu,
              static_cast<long long>(gridDim.x) * kWarps * kUnits);
   bool bad = false;
@@ -450,8 +462,7 @@ __global__ void __launch_bounds__(kSortThreads) token_plan_block_kernel(Ids ids,
     at += __popc(starts[r]);
   }
   if (tid == 0) {
-    plan.start[all] = T;
-    *plan.count = all;
+    plan.finish(all, T, rows);
   }
 }
 
@@ -613,8 +624,7 @@ __global__ void __launch_bounds__(kSortThreads) token_plan_kernel(Ids ids, int T
     if (b + t * kSortThreads < e) write_starts(b + t * kSortThreads + tid, kept[t]);
   for (int i0 = b + kKeepTiles * kSortThreads; i0 < e; i0 += kSortThreads) write_starts(i0 + tid, starts_of(i0 + tid));
   if (rank == 0 && tid == 0) {
-    plan.start[all] = T;
-    *plan.count = all;
+    plan.finish(all, T, rows);
   }
   cluster_sync();  // nobody reads this CTA's shared memory any more
 }
@@ -684,15 +694,16 @@ __device__ __forceinline__ void add_row(const T* row, int col, int cols, bool ve
 // the block's are left in partials[blockIdx.x][K].
 template <typename T>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
-    embed_gategrad_kernel(const __grid_constant__ CandSet cs, Plan plan, int rows, int units_per_row, int cols,
-                          const T* __restrict__ dy, long long lddy, bool vec, double* __restrict__ partials, int* err) {
+    embed_gategrad_kernel(const __grid_constant__ CandSet cs, Plan plan, int tokens, int rows, int units_per_row,
+                          int cols, const T* __restrict__ dy, long long lddy, bool vec, double* __restrict__ partials,
+                          int* err) {
   extern __shared__ __align__(16) uint8_t esmem[];
   double* acc = reinterpret_cast<double*>(esmem);  // [K][kThreads]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int lu = lane >> 3, c = lane & 7;
   uint8_t* buf = esmem + cs.K * kThreads * sizeof(double) + warp * warp_bytes(cs);
   for (int k = 0; k < cs.K; ++k) acc[k * kThreads + threadIdx.x] = 0.0;
-  UnitWalk<true> w{plan, Ids{nullptr, false}, *plan.count, 0, rows, units_per_row};
+  UnitWalk<true> w{plan, Ids{nullptr, false}, plan.pieces(tokens, rows, err), 0, rows, units_per_row};
   w.start_at((static_cast<long long>(blockIdx.x) * kWarps + warp) * kUnits + lu,
              static_cast<long long>(gridDim.x) * kWarps * kUnits);
   for (;; w.step()) {

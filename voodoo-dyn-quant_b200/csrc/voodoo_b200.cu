@@ -1440,8 +1440,8 @@ int launch_embed_gategrad(const vq::CandSet& cs, const vq::embed::Plan& plan, lo
   const int smem = cs.K * kThreads * static_cast<int>(sizeof(double)) + kWarps * warp_bytes(cs);
   if (int rc = one_wave(embed_gategrad_kernel<T>, smem, tokens * upr, blocks)) return rc;
   const bool vec = aligned16(dy) && lddy * sizeof(T) % 16 == 0;
-  embed_gategrad_kernel<T><<<*blocks, kThreads, smem, st>>>(cs, plan, static_cast<int>(rows), upr, cols,
-                                                            static_cast<const T*>(dy), lddy, vec, partials, err);
+  embed_gategrad_kernel<T><<<*blocks, kThreads, smem, st>>>(cs, plan, static_cast<int>(tokens), static_cast<int>(rows), upr,
+                                                            cols, static_cast<const T*>(dy), lddy, vec, partials, err);
   VQ_CUDA(cudaGetLastError());
   return 0;
 }
