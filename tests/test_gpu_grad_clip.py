@@ -62,6 +62,9 @@ CASES = [
     ([(1,)], [BF16]),
     ([(3,), (0,), (5, 7), ()], [F16]),
     ([(16384,)], [F32]),
+    ([(4096,)], [F32]),
+    ([(4097,)], [F32]),
+    ([(255,), (256,), (257,), (1,), (2000,), (512,), (513,)], [BF16, F32, F16]),
     ([(16385,)], [F32]),
     ([(257, 129), (8191,), (8192,), (8193,), (1,), (100003,)], [BF16]),
     ([(n,) for n in range(1, 60)], [F32, BF16, F16]),

@@ -26,6 +26,7 @@ constexpr int kVecs = kChunkBytes / (16 * kThreads);
 // 4, 490 with 1).
 constexpr int kBlocksPerSm = 4, kScaleBlocksPerSm = 3;
 constexpr int kSmallThreads = 1024;
+constexpr int kSmallChunkBytes = 512;
 constexpr int kMaxBlocks = 1024;  // of one launch: the partials it leaves
 
 enum DType : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
@@ -282,27 +283,34 @@ __global__ void __launch_bounds__(kThreads, kScaleBlocksPerSm)
 }
 
 // Few values in all: one block takes the norm and scales, in one launch.  A
-// warp per tensor, since such tensors (a layer's gates) hold a few values.
+// warp per piece of kSmallChunkBytes of a tensor: tensors of a few values (a
+// layer's gates) take a warp each, one of some thousand is spread over all.
+template <int N, class Op>
+__device__ __forceinline__ void small_pieces(const Table<N>& tab, Op op) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int c = warp; c < tab.chunks; c += kSmallThreads / 32) {
+    const int t = tab.chunks == tab.n ? c : tensor_of(tab, c);
+    const int dt = tab.dtype[t], es = esize(dt);
+    const long long at = static_cast<long long>(c - tab.first_chunk[t]) * kSmallChunkBytes;
+    const long long left = tab.bytes[t] - at;
+    const uintptr_t b = tab.ptr[t] + static_cast<uintptr_t>(at);
+    const uintptr_t e = b + static_cast<uintptr_t>(left < kSmallChunkBytes ? left : kSmallChunkBytes);
+#pragma unroll 4
+    for (uintptr_t a = b + lane * es; a < e; a += 32 * es) op(a, dt);
+  }
+}
+
 template <int N, bool kMax>
 __global__ void __launch_bounds__(kSmallThreads) small_kernel(const __grid_constant__ Table<N> tab, float max_norm,
                                                               bool scale, float* __restrict__ norm_out) {
   __shared__ double red[kSmallThreads / 32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   double acc = 0.0;
-  for (int t = warp; t < tab.n; t += kSmallThreads / 32) {
-    const int dt = tab.dtype[t], es = esize(dt);
-    const uintptr_t e = tab.ptr[t] + static_cast<uintptr_t>(tab.bytes[t]);
-    for (uintptr_t a = tab.ptr[t] + lane * es; a < e; a += 32 * es) acc = join<kMax>(acc, one<kMax>(load_one(a, dt)));
-  }
+  small_pieces(tab, [&](uintptr_t a, int dt) { acc = join<kMax>(acc, one<kMax>(load_one(a, dt))); });
   float norm;
   const float s = clip_scale(block_join<kMax>(acc, red), kMax, max_norm, &norm);
   if (threadIdx.x == 0 && norm_out != nullptr) *norm_out = norm;
   if (!scale || s == 1.f) return;
-  for (int t = warp; t < tab.n; t += kSmallThreads / 32) {
-    const int dt = tab.dtype[t], es = esize(dt);
-    const uintptr_t e = tab.ptr[t] + static_cast<uintptr_t>(tab.bytes[t]);
-    for (uintptr_t a = tab.ptr[t] + lane * es; a < e; a += 32 * es) store_one(a, dt, load_one(a, dt) * s);
-  }
+  small_pieces(tab, [&](uintptr_t a, int dt) { store_one(a, dt, load_one(a, dt) * s); });
 }
 
 }  // namespace clip
