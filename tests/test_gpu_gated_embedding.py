@@ -256,12 +256,13 @@ def test_unaligned_blocks(cuda):
             assert torch.equal(_C.embed_mix(ids.to(cuda), _C.EmbedTable([qt], [b], V, D, D), one), want)
 
 
-def test_streams_graphs_and_repeats(cuda):
+@pytest.mark.parametrize("T", [3000, 5000])  # a plan by one block, and by a cluster
+def test_streams_graphs_and_repeats(cuda, T):
     """Two captured graphs, replayed one after the other and on two streams at once, give the eager calls' bits."""
     from voodoo_quant import _C
 
     types = ["Q3_K", "Q4_K", "Q8_0"]
-    V, D, T = 500, 768, 3000
+    V, D = 500, 768
     _, _, blocks, dec, p = _table(V, D, types, 8, cuda)
     sets = [(_ids(T, V, s).to(cuda), torch.randn(T, D, generator=torch.Generator().manual_seed(s)).to(torch.bfloat16).to(cuda))
             for s in (1, 2)]
@@ -331,3 +332,26 @@ def test_module_uses_the_fused_lookup(cuda):
     q8 = _C.dequant(teacher.emb.qweight, "Q8_0", V, D).double().cpu()
     _check_lookup(teacher.emb(ids), ids.cpu(), [q8], torch.ones(1), scale, 0, V)
     assert (q8 - weight.double().cpu()).abs().max() < 0.02 * float(weight.abs().max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.float32, torch.float16])
+def test_module_returns_its_sources_type(cuda, dtype):
+    """The values are the mixture's in bfloat16, whatever the source's type."""
+    import torch.nn as nn
+
+    from voodoo_quant import _C
+    from voodoo_quant.layers import replace_embedding_with_mixed_quant
+    from voodoo_quant.training.synthetic import rtn_candidate_provider
+
+    types = ["Q4_K", "Q8_0"]
+    V, D = 40, 256
+    m = nn.Module()
+    m.emb = nn.Embedding(V, D, device=cuda, dtype=dtype)
+    replace_embedding_with_mixed_quant(m, types, candidate_provider=rtn_candidate_provider)
+    ids = _ids(21, V, 3).to(cuda)
+    out = m.emb(ids)
+    assert out.dtype == dtype
+    dec = [_C.dequant(b, q, V, D).double().cpu() for q, b in zip(types, m.emb._candidate_blocks())]
+    _check_lookup(out.detach(), ids.cpu(), dec, torch.tensor([0.5, 0.5]), 1.0, 0, V)
+    out.sum().backward()
+    assert m.emb.gates.grad.shape == (2,) and m.emb.gates.grad.any()

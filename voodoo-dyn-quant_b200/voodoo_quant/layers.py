@@ -739,6 +739,9 @@ def _embedding_rows(probs, ids, table, scale, vocab_start, dtype, plan=None):
     return out if dtype == torch.bfloat16 else out.to(dtype)
 
 
+_ROW_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
 def gated_embedding(ids: torch.Tensor, probs: torch.Tensor, candidate_types, candidate_blocks, num_embeddings: int,
                     embedding_dim: int, scale: float = 1.0, vocab_start: int | None = None,
                     dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -749,7 +752,7 @@ def gated_embedding(ids: torch.Tensor, probs: torch.Tensor, candidate_types, can
     ``vocab_start``: the table is the vocabulary shard of ``num_embeddings`` rows from there on; tokens of other shards
     get zeros and add nothing to the gradient.  Without it every id must be a row of the table: another one gets zeros
     and sets the device error word (``_C.device_error``)."""
-    if dtype not in (torch.float32, torch.bfloat16, torch.float16):
+    if dtype not in _ROW_TYPES:
         raise ValueError(f"gated_embedding: float32, bfloat16 or float16 rows, got {dtype}")
     if vocab_start is not None and vocab_start < 0:
         raise ValueError(f"gated_embedding: vocab_start {vocab_start} is negative")
@@ -1077,8 +1080,11 @@ class MixedQuantEmbedding(_MixedQuantBase):
 
     def _fused_lookup(self, ids: torch.Tensor, vocab_start: int | None = None) -> torch.Tensor:
         dev = self._cand_arena.device
-        return gated_embedding(ids.to(dev), self.get_probs().to(dev), self.candidate_types, self._candidate_blocks(),
-                               self.num_embeddings, self.embedding_dim, self.scale, vocab_start, self.source_dtype)
+        # rows in the source's type; a type that the lookup has no rows of (float64) is cast to
+        dtype = self.source_dtype if self.source_dtype in _ROW_TYPES else torch.float32
+        rows = gated_embedding(ids.to(dev), self.get_probs().to(dev), self.candidate_types, self._candidate_blocks(),
+                               self.num_embeddings, self.embedding_dim, self.scale, vocab_start, dtype)
+        return rows if dtype == self.source_dtype else rows.to(self.source_dtype)
 
     def _embedding_lookup(self, ids: torch.Tensor) -> torch.Tensor:
         e = self._rows_lookup(ids)
