@@ -191,3 +191,46 @@ def test_head_norm_models_build_and_fuse_on_cpu():
     x = torch.randint(0, shape.vocab, (1, 16))
     with torch.no_grad():
         assert torch.equal(a(input_ids=x, use_cache=False).logits, b(input_ids=x, use_cache=False).logits)
+
+
+def _windowed_decoder(window):
+    from transformers import Qwen3Config, Qwen3ForCausalLM
+
+    cfg = Qwen3Config(vocab_size=64, hidden_size=32, intermediate_size=48, num_hidden_layers=2, num_attention_heads=2,
+                      num_key_value_heads=1, head_dim=16, use_sliding_window=True, sliding_window=window,
+                      max_window_layers=1, max_position_embeddings=64)
+    cfg._attn_implementation = "sdpa"
+    assert ("sliding_attention" in cfg.layer_types) == (window is not None)
+    torch.manual_seed(3)
+    return Qwen3ForCausalLM(cfg)
+
+
+def test_attention_windows_are_not_dropped(monkeypatch):
+    """The paths that pass no mask to the layers refuse a window shorter than the batch, or are not taken."""
+    pytest.importorskip("transformers")
+    from types import SimpleNamespace
+
+    from voodoo_quant import fused_blocks, parallel
+    from voodoo_quant.training.trainer import GatedDistillTrainer, StepArgs
+
+    model = _windowed_decoder(8)
+    assert fused_blocks.windowed(model.model.layers, 9) and not fused_blocks.windowed(model.model.layers, 8)
+    assert fused_blocks.windowed(model.model.layers)
+    fused_blocks.use_sequence_parallel(model)
+    x = torch.randint(0, 64, (1, 12))
+    with torch.no_grad():
+        want = _windowed_decoder(8)(input_ids=x, use_cache=False).logits
+        assert torch.equal(model(input_ids=x, use_cache=False).logits, want)  # off: the model's own forward
+        monkeypatch.setattr(parallel, "sp_enabled", lambda: True)
+        with pytest.raises(ValueError, match="no window"):
+            model.model(input_ids=x)
+    monkeypatch.setattr(parallel, "sp_enabled", lambda: False)
+    plain = _windowed_decoder(None)
+
+    def joint(student, teacher):
+        t = SimpleNamespace(args=StepArgs(joint_teacher=True), tp=True, _tsplit=(0, 0, 0, 1), student=student,
+                            teacher=teacher)
+        return GatedDistillTrainer._joint_ok(t)
+
+    assert joint(plain, plain)
+    assert not joint(model, plain) and not joint(plain, model)

@@ -22,6 +22,7 @@ other dtypes or devices) runs the module's original forward unchanged.
 
 from __future__ import annotations
 
+import math
 import types
 
 import torch
@@ -240,6 +241,14 @@ def _head_norms_fusable(attn, hidden_states: torch.Tensor) -> bool:
     return (attn.head_dim <= 512 and attn.q_norm.variance_epsilon == attn.k_norm.variance_epsilon
             and (window is None or hidden_states.shape[1] <= window)
             and not (attn.training and getattr(attn, "attention_dropout", 0.0)))
+
+
+def windowed(layers, length: float = math.inf) -> bool:
+    """Whether any decoder layer's attention window is shorter than sequences
+    of ``length``: such layers need the mask that the model's own forward
+    builds."""
+    windows = (getattr(getattr(layer, "self_attn", None), "sliding_window", None) for layer in layers)
+    return any(w is not None and length > w for w in windows)
 
 
 def _attention_forward(self, hidden_states: torch.Tensor, position_embeddings=None, attention_mask=None,
@@ -462,6 +471,9 @@ def _sp_model_forward(self, input_ids=None, attention_mask=None, position_ids=No
             attention_mask is not None:
         raise ValueError("sequence parallelism runs whole causal batches from input_ids only "
                          "(no attention mask, cache or inputs_embeds)")
+    if windowed(self.layers[: self.config.num_hidden_layers], input_ids.shape[1]):
+        raise ValueError("sequence parallelism runs attention over whole sequences only (no window shorter than "
+                         f"the batch's {input_ids.shape[1]} positions)")
     e = self.embed_tokens(input_ids)
     B, S, H = e.shape
     h = sp_scatter(e.reshape(B * S, H))

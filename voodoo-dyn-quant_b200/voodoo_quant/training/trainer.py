@@ -235,14 +235,18 @@ class GatedDistillTrainer:
     def _joint_ok(self) -> bool:
         """Whether this step interleaves the teacher with the student
         (StepArgs.joint_teacher; TP with a TP-1 teacher on the rank's batch
-        slice, the plain loss path, no sequence parallelism)."""
+        slice, the plain loss path, no sequence parallelism, no attention
+        windows, whose mask only the models' own forward builds)."""
+        from voodoo_quant.fused_blocks import windowed
         from voodoo_quant.parallel import sp_enabled
 
         a = self.args
         return (a.joint_teacher and self.tp and self._tsplit is not None and self._tsplit[3] == 1
                 and a.logits_chunk <= 0 and not sp_enabled()
                 and hasattr(getattr(self.student, "model", None), "layers")
-                and hasattr(getattr(self.teacher, "model", None), "layers"))
+                and hasattr(getattr(self.teacher, "model", None), "layers")
+                and not windowed(self.student.model.layers)
+                and not windowed(self.teacher.model.layers))
 
     def _joint_forward(self, x: torch.Tensor):
         """Student logits (autograd) and teacher logits (no grad, in the
