@@ -200,6 +200,23 @@ def test_shared_memory_is_refused(cuda):
 
 
 @pytest.mark.parametrize("n", [6, 30000])
+def test_a_graph_that_saved_a_gradient_notices(cuda, n):
+    """As after any other change in place: the backward of what was computed from the gradients before they were scaled
+    raises; taking the norm alone changes nothing."""
+    from voodoo_quant.training.grad_clip import clip_grad_norm_, grad_norm
+
+    p = torch.nn.Parameter(torch.ones(n, device=cuda))
+    (p.grad,) = torch.autograd.grad((p ** 3).sum(), p, create_graph=True)
+    penalty = (p.grad ** 2).sum()
+    grad_norm([p.grad])
+    (g,) = torch.autograd.grad(penalty, p, retain_graph=True)
+    assert torch.equal(g, torch.full_like(g, 36.0))  # d(3 p^2)^2 / dp = 36 p^3
+    clip_grad_norm_([p], 1e-3)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(penalty, p)
+
+
+@pytest.mark.parametrize("n", [6, 30000])
 def test_streams_graphs_and_repeats(cuda, n):
     from voodoo_quant.training.grad_clip import clip_grad_norm_
 

@@ -12,6 +12,7 @@ failures raise ``RuntimeError``.
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 from array import array
 from operator import attrgetter
@@ -875,6 +876,8 @@ def clip_grad_norm(tensors, max_norm: float = float("inf"), norm_inf: bool = Fal
         array("i", [_FLOAT_CODE[t.dtype] for t in tensors])
     ptrs = array("Q", map(torch.Tensor.data_ptr, tensors))
     sizes = array("q", map(_nbytes_of, tensors))
+    if max_norm != math.inf:  # a graph that has saved one of them must notice
+        torch.autograd.graph.increment_version(tensors)
     device = tensors[0].device
     norm = torch.empty((), dtype=torch.float32, device=device)
     need = _lib.vq_clip_grad_norm_workspace_bytes(n)
