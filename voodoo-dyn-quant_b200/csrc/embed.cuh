@@ -247,7 +247,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
   __syncthreads();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int lu = lane >> 3, c = lane & 7;
-  uint8_t* buf = esmem + warp * warp_bytes(cs);
+  uint8_t* buf = esmem + kWarps * kUnits * 512 + warp * warp_bytes(cs);
+  uint4* rows_s = reinterpret_cast<uint4*>(esmem + (warp * kUnits + lu) * 512);
   UnitWalk<kRuns> w{plan, ids, kRuns ? plan.pieces(T, rows, err) : T, vocab_start, rows, units_per_row};
   w.start_at((static_cast<long long>(blockIdx.x) * kWarps + warp) * kUnits + lu,
              static_cast<long long>(gridDim.x) * kWarps * kUnits);
@@ -280,26 +281,40 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
       }
     }
     bad |= now.row < 0 && len > 0;
-    __align__(16) __nv_bfloat162 hv[16];
+    // Lane c holds columns 32 c to 32 c + 31 of the unit; written like that a
+    // store would touch half of each 32-byte sector.  By way of shared memory
+    // it gets columns 64 v + 8 c for v = 0..3, 128 bytes of the row a store.
+    uint4 hv[4];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float cs0 = cst[j >> 3];
-      const float x = acc[2 * j] + cs0, y = acc[2 * j + 1] + cs0;
-      hv[j] = scaled ? __floats2bfloat162_rn(x * scale, y * scale) : __floats2bfloat162_rn(x, y);
+    for (int v = 0; v < 4; ++v) {
+      __align__(16) __nv_bfloat162 h[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float cs0 = cst[v >> 1];
+        const float x = acc[8 * v + 2 * j] + cs0, y = acc[8 * v + 2 * j + 1] + cs0;
+        h[j] = scaled ? __floats2bfloat162_rn(x * scale, y * scale) : __floats2bfloat162_rn(x, y);
+      }
+      rows_s[c * 4 + (v ^ (c >> 1))] = *reinterpret_cast<const uint4*>(h);
     }
+    __syncwarp();
+#pragma unroll
+    for (int v = 0; v < 4; ++v) hv[v] = rows_s[v * 8 + (c & 4) + ((c & 3) ^ v)];
     const int most = kRuns ? __reduce_max_sync(0xffffffffu, len) : 1;
+    const int col0 = 256 * now.u + 8 * c;
     for (int i = 0; i < most; ++i) {
       const int tok = kRuns ? __shfl_sync(0xffffffffu, mine, (lane & 24) + i) : mine;
-      if (i >= len || col >= cols) continue;
-      __nv_bfloat16* dst = out + static_cast<long long>(tok) * ldo + col;
-      if (vec && col + 32 <= cols) {
+      if (i >= len) continue;
+      __nv_bfloat16* dst = out + static_cast<long long>(tok) * ldo + col0;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) reinterpret_cast<uint4*>(dst)[v] = reinterpret_cast<const uint4*>(hv)[v];
-      } else {
+      for (int v = 0; v < 4; ++v) {
+        const int left = cols - col0 - 64 * v;
+        if (vec && left >= 8) {
+          *reinterpret_cast<uint4*>(dst + 64 * v) = hv[v];
+        } else if (left > 0) {
+          const __nv_bfloat16* h = reinterpret_cast<const __nv_bfloat16*>(&hv[v]);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          if (col + 2 * j < cols) dst[2 * j] = hv[j].x;
-          if (col + 2 * j + 1 < cols) dst[2 * j + 1] = hv[j].y;
+          for (int j = 0; j < 8; ++j)
+            if (j < left) dst[64 * v + j] = h[j];
         }
       }
     }

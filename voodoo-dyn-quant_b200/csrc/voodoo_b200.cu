@@ -1520,7 +1520,7 @@ int vq_embed_mix(int K, const int* types, const void* const* blocks, const float
   int* err = nullptr;
   if (int rc = device_error_ptr(&err)) return rc;
   using namespace vq::embed;
-  const int smem = kWarps * warp_bytes(cs);
+  const int smem = kWarps * (kUnits * 512 + warp_bytes(cs));
   const int upr = static_cast<int>(padded_cols / 256);
   auto kern = plan != nullptr ? embed_mix_kernel<true> : embed_mix_kernel<false>;
   int grid = 0;
