@@ -136,6 +136,23 @@ struct URef {
   }
 };
 
+// The same of a unit that starts at an even byte, as every unit does whose
+// candidate's blocks are 2-byte aligned: single fields are read as they are.
+struct URefHalf {
+  const uint32_t* s;
+  int delta;  // 0 or 2
+  __device__ __forceinline__ uint32_t wq(int i, int extra = 0) const {
+    return __funnelshift_r(s[i], s[i + 1], 8 * delta + extra);
+  }
+  __device__ __forceinline__ const uint8_t* at(int off) const { return reinterpret_cast<const uint8_t*>(s) + delta + off; }
+  __device__ __forceinline__ uint32_t b16(int off) const { return *reinterpret_cast<const uint16_t*>(at(off)); }
+  __device__ __forceinline__ uint32_t b8(int off) const { return *at(off); }
+  __device__ __forceinline__ void wq8(int i, int extra, uint32_t (&q)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = wq(i + j, extra);
+  }
+};
+
 // The same of a unit that starts at a word (kVec: at a 16-byte vector) of
 // shared memory: no joining of words, and runs of words read as vectors.  The
 // bits that `extra` shifts in from the next word are zeros here; every field
@@ -144,8 +161,9 @@ template <bool kVec>
 struct URefAligned {
   const uint32_t* s;
   __device__ __forceinline__ uint32_t wq(int i, int extra = 0) const { return s[i] >> extra; }
-  __device__ __forceinline__ uint32_t b16(int off) const { return (s[off >> 2] >> (8 * (off & 3))) & 0xFFFFu; }
-  __device__ __forceinline__ uint32_t b8(int off) const { return (s[off >> 2] >> (8 * (off & 3))) & 0xFFu; }
+  __device__ __forceinline__ const uint8_t* at(int off) const { return reinterpret_cast<const uint8_t*>(s) + off; }
+  __device__ __forceinline__ uint32_t b16(int off) const { return *reinterpret_cast<const uint16_t*>(at(off)); }
+  __device__ __forceinline__ uint32_t b8(int off) const { return *at(off); }
   __device__ __forceinline__ void wq8(int i, int extra, uint32_t (&q)[8]) const {
     if (kVec) {
       const uint4 a = *reinterpret_cast<const uint4*>(s + i), b = *reinterpret_cast<const uint4*>(s + i + 4);
@@ -172,6 +190,21 @@ __device__ __forceinline__ void k4_scale_min_u(const U& u, int j, uint32_t& sc, 
   }
 }
 
+// The same without a branch, for lanes that hold different sub-blocks.
+template <class U>
+__device__ __forceinline__ void k4_scale_min_all(const U& u, int j, uint32_t& sc, uint32_t& mn) {
+  const uint32_t a = u.b8(4 + (j & 3)), b = u.b8(8 + (j & 3)), c = u.b8(12 + (j & 3));
+  sc = j < 4 ? a & 63u : (c & 15u) | ((a >> 2) & 48u);
+  mn = j < 4 ? b & 63u : (c >> 4) | ((b >> 2) & 48u);
+}
+__device__ __forceinline__ void k4_scale_min_u(const URefHalf& u, int j, uint32_t& sc, uint32_t& mn) {
+  k4_scale_min_all(u, j, sc, mn);
+}
+template <bool kVec>
+__device__ __forceinline__ void k4_scale_min_u(const URefAligned<kVec>& u, int j, uint32_t& sc, uint32_t& mn) {
+  k4_scale_min_all(u, j, sc, mn);
+}
+
 // Sub-block c (32 weights) of a unit as w = a[h] * q + b[h] (h = half of the
 // sub-block), with the codes q + kSub - 2^23 one per byte of qb.  The same
 // products, in the same order, as Chunk<F> (and so as the exact decoders up
@@ -183,7 +216,8 @@ template <>
 struct MixChunk<kQ8_0> {
   static constexpr bool kMin = false;
   static constexpr float kSub = 8388736.0f;  // 2^23 + 128: int8 codes stored with the sign bit flipped
-  __device__ __forceinline__ static void get(const URef& u, int c, float (&a)[2], float (&b)[2], uint32_t (&qb)[8]) {
+  template <class U>
+  __device__ __forceinline__ static void get(const U& u, int c, float (&a)[2], float (&b)[2], uint32_t (&qb)[8]) {
     a[0] = a[1] = h2f(u.b16(34 * c));
     b[0] = b[1] = 0.f;
     const int o0 = 34 * c + 2 + u.delta;  // the block's codes
@@ -234,7 +268,8 @@ template <>
 struct MixChunk<kQ6_K> {
   static constexpr bool kMin = false;
   static constexpr float kSub = 8388640.0f;  // 2^23 + 32
-  __device__ __forceinline__ static void get(const URef& u, int c, float (&a)[2], float (&b)[2], uint32_t (&qb)[8]) {
+  template <class U>
+  __device__ __forceinline__ static void get(const U& u, int c, float (&a)[2], float (&b)[2], uint32_t (&qb)[8]) {
     const int h = c >> 2, g = c & 3;
     const float d = h2f(u.b16(208));
     const uint32_t sw = u.b16(192 + 8 * h + 2 * g);  // two int8 scales
@@ -274,7 +309,8 @@ template <>
 struct MixChunk<kQ3_K> {
   static constexpr bool kMin = false;
   static constexpr float kSub = 8388612.0f;  // 2^23 + 4
-  __device__ __forceinline__ static void get(const URef& u, int c, float (&a)[2], float (&b)[2], uint32_t (&qb)[8]) {
+  template <class U>
+  __device__ __forceinline__ static void get(const U& u, int c, float (&a)[2], float (&b)[2], uint32_t (&qb)[8]) {
     const int h = c >> 2, sft = c & 3;
     const float d = h2f(u.b16(108));
 #pragma unroll

@@ -37,15 +37,25 @@ constexpr int kMaxBlocks = 1184;  // of a launch: the partials that the gradient
 
 // A unit's slot: the 16-byte aligned span of a 2-byte aligned unit, and a
 // word more for the field reads that join two words.
-__host__ __device__ inline int slot_bytes(int ub) { return ((ub + 14 + 15) & ~15) + 16; }
-__host__ __device__ inline int warp_bytes(const CandSet& cs) {
-  int s = 0;
-  for (int k = 0; k < cs.K; ++k) s += kUnits * slot_bytes(cs.ubytes[k]);
-  return s;
-}
+inline int slot_bytes(int ub) { return ((ub + 14 + 15) & ~15) + 16; }
 
-__device__ __forceinline__ void async_copy16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+// The candidates of a launch.  In a warp's buffer the four slots of candidate
+// k start at byte `region`.
+struct Cands {
+  struct Info {
+    int decode, ubytes, slot, region;
+  };
+  const uint8_t* ptr[kMaxCandidates];
+  Info info[kMaxCandidates];
+  int K, warp_bytes;
+};
+
+__device__ __forceinline__ void async_copy16(uint32_t dst, const void* src, bool on) {
+  asm volatile(
+      "{ .reg .pred p; setp.ne.s32 p, %2, 0;\n"
+      "  @p cp.async.cg.shared.global [%0], [%1], 16; }" ::"r"(dst),
+      "l"(src), "r"(static_cast<int>(on))
+      : "memory");
 }
 __device__ __forceinline__ void async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -56,18 +66,17 @@ __device__ __forceinline__ void async_wait() {
 // Copies unit `unit` (of the whole table) of every candidate into slot `lu`
 // of the warp's buffer; lane c of the unit's eight takes every eighth vector
 // (18 at most: a Q8_0 unit that starts inside a vector).
-__device__ __forceinline__ void stage_unit(const CandSet& cs, uint32_t buf, int lu, int c, long long unit) {
+__device__ __forceinline__ void stage_unit(const Cands& cs, uint32_t buf, int lu, int c, long long unit) {
   for (int k = 0; k < cs.K; ++k) {
-    const int ub = cs.ubytes[k], slot = slot_bytes(ub);
-    const uint8_t* a = cs.ptr[k] + unit * ub;
+    const Cands::Info f = cs.info[k];
+    const uint8_t* a = cs.ptr[k] + unit * f.ubytes;
     const int rel = static_cast<int>(reinterpret_cast<uintptr_t>(a) & 15u);
     const uint8_t* src = a - rel + 16 * c;
-    const uint32_t dst = buf + lu * slot + 16 * c;
-    const int left = rel + ub - 16 * c;  // bytes from this lane's first vector on
-    if (left > 0) async_copy16(dst, src);
-    if (left > 128) async_copy16(dst + 128, src + 128);
-    if (left > 256) async_copy16(dst + 256, src + 256);
-    buf += kUnits * slot;
+    const uint32_t dst = buf + f.region + lu * f.slot + 16 * c;
+    const int left = rel + f.ubytes - 16 * c;  // bytes from this lane's first vector on
+    async_copy16(dst, src, left > 0);
+    async_copy16(dst + 128, src + 128, left > 128);
+    async_copy16(dst + 256, src + 256, left > 256);
   }
 }
 
@@ -92,18 +101,18 @@ inline int decode_code(int fmt, const uint8_t* p) {
 template <int F>
 using Format = std::integral_constant<int, F>;
 
-// Calls op(format, unit) for the staged unit of candidate k (whose cs.fmt is
-// its decode_code), whose slots start at `region`; `unit` counts modulo 2^32.
+// Calls op(format, unit) for the staged unit of candidate k; `unit` counts
+// modulo 2^32.
 template <class Op>
-__device__ __forceinline__ void with_unit(const CandSet& cs, const uint8_t* region, int k, int lu, uint32_t unit,
+__device__ __forceinline__ void with_unit(const Cands& cs, const uint8_t* buf, int k, int lu, uint32_t unit,
                                           const Op& op) {
-  const int ub = cs.ubytes[k];
-  const uint32_t rel = (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(cs.ptr[k])) + unit * ub) & 15u;
-  const uint32_t* s = reinterpret_cast<const uint32_t*>(region + lu * slot_bytes(ub) + (rel & ~3u));
-  const URef any{s, static_cast<int>(rel & 3u), 8u * (rel & 3u)};
+  const Cands::Info f = cs.info[k];
+  const uint32_t rel = (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(cs.ptr[k])) + unit * f.ubytes) & 15u;
+  const uint32_t* s = reinterpret_cast<const uint32_t*>(buf + f.region + lu * f.slot + (rel & ~3u));
+  const URefHalf any{s, static_cast<int>(rel & 2u)};
   const URefAligned<false> words{s};
   const URefAligned<true> vectors{s};
-  switch (cs.fmt[k]) {
+  switch (f.decode) {
     case kDQ8: op(Format<kQ8_0>{}, any); break;
     case kDQ3: op(Format<kQ3_K>{}, any); break;
     case kDQ6: op(Format<kQ6_K>{}, any); break;
@@ -238,7 +247,7 @@ __device__ __forceinline__ void mix_unit(const U& u, int c, float pk, float (&ac
 // otherwise once per token, with no plan to wait for.
 template <bool kRuns>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
-    embed_mix_kernel(const __grid_constant__ CandSet cs, const float* __restrict__ probs, Ids ids, int T, Plan plan,
+    embed_mix_kernel(const __grid_constant__ Cands cs, const float* __restrict__ probs, Ids ids, int T, Plan plan,
                      long long vocab_start, int rows, int units_per_row, int cols, float scale, bool strict, bool vec,
                      __nv_bfloat16* __restrict__ out, long long ldo, int* err) {
   extern __shared__ __align__(16) uint8_t esmem[];
@@ -247,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
   __syncthreads();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int lu = lane >> 3, c = lane & 7;
-  uint8_t* buf = esmem + kWarps * kUnits * 512 + warp * warp_bytes(cs);
+  uint8_t* buf = esmem + kWarps * kUnits * 512 + warp * cs.warp_bytes;
   uint4* rows_s = reinterpret_cast<uint4*>(esmem + (warp * kUnits + lu) * 512);
   UnitWalk<kRuns> w{plan, ids, kRuns ? plan.pieces(T, rows, err) : T, vocab_start, rows, units_per_row};
   w.start_at((static_cast<long long>(blockIdx.x) * kWarps + warp) * kUnits + lu,
@@ -271,13 +280,11 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
     async_wait<0>();
     __syncwarp();
     if (now.row >= 0 && col < cols) {
-      const uint8_t* region = buf;
       for (int k = 0; k < cs.K; ++k) {
         const float pk = pk_s[k];
-        with_unit(cs, region, k, lu, static_cast<uint32_t>(unit), [&](auto f, const auto& u) {
+        with_unit(cs, buf, k, lu, static_cast<uint32_t>(unit), [&](auto f, const auto& u) {
           mix_unit<decltype(f)::value>(u, c, pk, acc, cst);
         });
-        region += kUnits * slot_bytes(cs.ubytes[k]);
       }
     }
     bad |= now.row < 0 && len > 0;
@@ -290,9 +297,9 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
       __align__(16) __nv_bfloat162 h[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float cs0 = cst[v >> 1];
-        const float x = acc[8 * v + 2 * j] + cs0, y = acc[8 * v + 2 * j + 1] + cs0;
-        h[j] = scaled ? __floats2bfloat162_rn(x * scale, y * scale) : __floats2bfloat162_rn(x, y);
+        float2 x = __fadd2_rn(make_float2(acc[8 * v + 2 * j], acc[8 * v + 2 * j + 1]), make_float2(cst[v >> 1], cst[v >> 1]));
+        if (scaled) x = make_float2(x.x * scale, x.y * scale);
+        h[j] = __floats2bfloat162_rn(x.x, x.y);
       }
       rows_s[c * 4 + (v ^ (c >> 1))] = *reinterpret_cast<const uint4*>(h);
     }
@@ -683,13 +690,14 @@ __device__ __forceinline__ void add_row(const T* row, int col, int cols, bool ve
       for (int i = 0; i < 4; ++i) {
         if constexpr (sizeof(T) == 4) {
           g[4 * j + i] += __uint_as_float(w[i]);
-        } else if constexpr (std::is_same<T, __half>::value) {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-          g[8 * j + 2 * i] += f.x;
-          g[8 * j + 2 * i + 1] += f.y;
         } else {
-          g[8 * j + 2 * i] += __uint_as_float(w[i] << 16);
-          g[8 * j + 2 * i + 1] += __uint_as_float(w[i] & 0xffff0000u);
+          float2 f;
+          if constexpr (std::is_same<T, __half>::value)
+            f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+          else
+            f = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+          f = __fadd2_rn(make_float2(g[8 * j + 2 * i], g[8 * j + 2 * i + 1]), f);
+          g[8 * j + 2 * i] = f.x, g[8 * j + 2 * i + 1] = f.y;
         }
       }
     }
@@ -709,14 +717,14 @@ __device__ __forceinline__ void add_row(const T* row, int col, int cols, bool ve
 // the block's are left in partials[blockIdx.x][K].
 template <typename T>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
-    embed_gategrad_kernel(const __grid_constant__ CandSet cs, Plan plan, int tokens, int rows, int units_per_row,
+    embed_gategrad_kernel(const __grid_constant__ Cands cs, Plan plan, int tokens, int rows, int units_per_row,
                           int cols, const T* __restrict__ dy, long long lddy, bool vec, double* __restrict__ partials,
                           int* err) {
   extern __shared__ __align__(16) uint8_t esmem[];
   double* acc = reinterpret_cast<double*>(esmem);  // [K][kThreads]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int lu = lane >> 3, c = lane & 7;
-  uint8_t* buf = esmem + cs.K * kThreads * sizeof(double) + warp * warp_bytes(cs);
+  uint8_t* buf = esmem + cs.K * kThreads * sizeof(double) + warp * cs.warp_bytes;
   for (int k = 0; k < cs.K; ++k) acc[k * kThreads + threadIdx.x] = 0.0;
   UnitWalk<true> w{plan, Ids{nullptr, false}, plan.pieces(tokens, rows, err), 0, rows, units_per_row};
   w.start_at((static_cast<long long>(blockIdx.x) * kWarps + warp) * kUnits + lu,
@@ -739,20 +747,23 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
       const int tok = __shfl_sync(0xffffffffu, mine, (lane & 24) + i);
       if (i < len && on) add_row<T>(dy + static_cast<long long>(tok) * lddy, col, cols, vec, g);
     }
-    float gs[2] = {0.f, 0.f};
+    float gs[2];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) gs[j >> 4] += g[j];
+    for (int h = 0; h < 2; ++h) {
+      float2 t = make_float2(g[16 * h], g[16 * h + 1]);
+#pragma unroll
+      for (int j = 2; j < 16; j += 2) t = __fadd2_rn(t, make_float2(g[16 * h + j], g[16 * h + j + 1]));
+      gs[h] = t.x + t.y;
+    }
     async_wait<0>();
     __syncwarp();
     if (on) {
-      const uint8_t* region = buf;
       for (int k = 0; k < cs.K; ++k) {
         float d = 0.f;
-        with_unit(cs, region, k, lu, static_cast<uint32_t>(unit), [&](auto f, const auto& u) {
+        with_unit(cs, buf, k, lu, static_cast<uint32_t>(unit), [&](auto f, const auto& u) {
           d = dot_unit<decltype(f)::value>(u, c, g, gs);
         });
         acc[k * kThreads + threadIdx.x] += static_cast<double>(d);
-        region += kUnits * slot_bytes(cs.ubytes[k]);
       }
     }
     __syncwarp();  // the slots are filled again

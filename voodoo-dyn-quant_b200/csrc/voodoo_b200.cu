@@ -1365,9 +1365,18 @@ namespace {
 
 // ---- gated embedding ----
 // The candidates with the alignment of their blocks in the formats' codes.
-int build_table(vq::CandSet* cs, int K, const int* types, const void* const* blocks) {
-  if (int rc = build_candset(cs, K, types, blocks)) return rc;
-  for (int k = 0; k < K; ++k) cs->fmt[k] = vq::embed::decode_code(cs->fmt[k], cs->ptr[k]);
+int build_table(vq::embed::Cands* out, int K, const int* types, const void* const* blocks) {
+  using namespace vq::embed;
+  vq::CandSet cs;
+  if (int rc = build_candset(&cs, K, types, blocks)) return rc;
+  *out = Cands{};
+  out->K = K;
+  for (int k = 0; k < K; ++k) {
+    const int slot = slot_bytes(cs.ubytes[k]);
+    out->ptr[k] = cs.ptr[k];
+    out->info[k] = Cands::Info{decode_code(cs.fmt[k], cs.ptr[k]), cs.ubytes[k], slot, out->warp_bytes};
+    out->warp_bytes += kUnits * slot;
+  }
   return 0;
 }
 
@@ -1433,11 +1442,11 @@ int one_wave(Kernel kern, int smem, long long units, int* grid) {
 }
 
 template <typename T>
-int launch_embed_gategrad(const vq::CandSet& cs, const vq::embed::Plan& plan, long long tokens, long long rows, int upr,
+int launch_embed_gategrad(const vq::embed::Cands& cs, const vq::embed::Plan& plan, long long tokens, long long rows, int upr,
                           int cols, const void* dy, long long lddy, double* partials, int* blocks, int* err,
                           cudaStream_t st) {
   using namespace vq::embed;
-  const int smem = cs.K * kThreads * static_cast<int>(sizeof(double)) + kWarps * warp_bytes(cs);
+  const int smem = cs.K * kThreads * static_cast<int>(sizeof(double)) + kWarps * cs.warp_bytes;
   if (int rc = one_wave(embed_gategrad_kernel<T>, smem, tokens * upr, blocks)) return rc;
   const bool vec = aligned16(dy) && lddy * sizeof(T) % 16 == 0;
   embed_gategrad_kernel<T><<<*blocks, kThreads, smem, st>>>(cs, plan, static_cast<int>(tokens), static_cast<int>(rows), upr,
@@ -1506,7 +1515,7 @@ int vq_embed_mix(int K, const int* types, const void* const* blocks, const float
                  int64_t T, const void* plan, size_t plan_bytes, int64_t vocab_start, int64_t rows, int64_t padded_cols,
                  int64_t cols, float scale, int strict, void* out, int64_t ldo, void* stream) {
   DeviceScope scope(out);
-  vq::CandSet cs;
+  vq::embed::Cands cs;
   if (int rc = build_table(&cs, K, types, blocks)) return rc;
   if (int rc = check_table(T, vocab_start, rows, padded_cols, cols)) return rc;
   if (int rc = check_matrix(out, T, cols, ldo, "out")) return rc;
@@ -1520,7 +1529,7 @@ int vq_embed_mix(int K, const int* types, const void* const* blocks, const float
   int* err = nullptr;
   if (int rc = device_error_ptr(&err)) return rc;
   using namespace vq::embed;
-  const int smem = kWarps * (kUnits * 512 + warp_bytes(cs));
+  const int smem = kWarps * (kUnits * 512 + cs.warp_bytes);
   const int upr = static_cast<int>(padded_cols / 256);
   auto kern = plan != nullptr ? embed_mix_kernel<true> : embed_mix_kernel<false>;
   int grid = 0;
@@ -1542,7 +1551,7 @@ int vq_embed_gategrad(int K, const int* types, const void* const* blocks, const 
                       int64_t rows, int64_t padded_cols, int64_t cols, float scale, const void* dy, int64_t lddy,
                       int dy_dtype, void* workspace, size_t workspace_bytes, float* grad, void* stream) {
   DeviceScope scope(grad);
-  vq::CandSet cs;
+  vq::embed::Cands cs;
   if (int rc = build_table(&cs, K, types, blocks)) return rc;
   if (int rc = check_table(T, 0, rows, padded_cols, cols)) return rc;
   if (int rc = check_matrix(dy, T, cols, lddy, "dy")) return rc;
