@@ -10,8 +10,8 @@
 // sums a piece's rows of dy first and multiplies the decoded weights into that
 // sum as it decodes them.  What they cannot do without is the packed rows and
 // T x D of out or dy (16384 x 4096 of text, six candidates: 35 us of HBM each);
-// the decoding bounds them, some 245 instructions for 32 weights of a
-// candidate (82 us the lookup, 81 us the gradient).
+// the decoding bounds them, 220 to 330 instructions for 32 weights of a
+// candidate (63 us the lookup, 71 us the gradient).
 //
 // Eight lanes hold a unit (256 weights) of a row, a lane 32 consecutive
 // weights.  The lanes of a unit copy its packed bytes of every candidate into
@@ -26,13 +26,14 @@
 namespace vq {
 namespace embed {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kUnits = 4;  // units of a warp
-// Resident blocks per SM, and so 80 registers a thread: decoding keeps every
-// pipe half busy and waits for its own results, so warps count (16384 x 4096
-// text, six candidates: 82 us with 3, 95 with 2; 4 blocks spill and take 113).
-constexpr int kBlocksPerSm = 3;
+// Resident blocks per SM, and so 72 registers a thread: decoding waits for its
+// own results, so warps count, until they spill (16384 x 4096 text, six
+// candidates, lookup and gradient: 63 and 71 us with 7, 63 and 76 with 6, 64
+// and 82 with 8; blocks of 256 threads 65 and 75 with 3, 66 and 81 with 4).
+constexpr int kBlocksPerSm = 7;
 constexpr int kMaxBlocks = 1184;  // of a launch: the partials that the gradient leaves
 
 // A unit's slot: the 16-byte aligned span of a 2-byte aligned unit, and a
@@ -50,11 +51,13 @@ struct Cands {
   int K, warp_bytes;
 };
 
-__device__ __forceinline__ void async_copy16(uint32_t dst, const void* src, bool on) {
+// The 16 bytes at kAbove, where a > kAbove.
+template <int kAbove>
+__device__ __forceinline__ void async_copy16(uint32_t dst, const void* src, int a) {
   asm volatile(
-      "{ .reg .pred p; setp.ne.s32 p, %2, 0;\n"
-      "  @p cp.async.cg.shared.global [%0], [%1], 16; }" ::"r"(dst),
-      "l"(src), "r"(static_cast<int>(on))
+      "{ .reg .pred p; setp.gt.s32 p, %2, %3;\n"
+      "  @p cp.async.cg.shared.global [%0 + %3], [%1 + %3], 16; }" ::"r"(dst),
+      "l"(src), "r"(a), "n"(kAbove)
       : "memory");
 }
 __device__ __forceinline__ void async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -74,9 +77,9 @@ __device__ __forceinline__ void stage_unit(const Cands& cs, uint32_t buf, int lu
     const uint8_t* src = a - rel + 16 * c;
     const uint32_t dst = buf + f.region + lu * f.slot + 16 * c;
     const int left = rel + f.ubytes - 16 * c;  // bytes from this lane's first vector on
-    async_copy16(dst, src, left > 0);
-    async_copy16(dst + 128, src + 128, left > 128);
-    async_copy16(dst + 256, src + 256, left > 256);
+    async_copy16<0>(dst, src, left);
+    async_copy16<128>(dst, src, left);
+    async_copy16<256>(dst, src, left);
   }
 }
 
@@ -262,7 +265,6 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
   w.start_at((static_cast<long long>(blockIdx.x) * kWarps + warp) * kUnits + lu,
              static_cast<long long>(gridDim.x) * kWarps * kUnits);
   bool bad = false;
-  const bool scaled = scale != 1.f;
   for (;; w.step()) {
     const auto now = w.get();
     if (!__any_sync(0xffffffffu, now.begin < now.end)) break;
@@ -298,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float2 x = __fadd2_rn(make_float2(acc[8 * v + 2 * j], acc[8 * v + 2 * j + 1]), make_float2(cst[v >> 1], cst[v >> 1]));
-        if (scaled) x = make_float2(x.x * scale, x.y * scale);
+        x = __fmul2_rn(x, make_float2(scale, scale));  // exact for scale 1
         h[j] = __floats2bfloat162_rn(x.x, x.y);
       }
       rows_s[c * 4 + (v ^ (c >> 1))] = *reinterpret_cast<const uint4*>(h);
@@ -714,7 +716,7 @@ __device__ __forceinline__ void add_row(const T* row, int col, int cols, bool ve
 // into several pieces is finished in each, the products being linear.  Sums
 // over pieces are held in 64 bits, in the thread's own place of shared memory
 // (an index that varies would put a register array into local memory), and
-// the block's are left in partials[blockIdx.x][K].
+// the block's are left in partials[K][gridDim.x].
 template <typename T>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
     embed_gategrad_kernel(const __grid_constant__ Cands cs, Plan plan, int tokens, int rows, int units_per_row,
@@ -774,7 +776,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
     for (int i = lane; i < kThreads; i += 32) t += acc[k * kThreads + i];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t += __shfl_down_sync(0xffffffffu, t, o);
-    if (lane == 0) partials[static_cast<long long>(blockIdx.x) * cs.K + k] = t;
+    if (lane == 0) partials[k * gridDim.x + blockIdx.x] = t;
   }
 }
 
@@ -785,7 +787,8 @@ __global__ void __launch_bounds__(32 * kMaxCandidates) embed_gategrad_join_kerne
   const int k = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (k >= K) return;
   double t = 0.0;
-  for (int b = lane; b < blocks; b += 32) t += partials[static_cast<long long>(b) * K + k];
+#pragma unroll 8
+  for (int b = lane; b < blocks; b += 32) t += partials[k * blocks + b];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) t += __shfl_down_sync(0xffffffffu, t, o);
   if (lane == 0) grad[k] = static_cast<float>(t * static_cast<double>(scale));
