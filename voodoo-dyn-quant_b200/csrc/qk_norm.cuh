@@ -16,9 +16,9 @@
 // D / 16 of a head that is no power of two carry nothing.  Arithmetic is fp32
 // from the load to the one rounding of the store.
 //
-// 16384 positions x 40 heads of 128 in bf16: forward 66 us (5.1 TB/s),
-// backward with the weights' gradients 92 to 97 us (5.2 to 5.5 TB/s); 16384 x
-// 24: 37 and 53 us (5.4 and 5.7 TB/s).  A plain copy of that size reaches 6.5.
+// 16384 positions x 40 heads of 128 in bf16: forward 56.5 us (5.9 TB/s),
+// backward with the weights' gradients 89 us (5.7 TB/s); 16384 x 24: 35 and
+// 51 us (5.8 and 5.9 TB/s).  A plain copy of that size reaches 6.5.
 #pragma once
 
 #include "common.cuh"

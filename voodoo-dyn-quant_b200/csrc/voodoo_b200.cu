@@ -1161,13 +1161,17 @@ int qk_plan(QkPlan* p, int64_t positions, int64_t Hq, int64_t Hk, int64_t D, int
     *chunks[i] = *iters[i] > 0 ? static_cast<int>((all + *iters[i] - 1) / *iters[i]) : 0;
     items[i] = positions * *chunks[i];
   }
-  // one wave of blocks, shared by the sides as their heads are
+  // One wave of blocks, shared by the sides as their work is.  An item's start (its tables' way from L2) takes as long
+  // as some four of its steps: 32 + 8 heads of 128 at 16384 positions, forward 56.5 us and backward 89, shared as the
+  // heads are 66.6 and 97; 16 + 8 heads 35 and 51, not 37 and 53.
+  constexpr int kItemStart = 4;
   const long long wave = static_cast<long long>(blocks_per_sm) * sms;
   const long long cap = wave < vq::qknorm::kMaxBlocks ? wave : vq::qknorm::kMaxBlocks;
   long long qb = (items[0] + vq::qknorm::kWarps - 1) / vq::qknorm::kWarps;
   long long kb = (items[1] + vq::qknorm::kWarps - 1) / vq::qknorm::kWarps;
   if (qb + kb > cap) {
-    long long qc = cap * Hq / (Hq + Hk);
+    const long long qcost = items[0] * (*iters[0] + kItemStart), kcost = items[1] * (*iters[1] + kItemStart);
+    long long qc = cap * qcost / (qcost + kcost);
     if (Hq > 0 && qc < 1) qc = 1;
     if (Hk > 0 && qc > cap - 1) qc = cap - 1;
     if (qb > qc) qb = qc;
