@@ -227,7 +227,12 @@ __device__ __forceinline__ void scale_chunk(const Chunk& c, float s) {
 #pragma unroll
     for (int j = 0; j < kVecs; ++j) v[j] = p[j * kThreads];
 #pragma unroll
-    for (int j = 0; j < kVecs; ++j) p[j * kThreads] = Values<kType>(v[j]).scaled(s);
+    for (int j = 0; j < kVecs; ++j) {
+      const uint4 w = Values<kType>(v[j]).scaled(s);
+      // a factor just below 1 leaves most 16-bit values as they are: not written (0.59 G bf16 values and a factor of
+      // 0.999: 338 us the two passes, 550 when written; 550 either way for 0.9)
+      if (((w.x ^ v[j].x) | (w.y ^ v[j].y) | (w.z ^ v[j].z) | (w.w ^ v[j].w)) != 0) p[j * kThreads] = w;
+    }
     return;
   }
   constexpr int kSize = kType == kF32 ? 4 : 2;
