@@ -248,12 +248,19 @@ def test_unaligned_blocks(cuda):
         _, _, blocks, dec, p = _table(V, D, [qt], 6, cuda)
         ids = _ids(T, V, 7)
         one = torch.ones(1, device=cuda)
-        want = _C.embed_mix(ids.to(cuda), _C.EmbedTable([qt], blocks, V, D, D), one)
+        table = _C.EmbedTable([qt], blocks, V, D, D)
+        want = _C.embed_mix(ids.to(cuda), table, one)
+        plan = _C.embed_plan(ids.to(cuda), V)
+        dy = torch.randn(T, D, generator=torch.Generator().manual_seed(5)).to(cuda)
+        grad = _C.embed_gategrad(dy, table, plan)
         for off in (2, 6, 14):
             buf = torch.empty(blocks[0].numel() + 16, dtype=torch.uint8, device=cuda)
             b = buf[off:off + blocks[0].numel()]
             b.copy_(blocks[0].reshape(-1))
-            assert torch.equal(_C.embed_mix(ids.to(cuda), _C.EmbedTable([qt], [b], V, D, D), one), want)
+            table = _C.EmbedTable([qt], [b], V, D, D)
+            assert torch.equal(_C.embed_mix(ids.to(cuda), table, one), want)
+            assert torch.equal(_C.embed_mix(ids.to(cuda), table, one, plan=plan), want)
+            assert torch.equal(_C.embed_gategrad(dy, table, plan), grad)
 
 
 @pytest.mark.parametrize("T", [3000, 5000])  # a plan by one block, and by a cluster
@@ -355,3 +362,35 @@ def test_module_returns_its_sources_type(cuda, dtype):
     _check_lookup(out.detach(), ids.cpu(), dec, torch.tensor([0.5, 0.5]), 1.0, 0, V)
     out.sum().backward()
     assert m.emb.gates.grad.shape == (2,) and m.emb.gates.grad.any()
+
+
+def test_offsets_past_32_bits(cuda):
+    """A table of more than 2^32 bytes and rows of more than 2^31 values: the last ones are read and written as those of
+    a small call are."""
+    from voodoo_quant import _C
+
+    D, rows, T = 16384, 260_000, 140_000
+    _, _, small, _, _ = _table(3, D, ["Q8_0"], 12, cuda)
+    bytes_row = small[0].numel() // 3
+    big = torch.zeros(rows * bytes_row, dtype=torch.uint8, device=cuda)
+    assert big.numel() > 2 ** 32 and T * D > 2 ** 31
+    big[-3 * bytes_row:] = small[0].reshape(-1)
+    one = torch.ones(1, device=cuda)
+    table, few = _C.EmbedTable(["Q8_0"], [big], rows, D, D), _C.EmbedTable(["Q8_0"], small, 3, D, D)
+    ids = torch.zeros(T, dtype=torch.int64, device=cuda)
+    last = torch.tensor([2, 0, 1, 2], device=cuda)
+    ids[-4:] = last + (rows - 3)
+    want = _C.embed_mix(last, few, one)
+    plan = _C.embed_plan(ids, rows)
+    for q in (plan, None):
+        out = _C.embed_mix(ids, table, one, plan=q)
+        assert torch.equal(out[-4:], want) and not out[:-4].any()
+        del out
+    dy = torch.zeros(T, D, dtype=torch.bfloat16, device=cuda)
+    dy[-4:] = torch.randn(4, D, generator=torch.Generator().manual_seed(2)).to(cuda)
+    exact = float((dy[-4:].double() * want.double()).sum())
+    mag = float((dy[-4:].double() * want.double()).abs().sum())
+    grad = float(_C.embed_gategrad(dy, table, plan))
+    # the rows in bf16 against the decoded ones: 2^-8 of each product; the sums as elsewhere
+    assert abs(grad - exact) <= (2.0 ** -8 + 64 * 2.0 ** -24) * mag
+    assert _C.device_error() == 0

@@ -261,3 +261,17 @@ def test_trainer_clips_its_gates(cuda):
     for p, r in zip(trainer.trainable, ref):
         # the norms differ by a few roundings, and each value by its own
         assert torch.allclose(p.grad, r.grad, rtol=16 * ULP, atol=0)
+
+
+def test_a_tensor_of_more_than_2_to_the_31_values(cuda):
+    """Powers of two, so that the norm is known: n values of 1 / 2 have the norm sqrt(n) / 2."""
+    from voodoo_quant.training.grad_clip import clip_grad_norm_
+
+    n = 2 ** 31 + 2 ** 20 + 5
+    p = torch.nn.Parameter(torch.empty(0, dtype=torch.bfloat16, device=cuda))
+    p.data = torch.empty(1, dtype=torch.bfloat16, device=cuda).expand(n)
+    p.grad = torch.full((n,), 0.5, dtype=torch.bfloat16, device=cuda)
+    norm = clip_grad_norm_([p], math.sqrt(n) / 4)
+    assert abs(float(norm) - math.sqrt(n) / 2) <= 6 * ULP * float(norm)
+    # the factor is 1/2 within a few roundings of 2^-24: 0.25 is the nearest bf16 value by far
+    assert (p.grad[0], p.grad[-1]) == (0.25, 0.25) and int((p.grad == 0.25).sum()) == n

@@ -239,3 +239,34 @@ def test_frozen_weights_and_unused_outputs(cuda):
         lambda x: _forward64(x, w.double(), cos.double(), sin.double(), 1e-6, 0.0)[0].square().sum(), q.detach().double())[1]
     # |q| is kept by norm and rotation up to eps: the gradient is the difference of near equals, each of order 2
     assert (q.grad.double() - want).abs().max() < 64 * ULP * 16
+
+
+def test_offsets_past_32_bits(cuda):
+    """Heads of more than 2^31 values, and a layout whose batch stride is past 2^31: the last positions come out as those
+    of a call on them alone do."""
+    from voodoo_quant import _C
+
+    S, Hq, Hk, D = 440_000, 39, 1, 128
+    g = torch.Generator(device=cuda).manual_seed(4)
+    q = torch.zeros(1, S, Hq, D, dtype=torch.bfloat16, device=cuda)
+    k = torch.zeros(1, S, Hk, D, dtype=torch.bfloat16, device=cuda)
+    assert q.numel() > 2 ** 31
+    n = 3
+    for t in (q, k):
+        t[:, -n:] = torch.randn(1, n, t.shape[2], D, device=cuda, generator=g)
+    w = torch.ones(D, dtype=torch.bfloat16, device=cuda)
+    cos, sin = (torch.randn(1, S, D, device=cuda, generator=g).bfloat16() for _ in range(2))
+
+    def both(q, k, cos, sin):
+        qo, ko, ops, layout = _C.qk_norm_rope_fwd(q, k, w, w, cos, sin, 1e-6, 0.0, saved=True)
+        return qo, ko, *_C.qk_norm_rope_bwd(q, k, ops, layout, False)[:2]
+
+    want = both(q[:, -n:], k[:, -n:], cos[:, -n:], sin[:, -n:])
+    for got, exp in zip(both(q, k, cos, sin), want):
+        assert torch.equal(got[:, -n:], exp) and not got[:, :-n].any()
+    # two batch entries, 2^31 values and more apart
+    flat = q.reshape(-1)
+    far = flat.as_strided((2, n, Hq, D), (flat.numel() - n * Hq * D, Hq * D, D, 1))
+    kk, cc, ss = k[:, -n:].expand(2, n, Hk, D), cos[:, -n:], sin[:, -n:]
+    for got, exp in zip(both(far, kk, cc, ss), want):
+        assert torch.equal(got[1:], exp)
