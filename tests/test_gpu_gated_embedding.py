@@ -394,3 +394,35 @@ def test_offsets_past_32_bits(cuda):
     # the rows in bf16 against the decoded ones: 2^-8 of each product; the sums as elsewhere
     assert abs(grad - exact) <= (2.0 ** -8 + 64 * 2.0 ** -24) * mag
     assert _C.device_error() == 0
+
+
+def test_gradient_has_no_graph_of_its_own(cuda):
+    """The gradient taken with create_graph, and a second time, is the first one; a second derivative is refused."""
+    from voodoo_quant.layers import gated_embedding
+
+    types = ["Q4_K", "Q6_K"]
+    V, D = 30, 512
+    _, _, blocks, _, p = _table(V, D, types, 14, cuda)
+    for probs in (p.to(cuda).requires_grad_(), p.to(cuda).double().view(2, 1).requires_grad_()):
+        out = gated_embedding(_ids(50, V, 2).to(cuda), probs, types, blocks, V, D)
+        dy = torch.randn(50, D, device=cuda, generator=torch.Generator(device=cuda).manual_seed(1)).bfloat16()
+        (first,) = torch.autograd.grad(out, probs, dy, retain_graph=True)
+        assert first.shape == probs.shape and first.dtype == probs.dtype
+        dy.requires_grad_()
+        (again,) = torch.autograd.grad(out, probs, dy, create_graph=True)
+        assert torch.equal(first, again)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            again.sum().backward()
+
+
+def test_a_plan_of_another_size_is_refused(cuda):
+    from voodoo_quant import _C
+
+    types = ["Q8_0"]
+    _, _, blocks, _, p = _table(9, 256, types, 1, cuda)
+    table = _C.EmbedTable(types, blocks, 9, 256, 256)
+    plan = _C.embed_plan(torch.zeros(100, dtype=torch.int64, device=cuda), 9)
+    with pytest.raises(ValueError, match="plan of"):
+        _C.embed_gategrad(torch.zeros(500, 256, dtype=torch.bfloat16, device=cuda), table, plan)
+    with pytest.raises(ValueError, match="plan of"):
+        _C.embed_mix(torch.zeros(10, dtype=torch.int64, device=cuda), table, torch.ones(1, device=cuda), plan=plan)

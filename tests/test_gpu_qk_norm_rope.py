@@ -270,3 +270,21 @@ def test_offsets_past_32_bits(cuda):
     kk, cc, ss = k[:, -n:].expand(2, n, Hk, D), cos[:, -n:], sin[:, -n:]
     for got, exp in zip(both(far, kk, cc, ss), want):
         assert torch.equal(got[1:], exp)
+
+
+def test_gradients_have_no_graph_of_their_own(cuda):
+    """The gradients taken with create_graph are those taken without; a second derivative is refused, not zero."""
+    from voodoo_quant.fused_blocks import qk_norm_rope
+
+    g = torch.Generator(device=cuda).manual_seed(8)
+    q, k, gq, gk = (torch.randn(1, 5, 2, 64, device=cuda, generator=g) for _ in range(4))
+    w = torch.ones(64, device=cuda)
+    cos, sin = (torch.randn(1, 5, 64, device=cuda, generator=g) for _ in range(2))
+    leaves = [t.requires_grad_() for t in (q, k, w)]
+    out = qk_norm_rope(q, k, w, w, cos, sin)
+    plain = torch.autograd.grad(out, leaves, (gq, gk), retain_graph=True)
+    gq.requires_grad_()
+    graph = torch.autograd.grad(out, leaves, (gq, gk), create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(plain, graph))
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        graph[0].sum().backward()

@@ -1425,7 +1425,7 @@ int check_ids(const void* ids, int ids_i32) {
 
 int check_plan(const void* plan, size_t plan_bytes, int64_t T) {
   const size_t need = PlanLayout(T).bytes;
-  if (plan == nullptr || (reinterpret_cast<uintptr_t>(plan) & 15u) != 0 || plan_bytes < need)
+  if (plan == nullptr || (reinterpret_cast<uintptr_t>(plan) & 15u) != 0 || plan_bytes != need)
     return fail(VQ_ERR_INVALID, "plan of %zu bytes (16-byte aligned) needed, got %zu", need, plan_bytes);
   return 0;
 }

@@ -28,7 +28,6 @@ import types
 import torch
 import torch.nn.functional as F
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from voodoo_quant import _C
 
@@ -106,17 +105,18 @@ class _QKNormRopeFn(Function):
     def forward(ctx, q, k, q_weight, k_weight, constants: tuple):
         qo, ko, operands, ctx.layout = _C.qk_norm_rope_fwd(q, k, q_weight, k_weight, *constants, saved=True)
         ctx.save_for_backward(*operands)
-        ctx.weight_types = (q_weight.dtype, k_weight.dtype)
+        types = q_weight.dtype, k_weight.dtype
+        ctx.cast = None if types == (operands[2].dtype, operands[3].dtype) else types
         return qo, ko
 
     @staticmethod
-    @once_differentiable
+    @_C.first_order
     def backward(ctx, gq: torch.Tensor, gk: torch.Tensor):
-        need = ctx.needs_input_grad
-        dq, dk, dwq, dwk = _C.qk_norm_rope_bwd(gq, gk, ctx.saved_tensors, ctx.layout,
-                                               want_weight_grads=need[2] or need[3])
-        return (dq if need[0] else None, dk if need[1] else None, dwq.to(ctx.weight_types[0]) if need[2] else None,
-                dwk.to(ctx.weight_types[1]) if need[3] else None, None)
+        need_q, need_k, need_wq, need_wk, _ = ctx.needs_input_grad
+        dq, dk, dwq, dwk = _C.qk_norm_rope_bwd(gq, gk, ctx.saved_tensors, ctx.layout, need_wq or need_wk)
+        if ctx.cast is not None and dwq is not None:
+            dwq, dwk = dwq.to(ctx.cast[0]), dwk.to(ctx.cast[1])
+        return (dq if need_q else None, dk if need_k else None, dwq if need_wq else None, dwk if need_wk else None, None)
 
 
 class _SwiGLUFn(Function):

@@ -35,7 +35,6 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 import voodoo_quant
 from voodoo_quant import _C
@@ -723,14 +722,17 @@ class _GatedEmbeddingFunction(Function):
                 vocab_start: int | None, dtype: torch.dtype):
         plan = _C.embed_plan(ids, table.rows, vocab_start)
         ctx.save_for_backward(plan)
-        ctx.table, ctx.scale, ctx.like = table, scale, (probs.dtype, probs.shape)  # the candidates are constants
+        ctx.table, ctx.scale = table, scale  # the candidates are constants
+        ctx.like = None if probs.dtype == torch.float32 and probs.dim() == 1 else (probs.dtype, probs.shape)
         return _embedding_rows(probs, ids, table, scale, vocab_start, dtype, plan)
 
     @staticmethod
-    @once_differentiable
+    @_C.first_order
     def backward(ctx, g: torch.Tensor):
         gp = _C.embed_gategrad(g, ctx.table, ctx.saved_tensors[0], ctx.scale)
-        return gp.to(ctx.like[0]).view(ctx.like[1]), None, None, None, None, None
+        if ctx.like is not None:
+            gp = gp.to(ctx.like[0]).view(ctx.like[1])
+        return gp, None, None, None, None, None
 
 
 def _embedding_rows(probs, ids, table, scale, vocab_start, dtype, plan=None):
