@@ -20,6 +20,7 @@ from operator import attrgetter
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 LIB_NAME = "libvoodoo_b200.so"
@@ -165,6 +166,15 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+def no_tangents(what: str, *ts: torch.Tensor) -> None:
+    """Refuses forward-mode duals, whose tangents a kernel that gets the values' pointers would lose without a word.
+    (An autograd function without a ``jvp`` refuses them itself, but only where one is applied.)"""
+    if forward_ad._current_level >= 0:  # some level is open: rarely
+        for t in ts:
+            if forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{what}: no forward-mode derivative (a tensor carries a tangent)")
+
+
 def first_order(backward):
     """``once_differentiable`` for a Function's backward, without its bookkeeping where no graph of the gradients is
     built (7 us of the 140 of a short forward and backward: the engine's thread finds the interpreter's data cold)."""
@@ -172,6 +182,7 @@ def first_order(backward):
 
     @functools.wraps(backward)
     def run(ctx, *grads):
+        no_tangents("backward", *grads)
         return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
 
     return run
@@ -880,6 +891,7 @@ def clip_grad_norm(tensors, max_norm: float = float("inf"), norm_inf: bool = Fal
     n = len(tensors)
     if n == 0:
         raise ValueError("clip_grad_norm: no tensors")
+    no_tangents("clip_grad_norm", *tensors)
     # one pass per property: a few hundred short tensors cost more here than on the GPU
     dev = _device_of(tensors[0])
     if set(map(torch.Tensor.get_device, tensors)) != {dev}:

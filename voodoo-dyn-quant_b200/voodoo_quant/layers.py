@@ -749,7 +749,7 @@ def gated_embedding(ids: torch.Tensor, probs: torch.Tensor, candidate_types, can
                     dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``scale`` times the rows of sum_k probs[k] W_k that the token ``ids`` (int64 or int32, any shape) name, for a
     table whose K candidates are packed GGUF blocks (uint8, rows padded to a multiple of 256 weights):
-    [*ids.shape, embedding_dim] in ``dtype``.  Differentiable in ``probs``.
+    [*ids.shape, embedding_dim] in ``dtype``.  Differentiable in ``probs`` (not in forward mode: a tangent is refused).
 
     ``vocab_start``: the table is the vocabulary shard of ``num_embeddings`` rows from there on; tokens of other shards
     get zeros and add nothing to the gradient.  Without it every id must be a row of the table: another one gets zeros
@@ -758,6 +758,7 @@ def gated_embedding(ids: torch.Tensor, probs: torch.Tensor, candidate_types, can
         raise ValueError(f"gated_embedding: float32, bfloat16 or float16 rows, got {dtype}")
     if vocab_start is not None and vocab_start < 0:
         raise ValueError(f"gated_embedding: vocab_start {vocab_start} is negative")
+    _C.no_tangents("gated_embedding", probs)
     table = _C.EmbedTable(candidate_types, candidate_blocks, num_embeddings, _padded(embedding_dim), embedding_dim)
     scale = float(scale)
     if not (probs.requires_grad and torch.is_grad_enabled()):

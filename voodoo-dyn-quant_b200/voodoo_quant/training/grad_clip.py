@@ -72,7 +72,7 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0,
     min(1, max_norm / (norm + 1e-6)), a norm that is not finite included (NaN gives NaN, inf gives zeros and NaN).
     An infinite ``max_norm`` leaves the gradients as they are.  ``error_if_nonfinite`` reads the norm on the host and
     raises RuntimeError before anything is scaled.  Parameters without a gradient are skipped; ``norm_type`` 2 or inf;
-    gradients that share memory are refused."""
+    gradients that share memory, or carry forward-mode tangents, are refused."""
     params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     grads = [g for g in [p.grad for p in params] if g is not None]
     max_norm = float(max_norm)
