@@ -56,6 +56,10 @@ int vq_format_info(int ggml_type, int* block_elems /* host */, int* block_bytes 
  * for another number of tokens or rows. */
 int vq_device_error(void* stream, int* code /* host */);
 
+/* Enqueue a copy of the error word of the device that `code` is on behind the
+ * work on `stream`; neither waits nor clears the word. */
+int vq_device_error_async(int* code /* device */, void* stream);
+
 /* K0 -- bit-exact dequantisation of one packed candidate into float32
  * out[rows, cols] (cols = padded in_features, a multiple of the block size).
  * Replaces dequantize_tensor_gpu, voodoo_quant/layers.py:298-319 (per-format

@@ -352,6 +352,15 @@ int vq_device_error(void* stream, int* code) {
   return 0;
 }
 
+int vq_device_error_async(int* code, void* stream) {
+  if (code == nullptr) return fail(VQ_ERR_INVALID, "null pointer");
+  DeviceScope scope(code);
+  int* dp = nullptr;
+  if (int rc = device_error_ptr(&dp)) return rc;
+  VQ_CUDA(cudaMemcpyAsync(code, dp, sizeof(int), cudaMemcpyDeviceToDevice, static_cast<cudaStream_t>(stream)));
+  return 0;
+}
+
 int vq_dequant(int ggml_type, const void* blocks, int64_t rows, int64_t cols, float* out, void* stream) {
   DeviceScope scope(out);
   if (!known_format(ggml_type)) return fail(VQ_ERR_UNSUPPORTED, "unsupported ggml type %d", ggml_type);

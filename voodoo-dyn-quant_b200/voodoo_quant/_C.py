@@ -47,6 +47,7 @@ def _declare(lib):
         "vq_abi_version": (_int, []),
         "vq_format_info": (_int, [_int, ctypes.POINTER(_int), ctypes.POINTER(_int)]),
         "vq_device_error": (_int, [_vp, ctypes.POINTER(_int)]),
+        "vq_device_error_async": (_int, [_vp, _vp]),
         "vq_dequant": (_int, [_int, _vp, _i64, _i64, _vp, _vp]),
         "vq_quantize": (_int, [_int, _vp, _int, _i64, _i64, _i64, _vp, _vp]),
         "vq_mix": (_int, [_int, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp]),
@@ -107,7 +108,7 @@ def _declare(lib):
 
 
 EXPORTED = (
-    "vq_last_error", "vq_abi_version", "vq_format_info", "vq_device_error", "vq_dequant", "vq_mix",
+    "vq_last_error", "vq_abi_version", "vq_format_info", "vq_device_error", "vq_device_error_async", "vq_dequant", "vq_mix",
     "vq_linear_fwd", "vq_linear_fwd_swiglu", "vq_linear_fwd_grouped", "vq_set_gategrad_sm_reserve", "vq_set_gemm_sm_reserve", "vq_quantize", "vq_route_prep", "vq_linear_dx", "vq_gategrad_workspace_bytes", "vq_gategrad", "vq_gategrad_noalloc",
     "vq_gategrad_grouped_workspace_bytes", "vq_gategrad_grouped",
     "vq_mixgemm_fwd", "vq_mixgemm_fwd_fused", "vq_mixgemm_dx",
@@ -245,6 +246,47 @@ def device_error(device: torch.device | None = None) -> int:
     st = torch.cuda.current_stream(device).cuda_stream
     _check(lib.vq_device_error(st, ctypes.byref(code)))
     return code.value
+
+
+_ERROR_TEXT = {1: "a kernel gave up waiting", 2: "unknown block format", 3: "misaligned shared memory",
+               4: "token id outside the embedding table", 5: "a lookup met the plan of other token ids"}
+
+
+def device_error_text(code: int) -> str:
+    return f"{_ERROR_TEXT.get(code >> 16, 'unknown error')} (device error word {code:#x})"
+
+
+class ErrorWatch:
+    """Reads the devices' error words behind each step's work without making the host wait for that step: ``poll``
+    raises what the kernels up to the poll before it reported, ``check`` what all of them did.  The word is cleared."""
+
+    def __init__(self, devices):
+        self._devices = [torch.device(d) for d in devices]
+        self._pending = []  # (word on the host, event behind its copy) of the poll before
+
+    def poll(self) -> None:
+        before, self._pending = self._pending, []
+        for d in self._devices:
+            with torch.cuda.device(d):
+                word = torch.empty(1, dtype=torch.int32, device=d)
+                _check(load_library().vq_device_error_async(word.data_ptr(), _raw_stream(d.index)))
+                word, event = word.to("cpu", non_blocking=True), torch.cuda.Event()
+                event.record()
+                self._pending.append((word, event))
+        for word, event in before:
+            event.synchronize()
+            if int(word):
+                self.check()
+
+    def check(self) -> None:
+        self._pending = []
+        codes = {}
+        for d in self._devices:
+            with torch.cuda.device(d):
+                codes[d] = device_error()
+        for d, code in codes.items():
+            if code:
+                raise RuntimeError(f"{d}: {device_error_text(code)}")
 
 
 def quantize(w: torch.Tensor, qtype: str) -> torch.Tensor:

@@ -133,6 +133,7 @@ class GatedDistillTrainer:
         self.scheduler = torch.optim.lr_scheduler.CosineAnnealingLR(self.optimizer, T_max=args.max_steps,
                                                                     eta_min=1e-3)
         self.step_idx = 0
+        self._watch = None
         student.train()
         teacher.eval()
 
@@ -351,6 +352,22 @@ class GatedDistillTrainer:
         self.optimizer.step()
         self.scheduler.step()
         self.step_idx += 1
+        self._errors().poll()
+
+    def _errors(self):
+        """Watch over the error words of the devices that the models' kernels run on."""
+        if self._watch is None:
+            from voodoo_quant._C import ErrorWatch
+
+            on = {t.device for m in (self.student, self.teacher) for t in (*m.parameters(), *m.buffers())}
+            self._watch = ErrorWatch(sorted((d for d in on if d.type == "cuda"), key=str))
+        return self._watch
+
+    def check_device(self) -> None:
+        """Wait for the steps so far and raise RuntimeError if a kernel reported an error: a token id outside the
+        vocabulary (whose embedding is a row of zeros), a wait that ran out.  ``apply_update`` raises it too, a step
+        late, so that the host need not wait for the step at hand."""
+        self._errors().check()
 
     def step(self, x: torch.Tensor, y: torch.Tensor) -> dict:
         out = self.forward_backward(x, y)
@@ -411,6 +428,7 @@ class GatedDistillTrainer:
         self._gout = None
 
     def assignments(self) -> dict[str, str]:
+        self.check_device()
         return {name: layer.get_assignment() for name, layer in self.replaced.items()}
 
 
