@@ -363,7 +363,7 @@ int vq_qk_norm_rope_bwd(const void* gq, const int64_t* gq_strides, const void* g
  * rows and at most 8 tokens (one begins at every 1024th place).  `plan` (vq_embed_plan_bytes(T), 16-byte aligned)
  * holds int32: the number of pieces P, T and `rows` at byte 0; order[T] from byte 256; then, each from a multiple of
  * 256 bytes, start[P] with T behind the last, and the pieces' rows key[P] (`rows` for ids outside the table).  A
- * lookup or gradient of another T or `rows` reports the plan (vq_device_error) and takes no token of it. */
+ * lookup or gradient of another T or `rows` reports the plan (vq_device_error) and takes no token of it: zeros. */
 size_t vq_embed_plan_bytes(int64_t T);
 int vq_embed_plan(const void* ids, int ids_i32, int64_t T, int64_t vocab_start, int64_t rows, void* plan,
                   size_t plan_bytes, void* stream);

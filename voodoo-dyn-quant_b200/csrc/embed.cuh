@@ -261,7 +261,13 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
   const int lu = lane >> 3, c = lane & 7;
   uint8_t* buf = esmem + kWarps * kUnits * 512 + warp * cs.warp_bytes;
   uint4* rows_s = reinterpret_cast<uint4*>(esmem + (warp * kUnits + lu) * 512);
-  UnitWalk<kRuns> w{plan, ids, kRuns ? plan.pieces(T, rows, err) : T, vocab_start, rows, units_per_row};
+  const int count = kRuns ? plan.pieces(T, rows, err) : T;
+  if (kRuns && count == 0) {  // another call's plan (T > 0 tokens have a piece): zeros, not what the memory held
+    for (int t = blockIdx.x; t < T; t += gridDim.x)
+      for (int j = threadIdx.x; j < cols; j += kThreads) out[t * ldo + j] = __float2bfloat16_rn(0.f);
+    return;
+  }
+  UnitWalk<kRuns> w{plan, ids, count, vocab_start, rows, units_per_row};
   w.start_at((static_cast<long long>(blockIdx.x) * kWarps + warp) * kUnits + lu,
              static_cast<long long>(gridDim.x) * kWarps * kUnits);
   bool bad = false;
