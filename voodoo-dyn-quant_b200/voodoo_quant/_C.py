@@ -860,6 +860,12 @@ class EmbedTable:
                 _require_cuda(*ts)
                 raise ValueError(f"tensors on cuda:{self.device} expected, got {t.device}")
 
+    def check_plan(self, plan: torch.Tensor) -> None:
+        self.check(plan)
+        if plan.dtype != torch.uint8 or not plan.is_contiguous():
+            raise ValueError(f"a plan as embed_plan made it expected, got {plan.dtype} {tuple(plan.shape)} with strides "
+                             f"{plan.stride()}")
+
 
 def embed_plan(ids: torch.Tensor, rows: int, vocab_start: int | None = None) -> torch.Tensor:
     """Plan of the token ids over a table of ``rows`` rows (uint8, its layout is the C header's): the tokens sorted by
@@ -882,6 +888,8 @@ def embed_mix(ids: torch.Tensor, table: EmbedTable, probs: torch.Tensor, scale: 
     up to 8 tokens that name it, else once per token."""
     table.check(ids, probs)
     ids = _ids_operand(ids)
+    if plan is not None:
+        table.check_plan(plan)
     if probs.numel() != table.K:
         raise ValueError(f"{table.K} probabilities expected, got {tuple(probs.shape)}")
     if probs.dtype != torch.float32 or not probs.is_contiguous():
@@ -898,7 +906,8 @@ def embed_mix(ids: torch.Tensor, table: EmbedTable, probs: torch.Tensor, scale: 
 def embed_gategrad(dy: torch.Tensor, table: EmbedTable, plan: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     """grad[k] = scale * sum_t <dy[t], W_k[ids[t]]> (float32 [K]) for dy [..., cols] in float32, bfloat16 or float16 and
     the plan of its ids; ids outside the table add nothing."""
-    table.check(dy, plan)
+    table.check(dy)
+    table.check_plan(plan)
     K, cols = table.K, table.cols
     code = _float_code(dy, "embed_gategrad")
     if dy.dim() < 1 or dy.shape[-1] != cols:
