@@ -177,11 +177,21 @@ __device__ __forceinline__ void async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Shared memory of a block: kDepth steps of every thread's own values.
+// Shared memory of a block: kDepth steps of every thread's own values, and for
+// a weight gradient each warp's sums of g * n by column.
 template <typename T, bool kGrad>
-constexpr int ring_bytes() {
-  return kDepth * (kGrad ? 4 : 2) * 8 * static_cast<int>(sizeof(T)) * kThreads;
-}
+constexpr int kRingBytes = kDepth * (kGrad ? 4 : 2) * 8 * static_cast<int>(sizeof(T)) * kThreads;
+constexpr int sums_bytes(int D) { return kWarps * D * static_cast<int>(sizeof(double)); }
+// Largest D of which three blocks with the ring of float32 heads fit an SM;
+// above, the launch is planned for the two that do (16 + 4 heads of 448,
+// 6144 positions: 204 us, planned for three 203; 10240: 319 and 355; 4 + 4
+// heads of 512, 10240 positions: 142 and 157).
+constexpr int kThreeBlockDim = 352;
+
+// Steps after which a lane's sums of g * n, held in 32 bits, go to its warp's
+// in 64: summed in 32 bits to the end their error grew with the batch (1.6e-7
+// of the result at 16384 positions, 1e-6 at a million).
+constexpr int kFlushSteps = 32;
 
 // What both kernels share: the lane's places in a head, and its walk over
 // the items (position, piece of its heads) of its side.  A thread copies the
@@ -403,7 +413,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(TC) == 4 ? kFwdBlocksWide : k
 }
 
 // Backward, on the same items.  kWeights: also leave this block's sum of
-// g * n, of its side's weight gradient, in partials[blockIdx.x][D].
+// g * n, of its side's weight gradient, in partials[blockIdx.x][D].  A lane
+// adds at most kFlushSteps - 1 and one item's steps in 32 bits.
 template <typename T, typename TC, bool kWeights, int kTeam>
 __global__ void __launch_bounds__(kThreads, sizeof(TC) == 4 ? kBwdBlocksWide : kBwdBlocks)
     qk_norm_rope_bwd_kernel(const __grid_constant__ Side<T> q, const __grid_constant__ Side<T> k,
@@ -421,6 +432,30 @@ __global__ void __launch_bounds__(kThreads, sizeof(TC) == 4 ? kBwdBlocksWide : k
     w1 = weights<T>(side.w, sh.w_f32, w.a, sh.offset);
     w2 = weights<T>(side.w, sh.w_f32, w.b, sh.offset);
   }
+  // this warp's sums; a column is the first team's lane's that holds it
+  double* sums = reinterpret_cast<double*>(qsmem + kRingBytes<T, true>) + (threadIdx.x >> 5) * sh.D;
+  const bool keeps = w.slot == 0 && w.live;
+  if (kWeights && keeps) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sums[w.a + j] = sums[w.b + j] = 0.0;
+  }
+  auto flush = [&] {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      for (int o = 1 << w.team_log2; o < 32; o <<= 1) {
+        dw1.v[j].x += __shfl_xor_sync(0xffffffffu, dw1.v[j].x, o);
+        dw1.v[j].y += __shfl_xor_sync(0xffffffffu, dw1.v[j].y, o);
+        dw2.v[j].x += __shfl_xor_sync(0xffffffffu, dw2.v[j].x, o);
+        dw2.v[j].y += __shfl_xor_sync(0xffffffffu, dw2.v[j].y, o);
+      }
+      if (keeps) {
+        sums[w.a + 2 * j] += dw1.v[j].x, sums[w.a + 2 * j + 1] += dw1.v[j].y;
+        sums[w.b + 2 * j] += dw2.v[j].x, sums[w.b + 2 * j + 1] += dw2.v[j].y;
+      }
+      dw1.v[j] = dw2.v[j] = both(0.f);
+    }
+  };
+  int steps = 0;
   bool more = w.at.item < w.items;
   while (more) {
     const unsigned bi = w.at.b, si = w.at.s;
@@ -483,33 +518,20 @@ __global__ void __launch_bounds__(kThreads, sizeof(TC) == 4 ? kBwdBlocksWide : k
       h += w.per_warp;
       op += ostep;
     }
+    if (kWeights && (steps += w.iters) >= kFlushSteps) {
+      flush();
+      steps = 0;
+    }
   }
   if (kWeights) {
-    // the same column lives in this lane's place of every team of every warp
-    __shared__ float red[kWarps][kMaxDim];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      for (int o = 1 << w.team_log2; o < 32; o <<= 1) {
-        dw1.v[j].x += __shfl_xor_sync(0xffffffffu, dw1.v[j].x, o);
-        dw1.v[j].y += __shfl_xor_sync(0xffffffffu, dw1.v[j].y, o);
-        dw2.v[j].x += __shfl_xor_sync(0xffffffffu, dw2.v[j].x, o);
-        dw2.v[j].y += __shfl_xor_sync(0xffffffffu, dw2.v[j].y, o);
-      }
-    }
-    if (w.slot == 0 && w.live) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float* r = red[threadIdx.x >> 5];
-        r[w.a + 2 * j] = dw1.v[j].x, r[w.a + 2 * j + 1] = dw1.v[j].y;
-        r[w.b + 2 * j] = dw2.v[j].x, r[w.b + 2 * j + 1] = dw2.v[j].y;
-      }
-    }
+    flush();
     __syncthreads();
+    const double* all = reinterpret_cast<const double*>(qsmem + kRingBytes<T, true>);
     for (int c = threadIdx.x; c < sh.D; c += kThreads) {
-      float t = 0.f;
+      double t = 0.0;
 #pragma unroll
-      for (int v = 0; v < kWarps; ++v) t += red[v][c];
-      partials[static_cast<long long>(blockIdx.x) * sh.D + c] = t;
+      for (int v = 0; v < kWarps; ++v) t += all[v * sh.D + c];
+      partials[static_cast<long long>(blockIdx.x) * sh.D + c] = static_cast<float>(t);
     }
   }
 }

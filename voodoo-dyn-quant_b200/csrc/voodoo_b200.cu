@@ -1261,10 +1261,11 @@ int launch_qk(const QkArgs& a, const QkPlan& p, float* partials, cudaStream_t st
   sh.eps = a.eps, sh.offset = a.offset;
   sh.w_f32 = a.w_f32;
   const int grid = p.q_blocks + p.k_blocks;
-  constexpr int smem = ring_bytes<T, kBackward>();
+  constexpr int ring = kRingBytes<T, kBackward>, most = ring + (kBackward ? sums_bytes(kMaxDim) : 0);
+  const int smem = ring + (kBackward && partials != nullptr ? sums_bytes(sh.D) : 0);
   auto start = [&](auto kern, auto... more) {
     cudaError_t e = cudaSuccess;
-    if (smem > 32 * 1024) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (smem > 48 * 1024) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e == cudaSuccess) kern<<<grid, kThreads, smem, st>>>(q, k, sh, more...);
     return e;
   };
@@ -1353,7 +1354,9 @@ int vq_qk_norm_rope_bwd(const void* gq, const int64_t* gq_strides, const void* g
     return fail(VQ_ERR_INVALID, "workspace of %zu bytes needed for the weight gradients", vq_qk_norm_rope_workspace_bytes(D));
   QkPlan p;
   if (int rc = qk_plan(&p, B * S, Hq, Hk, D,
-                       cs_f32 || dtype == 0 ? vq::qknorm::kBwdBlocksWide : vq::qknorm::kBwdBlocks))
+                       want_dw && dtype == 0 && D > vq::qknorm::kThreeBlockDim ? 2
+                       : cs_f32 || dtype == 0                                  ? vq::qknorm::kBwdBlocksWide
+                                                                               : vq::qknorm::kBwdBlocks))
     return rc;
   const QkArgs a{q,  k,  gq, gk, q_weight, k_weight, cos, sin, q_strides, k_strides, gq_strides, gk_strides, cs_strides,
                  Hq, Hk, B,  S,  D,        R,        weight_f32 != 0, cs_f32 != 0, eps, weight_offset, dq, dk};
