@@ -1,6 +1,9 @@
-"""The head norms' weight gradient where many terms meet in one lane."""
+"""The head norms' weight gradient where many terms meet in one lane, and where some of a step's
+lanes hold no head."""
 
 from __future__ import annotations
+
+import math
 
 import pytest
 import torch
@@ -33,3 +36,27 @@ def test_long_sums_keep_their_bits(cuda):
         want = r * (r.square().mean() + 1e-6).rsqrt() * (S * H)
         off = ((got.double() - want).abs() / want).max()
         assert off <= 64 * ULP, f"{off / ULP:.0f} roundings of 2^-24"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_an_infinite_gradient_of_the_last_head(cuda, dtype):
+    """5 heads of 128, four to a step: the lanes past the last head read it again and must add nothing of it, not even
+    infinity times 0."""
+    from voodoo_quant.fused_blocks import qk_norm_rope
+
+    S, H, D, R = 3, 5, 128, 32
+    g = torch.Generator(device="cpu").manual_seed(9)
+    q, k, gq, gk = (torch.randn(1, S, H, D, generator=g).to(dtype).to(cuda) for _ in range(4))
+    q[0, 1, H - 1, 100] = 0.5
+    w = torch.ones(D, dtype=dtype, device=cuda, requires_grad=True)
+    cos, sin = (torch.randn(1, S, R, generator=g).to(dtype).to(cuda) for _ in range(2))
+
+    def grad(gq):
+        return torch.autograd.grad(qk_norm_rope(q, k, w, w.detach(), cos, sin), w, (gq, gk))[0]
+
+    clean = grad(gq)
+    gq[0, 1, H - 1, 100] = math.inf
+    bad = grad(gq)
+    rest = torch.arange(D, device=cuda) != 100
+    assert torch.isfinite(clean).all() and torch.equal(bad[rest], clean[rest])
+    assert float(bad[100]) == math.inf

@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(TC) == 4 ? kBwdBlocksWide : k
       w.leave();
       const float ss = w.live ? sum_squares(n1, n2) : 0.f;
       const float r = rsqrtf(fmaf(team_sum<kTeam>(ss, w.team_log2), inv_d, eps));
-      const float rw = h < w.H ? r : 0.f;  // a team past the last head adds nothing to the weights' sum
+      const bool counts = h < w.H;  // a team past the last head adds nothing to the weights' sum, not even inf * 0
       if (w.turned) {
         c1r.stay(), c2r.stay(), s1r.stay(), s2r.stay();
         const F8 c1 = widen(c1r), c2 = widen(c2r), s1 = widen(s1r), s2 = widen(s2r);
@@ -494,9 +494,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(TC) == 4 ? kBwdBlocksWide : k
       float2 dot = both(0.f);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        n1.v[j] = __fmul2_rn(n1.v[j], both(rw));
-        n2.v[j] = __fmul2_rn(n2.v[j], both(rw));
-        if (kWeights) {
+        n1.v[j] = __fmul2_rn(n1.v[j], both(r));
+        n2.v[j] = __fmul2_rn(n2.v[j], both(r));
+        if (kWeights && counts) {
           dw1.v[j] = __ffma2_rn(g1.v[j], n1.v[j], dw1.v[j]);
           dw2.v[j] = __ffma2_rn(g2.v[j], n2.v[j], dw2.v[j]);
         }
