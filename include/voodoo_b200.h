@@ -372,7 +372,8 @@ int vq_embed_plan(const void* ids, int ids_i32, int64_t T, int64_t vocab_start, 
  * candidates of a table of `rows` rows of padded_cols weights.  With a plan of the ids each row is decoded once per
  * piece (ids itself is not read); without (plan NULL) once per token.  An id outside [vocab_start, vocab_start + rows)
  * gives a row of zeros (a token of another vocabulary shard); with `strict` it also sets the device error word
- * (4 << 16 | 30).  For scale 1 the rows are vq_mix's bit for bit.  Replaces the gather, decode and mixture of
+ * (4 << 16 | 30).  For scale 1 the rows are vq_mix's bit for bit; a scale
+ * that is not finite is refused.  Replaces the gather, decode and mixture of
  * _MixedEmbeddingRowFunctionLazy, voodoo_quant/layers.py:670-750, and Q8Embedding's, training/q8_teacher.py:156-173. */
 int vq_embed_mix(int K, const int* types, const void* const* blocks, const float* probs, const void* ids, int ids_i32,
                  int64_t T, const void* plan, size_t plan_bytes, int64_t vocab_start, int64_t rows, int64_t padded_cols,

@@ -1,7 +1,10 @@
-"""What the Python calls of the gated embedding refuse of a plan and of its companions, before the library sees a pointer;
+"""What the Python calls of the gated embedding refuse of a plan and a factor, before anything is launched;
 the library is replaced, no GPU needed."""
 
 from __future__ import annotations
+
+import ctypes
+import math
 
 import pytest
 import torch
@@ -57,3 +60,18 @@ def test_the_plans_device_is_checked(table):
         with pytest.raises(AssertionError, match="was reached"):
             call()
         assert any(s is plan for s in seen)
+
+
+@pytest.mark.parametrize("scale", [math.inf, -math.inf, math.nan, 1e39])
+def test_a_scale_that_is_not_finite(scale):
+    """Rows of other shards' tokens and of no token are zeros, which such a factor would turn into NaN."""
+    from voodoo_quant import _C
+
+    lib = _C.load_library()
+    types, blocks = (ctypes.c_int * 1)(8), (ctypes.c_void_p * 1)(1 << 20)
+    one = 1 << 20  # stands for an aligned address that the checks never read
+    need = lib.vq_embed_gategrad_workspace_bytes(1)
+    for rc in (lib.vq_embed_mix(1, types, blocks, one, one, 0, 4, None, 0, 0, 10, 256, 256, scale, 1, one, 256, None),
+               lib.vq_embed_gategrad(1, types, blocks, one, lib.vq_embed_plan_bytes(4), 4, 10, 256, 256, scale, one, 256, 1,
+                                     one, need - 1, one, None)):
+        assert rc == -1 and "scale" in lib.vq_last_error().decode()

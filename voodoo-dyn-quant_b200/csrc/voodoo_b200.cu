@@ -1396,7 +1396,8 @@ int build_table(vq::embed::Cands* out, int K, const int* types, const void* cons
   return 0;
 }
 
-int check_table(int64_t T, int64_t vocab_start, int64_t rows, int64_t padded_cols, int64_t cols) {
+int check_table(int64_t T, int64_t vocab_start, int64_t rows, int64_t padded_cols, int64_t cols, float scale) {
+  if (!std::isfinite(scale)) return fail(VQ_ERR_INVALID, "scale must be finite");  // rows of no token are 0 * scale
   if (T < 0 || rows < 0 || cols < 0 || vocab_start < 0) return fail(VQ_ERR_INVALID, "negative shape or vocabulary start");
   if (padded_cols < cols || padded_cols % 256 != 0)
     return fail(VQ_ERR_INVALID, "padded columns %lld must be a multiple of 256 that holds %lld", (long long)padded_cols,
@@ -1533,7 +1534,7 @@ int vq_embed_mix(int K, const int* types, const void* const* blocks, const float
   DeviceScope scope(out);
   vq::embed::Cands cs;
   if (int rc = build_table(&cs, K, types, blocks)) return rc;
-  if (int rc = check_table(T, vocab_start, rows, padded_cols, cols)) return rc;
+  if (int rc = check_table(T, vocab_start, rows, padded_cols, cols, scale)) return rc;
   if (int rc = check_matrix(out, T, cols, ldo, "out")) return rc;
   if (T == 0 || cols == 0) return 0;
   if (probs == nullptr) return fail(VQ_ERR_INVALID, "null pointer");
@@ -1569,7 +1570,7 @@ int vq_embed_gategrad(int K, const int* types, const void* const* blocks, const 
   DeviceScope scope(grad);
   vq::embed::Cands cs;
   if (int rc = build_table(&cs, K, types, blocks)) return rc;
-  if (int rc = check_table(T, 0, rows, padded_cols, cols)) return rc;
+  if (int rc = check_table(T, 0, rows, padded_cols, cols, scale)) return rc;
   if (int rc = check_matrix(dy, T, cols, lddy, "dy")) return rc;
   if (dy_dtype < 0 || dy_dtype > 2) return fail(VQ_ERR_INVALID, "dtype %d (0 = float32, 1 = bfloat16, 2 = float16)", dy_dtype);
   if (grad == nullptr) return fail(VQ_ERR_INVALID, "null pointer");

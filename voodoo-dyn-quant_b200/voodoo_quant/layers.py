@@ -747,7 +747,7 @@ _ROW_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 def gated_embedding(ids: torch.Tensor, probs: torch.Tensor, candidate_types, candidate_blocks, num_embeddings: int,
                     embedding_dim: int, scale: float = 1.0, vocab_start: int | None = None,
                     dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """``scale`` times the rows of sum_k probs[k] W_k that the token ``ids`` (int64 or int32, any shape) name, for a
+    """``scale`` (finite) times the rows of sum_k probs[k] W_k that the token ``ids`` (int64 or int32, any shape) name, for a
     table whose K candidates are packed GGUF blocks (uint8, rows padded to a multiple of 256 weights):
     [*ids.shape, embedding_dim] in ``dtype``.  Differentiable in ``probs`` (not in forward mode: a tangent is refused).
 
