@@ -184,8 +184,8 @@ constexpr int kRingBytes = kDepth * (kGrad ? 4 : 2) * 8 * static_cast<int>(sizeo
 constexpr int sums_bytes(int D) { return kWarps * D * static_cast<int>(sizeof(double)); }
 // Largest D of which three blocks with the ring of float32 heads fit an SM;
 // above, the launch is planned for the two that do (16 + 4 heads of 448,
-// 6144 positions: 204 us, planned for three 203; 10240: 319 and 355; 4 + 4
-// heads of 512, 10240 positions: 142 and 157).
+// 6144 positions: 208 us, planned for three 205; 10240: 333 and 373; 4 + 4
+// heads of 512, 10240 positions: 141 and 158).
 constexpr int kThreeBlockDim = 352;
 
 // Steps after which a lane's sums of g * n, held in 32 bits, go to its warp's
