@@ -21,9 +21,10 @@ namespace clip {
 constexpr int kThreads = 256;
 constexpr int kChunkBytes = 32768;  // 8 vectors of 16 bytes per thread
 constexpr int kVecs = kChunkBytes / (16 * kThreads);
-// Resident blocks per SM of the two passes (0.59 G bf16 values: the norm takes
-// 167 us with 4, 171 with 3, 206 with 6; the scaling 407 us with 3, 411 with
-// 4, 490 with 1).
+// Resident blocks per SM of the two passes.  0.59 G bf16 values: the norm takes
+// 167 us with 4, 171 with 3, 204 with 6, and behind a pass that scaled, whose
+// last writes are still on their way to memory, 195, 188 and 211; the scaling
+// 382 us with 3, 388 with 4, 371 with 2, 462 with 1.
 constexpr int kBlocksPerSm = 4, kScaleBlocksPerSm = 3;
 constexpr int kSmallThreads = 1024;
 constexpr int kSmallChunkBytes = 512;
@@ -32,7 +33,8 @@ constexpr int kMaxBlocks = 1024;  // of one launch: the partials it leaves
 enum DType : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
 
 // The parameter space of a launch is 32764 bytes; the short table serves the
-// usual few hundred tensors without copying all of it on every launch.
+// usual few hundred tensors without copying all of it on every launch (226 of
+// six values: 4.9 us on the device, with the long table 5.1).
 constexpr int kShortTable = 240;
 constexpr int kLongTable = 1536;
 
@@ -116,7 +118,8 @@ __device__ __forceinline__ double one(float f) {
 }
 
 // A vector's share.  The squares of a vector are summed in fp32, which holds
-// them to 2^-22, and joined in 64 bits; where that sum leaves the range that
+// them to 2^-21 (eight sums, each rounded by 2^-24 at most), and joined in 64
+// bits; where that sum leaves the range that
 // fp32 squares keep their precision in, it is taken in 64 bits instead.
 template <bool kMax, int kType>
 __device__ __forceinline__ double of_vec(const uint4& v) {
@@ -229,8 +232,8 @@ __device__ __forceinline__ void scale_chunk(const Chunk& c, float s) {
 #pragma unroll
     for (int j = 0; j < kVecs; ++j) {
       const uint4 w = Values<kType>(v[j]).scaled(s);
-      // a factor just below 1 leaves most 16-bit values as they are: not written (0.59 G bf16 values and a factor of
-      // 0.999: 338 us the two passes, 550 when written; 550 either way for 0.9)
+      // Not written where no value changed, as for 16-bit values and a factor within about 2^-9 of 1 (0.59 G bf16
+      // values, both passes: 577 us for 0.9 either way; a factor that changes no value 330, not 577)
       if (((w.x ^ v[j].x) | (w.y ^ v[j].y) | (w.z ^ v[j].z) | (w.w ^ v[j].w)) != 0) p[j * kThreads] = w;
     }
     return;

@@ -11,7 +11,7 @@
 // sum as it decodes them.  What they cannot do without is the packed rows and
 // T x D of out or dy (16384 x 4096 of text, six candidates: 35 us of HBM each);
 // the decoding bounds them, 220 to 330 instructions for 32 weights of a
-// candidate (63 us the lookup, 71 us the gradient).
+// candidate (63 us the lookup, 75 us the gradient).
 //
 // Eight lanes hold a unit (256 weights) of a row, a lane 32 consecutive
 // weights.  The lanes of a unit copy its packed bytes of every candidate into
@@ -31,8 +31,8 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kUnits = 4;  // units of a warp
 // Resident blocks per SM, and so 72 registers a thread: decoding waits for its
 // own results, so warps count, until they spill (16384 x 4096 text, six
-// candidates, lookup and gradient: 63 and 71 us with 7, 63 and 76 with 6, 64
-// and 82 with 8; blocks of 256 threads 65 and 75 with 3, 66 and 81 with 4).
+// candidates, lookup and gradient: 63 and 75 us with 7, 63 and 77 with 6, 65
+// and 84 with 8).
 constexpr int kBlocksPerSm = 7;
 constexpr int kMaxBlocks = 1184;  // of a launch: the partials that the gradient leaves
 
@@ -168,9 +168,10 @@ struct Plan {
 
 // Most tokens of a piece: a token that fills much of a batch is then worked
 // on by many warps, each decoding its row again.  8 is what a unit's lanes
-// read in one load; 16 and 32 decode less (16384 tokens of text: 6300 and
-// 5800 pieces, not 7300) but measured 91 and 95 us for the lookup against 88,
-// the warps that got the long pieces ending last.
+// read in one load (16384 tokens of text, six candidates, 6600 rows: 7500
+// pieces, lookup and gradient 63 and 75 us; pieces of 4: 8600, 70 and 76).
+// Longer ones decode less, but the warps that get them end last: when the
+// lookup took 88 us, pieces of 16 and 32 took 91 and 95.
 constexpr int kPieceTokens = 8;
 
 // The units that eight lanes work on one after the other: unit u of piece

@@ -16,9 +16,9 @@
 // D / 16 of a head that is no power of two carry nothing.  Arithmetic is fp32
 // from the load to the one rounding of the store.
 //
-// 16384 positions x 40 heads of 128 in bf16: forward 56.5 us (5.9 TB/s),
-// backward with the weights' gradients 89 us (5.7 TB/s); 16384 x 24: 35 and
-// 51 us (5.8 and 5.9 TB/s).  A plain copy of that size reaches 6.5.
+// 16384 positions x 40 heads of 128 in bf16: forward 57 us (5.9 TB/s),
+// backward with the weights' gradients 90 us (5.6 TB/s); 16384 x 24: 35 and
+// 52 us (5.8 and 5.8 TB/s).  A plain copy of that size reaches 6.5.
 #pragma once
 
 #include "common.cuh"
@@ -29,7 +29,10 @@ namespace qknorm {
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxDim = 512;  // 32 lanes of 16 values
-constexpr int kDepth = 4;  // steps of the ring: one being computed, the others on their way (8 a backward: 122 us, not 92)
+// Steps of the ring: one being computed, the others on their way (16384
+// positions, forward and backward of 32 + 8 heads of 128: 57 and 90 us, with 2
+// 55 and 88, with 8 54 and 99; of 16 + 8: 35 and 52, 35 and 55, 38 and 67).
+constexpr int kDepth = 4;
 // Resident blocks per SM; fp32 heads or tables take twice the registers.
 constexpr int kFwdBlocks = 6, kBwdBlocks = 4, kFwdBlocksWide = 4, kBwdBlocksWide = 3;
 // Blocks of one launch at most: the rows of the weight-gradient partials.

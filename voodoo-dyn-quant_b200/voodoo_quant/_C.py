@@ -167,7 +167,7 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-def no_tangents(what: str, *ts: torch.Tensor) -> None:
+def no_tangents(what: str, ts) -> None:
     """Refuses forward-mode duals, whose tangents a kernel that gets the values' pointers would lose without a word.
     (An autograd function without a ``jvp`` refuses them itself, but only where one is applied.)"""
     if forward_ad._current_level >= 0:  # some level is open: rarely
@@ -183,7 +183,7 @@ def first_order(backward):
 
     @functools.wraps(backward)
     def run(ctx, *grads):
-        no_tangents("backward", *grads)
+        no_tangents("backward", grads)
         return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
 
     return run
@@ -942,7 +942,7 @@ def clip_grad_norm(tensors, max_norm: float = float("inf"), norm_inf: bool = Fal
     n = len(tensors)
     if n == 0:
         raise ValueError("clip_grad_norm: no tensors")
-    no_tangents("clip_grad_norm", *tensors)
+    no_tangents("clip_grad_norm", tensors)
     # one pass per property: a few hundred short tensors cost more here than on the GPU
     dev = _device_of(tensors[0])
     if set(map(torch.Tensor.get_device, tensors)) != {dev}:

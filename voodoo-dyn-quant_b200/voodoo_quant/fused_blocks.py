@@ -192,7 +192,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     unturned), in one pass; contiguous [B, S, H, D] outputs of q's type, rounded once.  q and k in float32, bfloat16
     or float16 with any strides; weights and tables of any of the three.  Differentiable in q, k and the weights (not
     in forward mode: tangents are refused); cos and sin are constants.  D and R are multiples of 16, D up to 512."""
-    _C.no_tangents("qk_norm_rope", q, k, q_weight, k_weight, cos, sin)
+    _C.no_tangents("qk_norm_rope", (q, k, q_weight, k_weight, cos, sin))
     if cos.requires_grad or sin.requires_grad:
         raise ValueError("qk_norm_rope: cos and sin are constants; they cannot require a gradient")
     if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad
